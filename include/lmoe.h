@@ -404,6 +404,93 @@ int lmoe_ep_combine(const float *back, int32_t tokens, int32_t world,
                     const void *residual, void *out, void *normed, float eps,
                     void *stream);
 
+/* ---- Paged key/value cache (no counterpart in the reference, whose dense
+ * backbone and its cache come from oMLX, dsv4_engine.py:22-42).  The cache is
+ * held the way the arena holds experts: stacked arrays indexed by a page id,
+ * rows in the affine format of the expert rows (uint32 codes LSB first, one
+ * scale and bias per group, in the activation dtype), or unquantised.
+ *
+ * One head row x of a token, split into groups of group_size; with n = 2^bits
+ * - 1 and T the activation dtype, each group holds
+ *   bias  = min x,
+ *   scale = T(fp32((max x - min x) / n)), one step of T lower where scale * n
+ *           + bias would exceed the largest finite T,
+ *   code  = clamp(rint((x - bias) / scale), 0, n), 0 where scale is 0,
+ * the quotients as if computed exactly, and stands for T(scale * code +
+ * bias).  A group with an infinity or a NaN holds scale = bias = NaN. */
+typedef struct lmoe_kv_cache {
+    void *k; /* bits 16: dtype [n_pages, kv_heads, page_size, head_dim];
+              * bits 8, 4: uint32 [n_pages, kv_heads, page_size, head_dim * bits / 32] */
+    void *v;
+    void *k_scales; /* dtype [n_pages, kv_heads, page_size, head_dim / group_size]; */
+    void *k_biases; /* NULL when bits is 16 */
+    void *v_scales;
+    void *v_biases;
+    int32_t n_pages;
+    int32_t page_size; /* tokens per page: a multiple of 16 */
+    int32_t kv_heads;
+    int32_t head_dim;   /* 64 or 128 */
+    int32_t dtype;      /* LMOE_BF16 or LMOE_F16 */
+    int32_t bits;       /* 16, 8 or 4 */
+    int32_t group_size; /* 32, 64 or 128, dividing head_dim; not read when bits is 16 */
+} lmoe_kv_cache;
+
+/* The token rows of a call.  Rows row_start[b] .. row_start[b + 1] - 1 are the
+ * last positions of sequence b, whose length with them is lens[b]: row i of
+ * its n_b rows has position lens[b] - n_b + i.  row_start NULL: one row for
+ * each sequence (n_rows == n_seqs).  Position p of sequence b lives in slot
+ * p % page_size of page page_table[b * table_stride + p / page_size].  Rows
+ * at and behind row_start[n_seqs] belong to no sequence and are left alone.
+ * All arrays are on the device and are read by the kernels only; entries of
+ * page_table behind a sequence's last page are not read.  A sequence's rows
+ * with a negative position (lens[b] < n_b) have no place.  Where a page id is
+ * outside [0, n_pages), a position needs an entry at or behind table_width,
+ * lens[b] is negative or row_start is not a non-decreasing run inside [0,
+ * n_rows], the kernels latch LMOE_EINDEX in the workspace's status word and
+ * take that part as absent. */
+typedef struct lmoe_kv_rows {
+    const int32_t *page_table;
+    int64_t table_stride; /* entries between the tables of two sequences */
+    int32_t table_width;  /* entries of one sequence's table */
+    int32_t n_seqs;
+    const int32_t *lens;      /* [n_seqs] */
+    const int32_t *row_start; /* [n_seqs + 1] or NULL */
+    int32_t n_rows;           /* rows of the row arrays */
+} lmoe_kv_rows;
+
+/* Write the rows' keys and values (k, v: dtype [n_rows, kv_heads, head_dim],
+ * strides in elements between tokens and between heads, multiples of 8, data
+ * 16-byte aligned) into their places, quantising them on the way.  Rows
+ * without a place are not written.  No two rows of a call may share a place.
+ * workspace: any lmoe workspace (its status word) or NULL; the same for the
+ * two calls below. */
+int lmoe_kv_append(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, const void *k, int64_t k_token_stride,
+                   int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                   void *workspace, void *stream);
+
+/* Read the rows' keys and values back: k, v [n_rows, kv_heads, head_dim] of
+ * dtype, contiguous, 16-byte aligned.  Rows of a sequence without a place are
+ * zero. */
+int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, void *v, void *workspace,
+                 void *stream);
+
+/* Attention of the rows over their sequences' cached positions (their own
+ * included: append first).  q [n_rows, q_heads, head_dim] of dtype (strides as
+ * above), q_heads a multiple of kv_heads (query head h reads key/value head
+ * h / (q_heads / kv_heads)); out [n_rows, q_heads, head_dim] contiguous, must
+ * not overlap q.  A row at position p sees position j of its sequence if 0 <=
+ * j <= p and (window <= 0 or j > p - window or j < sinks):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,
+ * zero for a row that sees nothing.  What a row does not see does not touch
+ * its result, infinities and NaN included.  Softmax statistics and sums are in
+ * fp32; q, the softmax terms and quantised keys and values enter the products
+ * in dtype.  scratch: lmoe_paged_attention_scratch() bytes, 16-byte aligned,
+ * with no need of initialisation, in use until the call's kernels end. */
+size_t lmoe_paged_attention_scratch(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, int32_t q_heads);
+int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, int32_t q_heads, const void *q,
+                         int64_t q_token_stride, int64_t q_head_stride, float scale, int32_t window, int32_t sinks,
+                         void *out, void *scratch, size_t scratch_bytes, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

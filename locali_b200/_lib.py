@@ -84,6 +84,36 @@ class Layer(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("k_biases", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("v_biases", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+    ]
+
+
+class KVRows(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("lens", ctypes.c_void_p),
+        ("row_start", ctypes.c_void_p),
+        ("n_rows", ctypes.c_int32),
+    ]
+
+
 class LmoeError(RuntimeError):
     def __init__(self, status: int, what: str = ""):
         self.status = status
@@ -145,6 +175,14 @@ _SIGS = {
                          _VP, ctypes.c_int32], ctypes.c_int),
     "lmoe_ep_combine": ([_VP, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _VP, _VP, _VP, _VP,
                          ctypes.c_float, _VP], ctypes.c_int),
+    "lmoe_kv_append": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _VP, ctypes.c_int64, ctypes.c_int64, _VP,
+                        ctypes.c_int64, ctypes.c_int64, _VP, _VP], ctypes.c_int),
+    "lmoe_kv_read": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _VP, _VP, _VP, _VP], ctypes.c_int),
+    "lmoe_paged_attention_scratch": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), ctypes.c_int32],
+                                     ctypes.c_size_t),
+    "lmoe_paged_attention": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), ctypes.c_int32, _VP, ctypes.c_int64,
+                              ctypes.c_int64, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _VP, _VP,
+                              ctypes.c_size_t, _VP, _VP], ctypes.c_int),
 }
 
 CORE_SYMBOLS = [

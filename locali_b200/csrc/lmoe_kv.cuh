@@ -1,0 +1,107 @@
+// Shared by the paged key/value cache's kernels (lmoe_kv.cu) and the
+// attention over it (lmoe_attn.cu): the cache as the kernels see it, where a
+// row's position lives, and the argument structs.
+#pragma once
+
+#include "lmoe_common.cuh"
+
+namespace lmoe {
+
+constexpr int kErrIndex = -3;  // LMOE_EINDEX
+constexpr int kErrCuda = -4;   // LMOE_ECUDA
+
+// Device view of the cache.  All offsets are 64-bit: a long cache passes 2^31
+// elements.
+struct KvView {
+    uint8_t *kv[2];      // keys, values
+    uint16_t *scale[2];  // nullptr when bits is 16
+    uint16_t *bias[2];
+    int32_t n_pages, page_size, kv_heads;
+    int32_t row_bytes;  // bytes of one head row: head_dim * bits / 8
+    int32_t groups;     // groups of one head row
+    int32_t group_size;
+    // row index (of head rows) of a slot in a page
+    __device__ __forceinline__ int64_t row(int32_t page, int32_t head, int32_t slot) const {
+        return ((int64_t)page * kv_heads + head) * page_size + slot;
+    }
+};
+
+struct KvRows {
+    const int32_t *table;
+    int64_t table_stride;
+    int32_t table_width;
+    int32_t n_seqs;
+    const int32_t *lens;
+    const int32_t *row_start;  // nullptr: row b is sequence b's
+    int32_t n_rows;
+    int32_t *err;
+    // first row of sequence b, held inside [0, n_rows]
+    __device__ __forceinline__ int start(int b) const {
+        return row_start ? min(max(row_start[b], 0), n_rows) : b;
+    }
+    // Threads i of n look through the sequences for lengths and row starts
+    // out of range (one block of a launch does).
+    __device__ __forceinline__ void validate(int i, int n) const {
+        for (int b = i; b < n_seqs; b += n) {
+            bool bad = lens[b] < 0;
+            if (row_start) bad |= row_start[b] < 0 || row_start[b + 1] < row_start[b] || row_start[b + 1] > n_rows;
+            if (bad) set_error(err, kErrIndex);
+        }
+    }
+    // the page that holds position p of sequence b, -1 when it has none
+    __device__ __forceinline__ int32_t page(const KvView &c, int b, int p) const {
+        const int e = p / c.page_size;
+        int32_t pg = -1;
+        if (e < table_width) pg = table[(int64_t)b * table_stride + e];
+        if (pg < 0 || pg >= c.n_pages) {
+            set_error(err, kErrIndex);
+            pg = -1;
+        }
+        return pg;
+    }
+    // The sequence that row r belongs to (the last b with start(b) <= r), its
+    // position in *pos; -1 when it belongs to none or has no place.
+    __device__ __forceinline__ int find(int r, int *pos) const {
+        int b = r;
+        if (row_start) {
+            int lo = 0, hi = n_seqs + 1;
+            while (lo < hi) {  // first b in [0, n_seqs] with start(b) > r, else n_seqs + 1
+                const int m = (lo + hi) >> 1;
+                if (start(m) > r) hi = m;
+                else lo = m + 1;
+            }
+            b = lo - 1;
+        }
+        if (b < 0 || b >= n_seqs) return -1;
+        const int p = lens[b] - (start(b + 1) - r);
+        *pos = p;
+        return p < 0 ? -1 : b;
+    }
+};
+
+struct KvCopyArgs {
+    KvView c;
+    KvRows r;
+    const uint16_t *src[2];  // append: new rows
+    int64_t tok_stride[2], head_stride[2];
+    uint16_t *dst[2];  // read: [n_rows, kv_heads, head_dim]
+    int32_t rows_per_block;
+};
+
+struct AttnArgs {
+    KvView c;
+    KvRows r;
+    const uint16_t *q;
+    int64_t q_tok_stride, q_head_stride;
+    uint16_t *out;
+    int32_t q_heads;
+    int32_t group;  // query heads of one key/value head
+    float scale_log2;  // scale * log2(e)
+    int32_t window, sinks;
+    uint8_t *scratch;
+};
+
+cudaError_t launch_attention(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st);
+size_t attention_scratch_bytes(const KvRows &r, int kv_heads, int group, int head_dim);
+
+}  // namespace lmoe
