@@ -26,7 +26,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-r
 
 LMOE_SOURCES = ["lmoe_route.cu", "lmoe_gemv.cu", "lmoe_stream.cu", "lmoe_vec.cu", "lmoe_prefill.cu", "lmoe_ep.cu", "lmoe_api.cu",
                 "lmoe_kv.cu", "lmoe_attn.cu"]
-LMOE_DEPS = LMOE_SOURCES + ["lmoe_common.cuh", "lmoe_kernels.cuh", "lmoe_kv.cuh"]
+LMOE_DEPS = LMOE_SOURCES + ["lmoe_common.cuh", "lmoe_kernels.cuh", "lmoe_kv.cuh", "lmoe_attn.cuh"]
 LMOE_LIB = PKG / "liblmoe.so"
 CORE_LIB = PKG / "liblocali_core.so"
 

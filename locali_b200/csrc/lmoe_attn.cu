@@ -1,104 +1,748 @@
-// Attention of new token rows over the paged key/value cache.
+// Attention of few rows (single tokens, a few drafted tokens) over the paged
+// key/value cache, and the join of tiles cut over several blocks.
 //
-// out = sum_j softmax_j(scale q . k_j) v_j over the positions a row sees, in
-// one pass over the keys with the running maximum and sum of the softmax.
-// One warp per (row, query head); lane l holds elements l, l + 32, ... of the
-// head.
-#include "lmoe_kernels.cuh"
-#include "lmoe_kv.cuh"
+// out = sum_j softmax_j(scale q . k_j) v_j in one pass over the keys with the
+// running maximum and sum of the softmax.  A tile's keys and values are read
+// once, which bounds the kernel: HBM.
+//
+// Work.  Tiles are 8 or 16 rows (tokens x query heads of one key/value head);
+// the stream of their key blocks is cut evenly over the launch (Share in
+// lmoe_attn.cuh).  Inside a launch block every warp takes key blocks of its
+// own (KS positions, 4 KB of codes) and streams them through a private ring of
+// shared-memory units with 16-byte cp.async, so warps never wait for one
+// another inside a tile; their results meet once per tile.
+//
+// Arithmetic.  Both products are computed transposed, with the keys (values)
+// as the 16-row operand of mma.m16n8k16 and the tile's 8 rows as its 8
+// columns: S^T = K Q^T and O^T = V^T P^T.  With a handful of query heads per
+// key/value head that halves the MMAs of the usual orientation, and the
+// operands that come from memory can be assembled in registers straight from
+// codes: the contraction order of K (the head dimension) and the row order of
+// V^T are free, so a lane takes whole words of codes where they lie.
+#include "lmoe_attn.cuh"
 
 namespace lmoe {
 
 namespace {
 
-template <typename TA, int BITS>
-__device__ __forceinline__ float cached_value(const KvView &c, int which, int64_t row, int e) {
-    if constexpr (BITS == 16) {
-        return Act<TA>::to_f(reinterpret_cast<const uint16_t *>(c.kv[which])[row * (c.row_bytes / 2) + e]);
+constexpr int kRowWarps = 4;
+constexpr int kRowThreads = kRowWarps * 32;
+constexpr int kRowBlocksPerSm = 4;  // at most
+
+template <int BITS, int D, int GS, int NT>
+struct RowsGeo {
+    static constexpr int R = 8 * NT;                               // rows of a tile
+    static constexpr int RB = D * BITS / 8;                        // bytes of a head row
+    static constexpr int KS = 4096 / RB < 64 ? 4096 / RB : 64;     // positions of a block
+    static constexpr int NG = BITS == 16 ? 0 : D / GS;             // groups of a head row
+    static constexpr int CB = KS * RB, SB = KS * NG * 2;           // code and scale bytes of a unit
+    static constexpr int UB = CB + 2 * SB;                         // a unit: codes, scales, biases
+    static constexpr int NU = 3;                                   // units of a warp's ring
+    static constexpr int KT = KS / 16, MT = D / 16, QS = D / 16;   // 16-key steps, V^T row tiles, K steps
+    static constexpr int MERGE = kRowWarps * R * (D + 4) * 4;      // per-warp results of a tile
+    static constexpr int RING = kRowWarps * NU * UB;
+    static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + kRowWarps * R * 8;
+};
+
+__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t movm(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+template <int N>  // 1, 2 or 4 words
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+    if constexpr (N == 1) {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
+    } else if constexpr (N == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
     } else {
-        const uint8_t by = c.kv[which][row * c.row_bytes + e * BITS / 8];
-        const uint32_t q = BITS == 8 ? by : (by >> (4 * (e & 1)) & 15u);
-        const int64_t gi = row * c.groups + e / c.group_size;
-        return fmaf(Act<TA>::to_f(c.scale[which][gi]), (float)q, Act<TA>::to_f(c.bias[which][gi]));
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(a)
+                     : "memory");
     }
 }
+__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts_u16(uint32_t a, uint16_t v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
+}
 
-template <typename TA, int BITS, int D>
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
-    constexpr int E = D / 32;
+// Byte offset in a unit's codes of byte `o` of position `row`.  16-byte chunks
+// are XOR-swizzled inside 128-byte lines so that a warp's reads fall in
+// distinct banks: 16-bit rows by the row (ldmatrix of 8 rows), K codes by the
+// row's parity (rows g with 4 neighbouring chunks), V codes by the row pair
+// (lane t reads rows 2t and 2t + 1).
+template <int BITS, int D, int WHICH>
+__device__ __forceinline__ int unit_off(int row, int o) {
+    constexpr int RB = D * BITS / 8;
+    const int lin = row * RB + o;
+    int h = 0;
+    if constexpr (BITS == 16) h = row & 7;
+    else if constexpr (WHICH == 0) h = RB == 128 ? (row & 1) << 2 : 0;
+    else h = RB == 32 ? ((row >> 2) & 1) << 1 : ((row >> 1) & 3) << 1;
+    return lin ^ (h << 4);
+}
+
+template <typename TA, int BITS, int D, int GS, int NT>
+__global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel(const AttnArgs a) {
+    using G = RowsGeo<BITS, D, GS, NT>;
+    constexpr int R = G::R, KS = G::KS, KT = G::KT, MT = G::MT, QS = G::QS, NG = G::NG, RB = G::RB;
+    constexpr bool Q = BITS != 16;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ long long s_plan[kRowWarps + 6];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring = smem_u32(sm) + warp * (G::NU * G::UB);
+    float *s_o = reinterpret_cast<float *>(sm);
+    float *s_ml = reinterpret_cast<float *>(sm + (G::SMEM - kRowWarps * R * 8));
+    MergeRec *rec = reinterpret_cast<MergeRec *>(a.scratch) + blockIdx.x;
     pdl_wait();
     pdl_trigger();
-    const int64_t wid = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (blockIdx.x == 0) a.r.validate(threadIdx.x, 256);
-    if (wid >= (int64_t)a.r.n_rows * a.q_heads) return;
-    const int r = (int)(wid / a.q_heads), h = (int)(wid % a.q_heads);
-    int pos = 0;
-    const int b = a.r.find(r, &pos);
-    if (b < 0 && pos >= 0) return;  // no sequence's row
-    const int hk = h / a.group;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
+    if (blockIdx.x == 0) a.r.validate(tid, kRowThreads);
+    Share sh;
+    Cursor cur;
+    // a run of at least one key block for each warp
+    const bool work = find_share<R, KS, kRowThreads>(a, kRowWarps, s_plan, sh, cur);
+    if (tid == 0) rec->parts = 0;
+    if (!work) return;
+    long long left = sh.begin(blockIdx.x + 1) - sh.begin(blockIdx.x);
+    const float sc = a.scale_log2;
+
+    while (left > 0) {
+        const Tile &t = cur.t;
+        const int b0 = cur.blk, b1 = (int)min((long long)t.nblk, b0 + left);
+        left -= b1 - b0;
+
+        // ---- the tile's rows as the column operand of S^T, in the order of K's words
+        uint32_t qf[NT][QS][2];
+        int pos[NT][2];  // positions of this lane's two columns' rows; -1: no row
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        q[i] = Act<TA>::to_f(a.q[r * a.q_tok_stride + h * a.q_head_stride + lane + 32 * i]) * a.scale_log2;
-        o[i] = 0.0f;
-    }
-    bool any = false;
-    if (b >= 0) {
-        const int low = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-        int j = a.sinks > 0 ? 0 : low;
-        int cur = -1;
-        int32_t page = -1;
-        for (; j <= pos; ++j) {
-            if (j < low && j >= a.sinks) j = low;
-            if (j / a.c.page_size != cur) {
-                cur = j / a.c.page_size;
-                page = a.r.page(a.c, b, j);
+        for (int n = 0; n < NT; ++n) {
+            const int row = t.rt * R + n * 8 + g;  // in the sequence's rows
+            const bool in = row < t.n * a.group;
+            const int tok = row / a.group;
+            const uint16_t *q = a.q + (int64_t)(t.row0 + tok) * a.q_tok_stride +
+                                (int64_t)(t.h * a.group + row - tok * a.group) * a.q_head_stride;
+#pragma unroll
+            for (int s = 0; s < QS; ++s) {
+                uint32_t x0 = 0, x1 = 0;
+                if constexpr (BITS == 16) {
+                    if (in) {
+                        x0 = *reinterpret_cast<const uint32_t *>(q + 16 * s + 2 * t4);
+                        x1 = *reinterpret_cast<const uint32_t *>(q + 16 * s + 8 + 2 * t4);
+                    }
+                } else if constexpr (BITS == 8) {
+                    // codes (c0, c2), (c1, c3) of word s of the lane's chunk
+                    uint2 v = make_uint2(0u, 0u);
+                    if (in) v = *reinterpret_cast<const uint2 *>(q + 64 * (s >> 2) + 16 * t4 + 4 * (s & 3));
+                    x0 = __byte_perm(v.x, v.y, 0x5410);
+                    x1 = __byte_perm(v.x, v.y, 0x7632);
+                } else {
+                    // codes (c0, c4), (c1, c5) of word s / 2, then (c2, c6), (c3, c7)
+                    uint2 lo = make_uint2(0u, 0u);
+                    if (in) {
+                        const uint16_t *p = q + t4 * (D / 4) + 8 * (s >> 1) + 2 * (s & 1);
+                        lo.x = *reinterpret_cast<const uint32_t *>(p);
+                        lo.y = *reinterpret_cast<const uint32_t *>(p + 4);
+                    }
+                    x0 = __byte_perm(lo.x, lo.y, 0x5410);
+                    x1 = __byte_perm(lo.x, lo.y, 0x7632);
+                }
+                qf[n][s][0] = x0;
+                qf[n][s][1] = x1;
             }
-            if (page < 0) continue;
-            any = true;
-            const int64_t row = a.c.row(page, hk, j % a.c.page_size);
-            float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = fmaf(q[i], cached_value<TA, BITS>(a.c, 0, row, lane + 32 * i), s);
-            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            const float mn = fmaxf(m, s);
-            const float f = mn == -INFINITY ? 1.0f : exp2f(m - mn), p = s == -INFINITY ? 0.0f : exp2f(s - mn);
-            m = mn;
-            l = l * f + p;
+            for (int c = 0; c < 2; ++c) {
+                const int rc = t.rt * R + n * 8 + 2 * t4 + c;
+                pos[n][c] = rc < t.n * a.group ? t.first + rc / a.group : -1;
+            }
+        }
+        float o[NT][MT][4], m[NT][2], l[NT][2];
+        bool seen[NT][2];
 #pragma unroll
-            for (int i = 0; i < E; ++i) o[i] = o[i] * f + p * cached_value<TA, BITS>(a.c, 1, row, lane + 32 * i);
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[n][c] = -INFINITY;
+                l[n][c] = 0.0f;
+                seen[n][c] = false;
+            }
+        }
+
+        // ---- this warp's blocks of [b0, b1), as units K, V, K, V, ...
+        const int nb = b0 + warp < b1 ? (b1 - b0 - warp + kRowWarps - 1) / kRowWarps : 0;
+        // page of 16-position run `lane` of block i of the warp's; -2: no such
+        // positions, -1: no page
+        auto pages_of = [&](int i) -> int32_t {
+            int32_t pg = -2;
+            if (lane < KT && i < nb) {
+                const int p = t.block(b0 + warp + i * kRowWarps) * KS + lane * 16;
+                if (p < t.hi) pg = a.r.page(a.c, t.b, p);
+            }
+            return pg;
+        };
+        auto issue = [&](auto which, int i, int32_t pg, int slot) {
+            constexpr int W = decltype(which)::value;
+            if (i < nb) {
+                const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
+                const uint32_t u = ring + slot * G::UB;
+                const int slot0 = k0 % a.c.page_size;  // positions of a run are in one page, runs in turn
+#pragma unroll
+                for (int it = 0; it < G::CB / 512; ++it) {
+                    const int ch = it * 32 + lane, row = ch / (RB / 16), c = ch % (RB / 16);
+                    const int32_t p = __shfl_sync(0xffffffffu, pg, row >> 4);
+                    int sl = slot0 + row;
+                    while (sl >= a.c.page_size) sl -= a.c.page_size;
+                    const bool in = p >= 0 && k0 + row < t.hi;
+                    const uint8_t *src = a.c.kv[W] + (in ? a.c.row(p, t.h, sl) * RB + c * 16 : 0);
+                    cp16z(u + unit_off<BITS, D, W>(row, c * 16), src, in ? 16 : 0);
+                }
+                if constexpr (Q) {
+                    constexpr int CPR = 2 * NG;  // 16-byte chunks of a run's scales
+                    static_assert(CPR * KT <= 32, "one chunk a lane");
+                    const int run = min(lane / CPR, KT - 1), c = lane % CPR;
+                    const int32_t p = __shfl_sync(0xffffffffu, pg, run);
+                    if (lane < CPR * KT) {
+                        int sl = slot0 + run * 16;
+                        while (sl >= a.c.page_size) sl -= a.c.page_size;
+                        int bytes = min(16, max(0, (t.hi - k0 - run * 16) * NG * 2 - c * 16));
+                        if (p < 0) bytes = 0;
+                        const int64_t off = bytes ? a.c.row(p, t.h, sl) * NG + c * 8 : 0;
+                        cp16z(u + G::CB + lane * 16, a.c.scale[W] + off, bytes);
+                        cp16z(u + G::CB + G::SB + lane * 16, a.c.bias[W] + off, bytes);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        using K0 = std::integral_constant<int, 0>;
+        using V1 = std::integral_constant<int, 1>;
+        int32_t pg_cur = pages_of(0), pg_next = pages_of(1), pg_far = pages_of(2);
+        issue(K0{}, 0, pg_cur, 0);
+        issue(V1{}, 0, pg_cur, 1);
+        issue(K0{}, 1, pg_next, 2);
+        int ks = 0;  // ring slot of the block's keys; its values follow
+        for (int i = 0; i < nb; ++i) {
+            const int vs = ks + 1 >= G::NU ? ks + 1 - G::NU : ks + 1;
+            const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
+            const uint32_t bad = __ballot_sync(0xffffffffu, pg_cur == -1);  // runs without a page
+            // every row of the tile sees every position of the block
+            const bool full = !bad && k0 + KS - 1 <= t.minpos &&
+                              (a.window == 0 || k0 > (long long)t.maxpos - a.window || k0 + KS <= a.sinks);
+
+            // ---- S^T = K Q^T
+            cp_wait<G::NU - 1>();
+            __syncwarp();
+            float s[KT][NT][4];
+            const uint32_t ku = ring + ks * G::UB;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.0f;
+                if constexpr (BITS == 16) {
+                    const int r = kt * 16 + (lane & 15), ch = lane >> 4;
+#pragma unroll
+                    for (int x = 0; x < QS; ++x) {
+                        uint32_t f[4];
+                        ldsm4(ku + unit_off<16, D, 0>(r, (2 * x + ch) * 16), f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            Act<TA>::mma(s[kt][n], f[0], f[1], f[2], f[3], qf[n][x][0], qf[n][x][1]);
+                    }
+                } else {
+                    constexpr int NC = BITS == 8 && D == 128 ? 2 : 1;  // word chunks of a lane's row part
+                    constexpr int WC = RB / 4 / 4 / NC;                // words of a chunk
+#pragma unroll
+                    for (int nc = 0; nc < NC; ++nc) {
+                        uint32_t w[2][WC], s2[2], b2[2];
+                        const int dim0 = BITS == 8 ? 64 * nc + 16 * t4 : (D / 4) * t4;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = kt * 16 + 8 * h + g;
+                            lds_words<WC>(ku + unit_off<BITS, D, 0>(r, dim0 * BITS / 8), w[h]);
+                            const uint32_t so = ku + G::CB + (r * NG + dim0 / GS) * 2;
+                            s2[h] = Pair<TA>::template scale<BITS>(lds_u16(so) * 0x10001u);
+                            b2[h] = lds_u16(so + G::SB) * 0x10001u;
+                        }
+#pragma unroll
+                        for (int x = 0; x < WC; ++x) {
+                            if constexpr (BITS == 8) {
+                                const int st = nc * WC + x;
+                                const uint32_t a0 = code_pair<TA, 8>(w[0][x], 0, s2[0], b2[0]);
+                                const uint32_t a1 = code_pair<TA, 8>(w[1][x], 0, s2[1], b2[1]);
+                                const uint32_t a2 = code_pair<TA, 8>(w[0][x], 1, s2[0], b2[0]);
+                                const uint32_t a3 = code_pair<TA, 8>(w[1][x], 1, s2[1], b2[1]);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+                                    Act<TA>::mma(s[kt][n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
+                            } else {
+#pragma unroll
+                                for (int hf = 0; hf < 2; ++hf) {
+                                    const int st = 2 * x + hf;
+                                    const uint32_t a0 = code_pair<TA, 4>(w[0][x], 2 * hf, s2[0], b2[0]);
+                                    const uint32_t a1 = code_pair<TA, 4>(w[1][x], 2 * hf, s2[1], b2[1]);
+                                    const uint32_t a2 = code_pair<TA, 4>(w[0][x], 2 * hf + 1, s2[0], b2[0]);
+                                    const uint32_t a3 = code_pair<TA, 4>(w[1][x], 2 * hf + 1, s2[1], b2[1]);
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n)
+                                        Act<TA>::mma(s[kt][n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            issue(V1{}, i + 1, pg_next, ks);  // the keys' slot is free
+
+            // ---- softmax over the block: mask, maximum, terms
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[kt][n][e] *= sc;
+                        if (!full) {
+                            const int j = k0 + kt * 16 + g + 8 * (e >> 1), p = pos[n][e & 1];
+                            const bool see = j <= p && !(bad >> kt & 1u) &&
+                                             (a.window == 0 || p - j < a.window || j < a.sinks);
+                            seen[n][e & 1] |= see;
+                            if (!see) s[kt][n][e] = -INFINITY;
+                        }
+                    }
+            bool moved = false;
+            float mu[NT][2], f[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = max_nan(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+                    for (int kt = 1; kt < KT; ++kt) x = max_nan(x, max_nan(s[kt][n][c], s[kt][n][c + 2]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    x = max_nan(m[n][c], x);
+                    if (full) seen[n][c] = true;
+                    mu[n][c] = x == -INFINITY ? 0.0f : x;
+                    f[n][c] = ex2(m[n][c] - mu[n][c]);
+                    moved |= !(x == m[n][c]);
+                    m[n][c] = x;
+                }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    l[n][0] *= f[n][0];
+                    l[n][1] *= f[n][1];
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        o[n][x][0] *= f[n][0];
+                        o[n][x][1] *= f[n][1];
+                        o[n][x][2] *= f[n][0];
+                        o[n][x][3] *= f[n][1];
+                    }
+                }
+            }
+            uint32_t pf[KT][NT][2];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = ex2(s[kt][n][e] - mu[n][e & 1]);
+                    l[n][0] += p[0] + p[2];
+                    l[n][1] += p[1] + p[3];
+                    pf[kt][n][0] = movm(Act<TA>::pack2(p[0], p[1]));
+                    pf[kt][n][1] = movm(Act<TA>::pack2(p[2], p[3]));
+                }
+
+            // ---- O^T += V^T P^T
+            cp_wait<G::NU - 1>();
+            __syncwarp();
+            const uint32_t vu = ring + vs * G::UB;
+            if (!full) {
+                // A value that is no number must not reach the rows that do
+                // not see its position (0 times it is no number either): it
+                // is added here to those that do and taken out of the unit.
+                constexpr int W4 = RB / 4, SW = NG;
+                bool odd = false;
+                if constexpr (Q) {
+                    for (int i2 = lane; i2 < KS * SW; i2 += 32) {
+                        const uint32_t x = lds_u16(vu + G::CB + i2 * 2), y = lds_u16(vu + G::CB + G::SB + i2 * 2);
+                        odd |= (x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask || (y & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
+                    }
+                } else {
+                    for (int i2 = lane; i2 < KS * W4; i2 += 32) {
+                        uint32_t x[1];
+                        lds_words<1>(vu + i2 * 4, x);
+                        odd |= (x[0] & Pair<TA>::kExpMask) == Pair<TA>::kExpMask ||
+                               (x[0] >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+                    for (int k = 0; k < KS; ++k) {
+                        const int j = k0 + k;
+#pragma unroll
+                        for (int x = 0; x < MT; ++x)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                // the lane's row of V^T (see the products below)
+                                const int dim = Q ? (D / 8) * g + h * (D / 16) + x : 16 * x + 8 * h + g;
+                                float v;
+                                if constexpr (Q) {
+                                    const int byte = dim * BITS / 8;
+                                    uint32_t w[1];
+                                    lds_words<1>(vu + unit_off<BITS, D, 1>(k, byte & ~3), w);
+                                    const uint32_t code = w[0] >> (dim * BITS % 32) & ((1u << BITS) - 1u);
+                                    const uint32_t so = vu + G::CB + (k * SW + dim / GS) * 2;
+                                    v = fmaf(Act<TA>::to_f((uint16_t)lds_u16(so)), (float)code,
+                                             Act<TA>::to_f((uint16_t)lds_u16(so + G::SB)));
+                                } else {
+                                    v = Act<TA>::to_f((uint16_t)lds_u16(vu + unit_off<16, D, 1>(k, dim * 2)));
+                                }
+                                if (!(fabsf(v) <= 3.402823466e38f)) {
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                        for (int c = 0; c < 2; ++c) {
+                                            const int p = pos[n][c];
+                                            if (j <= p && (a.window == 0 || p - j < a.window || j < a.sinks))
+                                                o[n][x][2 * h + c] += v;
+                                        }
+                                }
+                            }
+                    }
+                    __syncwarp();
+                    if constexpr (Q) {
+                        for (int i2 = lane; i2 < KS * SW; i2 += 32) {
+                            const uint32_t sa = vu + G::CB + i2 * 2;
+                            const uint32_t x = lds_u16(sa), y = lds_u16(sa + G::SB);
+                            if ((x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask ||
+                                (y & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) {
+                                sts_u16(sa, 0);
+                                sts_u16(sa + G::SB, 0);
+                            }
+                        }
+                    } else {
+                        for (int i2 = lane; i2 < KS * W4 * 2; i2 += 32)
+                            if ((lds_u16(vu + i2 * 2) & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) sts_u16(vu + i2 * 2, 0);
+                    }
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                if constexpr (BITS == 16) {
+                    const int r = kt * 16 + (lane & 7) + (lane >> 4) * 8, ch = lane >> 3 & 1;
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        uint32_t f4[4];
+                        ldsm4t(vu + unit_off<16, D, 1>(r, (2 * x + ch) * 16), f4);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            Act<TA>::mma(o[n][x], f4[0], f4[1], f4[2], f4[3], pf[kt][n][0], pf[kt][n][1]);
+                    }
+                } else {
+                    // lane: dims (D / 8) g .. of positions 2 t4, 2 t4 + 1 (first
+                    // half of the step) and 8 behind them; row g of row tile x
+                    // is dim (D / 8) g + x, row g + 8 is D / 16 further
+                    constexpr int WL = RB / 8 / 4;  // words of the lane's dims
+                    uint32_t u[2][WL][2], s2[2], b2[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = kt * 16 + 8 * h + 2 * t4;
+                        uint32_t w0[WL], w1[WL];
+                        lds_words<WL>(vu + unit_off<BITS, D, 1>(r, g * (RB / 8)), w0);
+                        lds_words<WL>(vu + unit_off<BITS, D, 1>(r + 1, g * (RB / 8)), w1);
+#pragma unroll
+                        for (int x = 0; x < WL; ++x) {
+                            u[h][x][0] = __byte_perm(w0[x], w1[x], 0x5410);
+                            u[h][x][1] = __byte_perm(w0[x], w1[x], 0x7632);
+                        }
+                        const uint32_t so = vu + G::CB + (r * NG + (D / 8) * g / GS) * 2;
+                        s2[h] = Pair<TA>::template scale<BITS>(lds_u16(so) | lds_u16(so + NG * 2) << 16);
+                        b2[h] = lds_u16(so + G::SB) | lds_u16(so + G::SB + NG * 2) << 16;
+                    }
+#pragma unroll
+                    for (int x = 0; x < MT; ++x) {
+                        // dims x and MT + x of the lane's: half-word and code in it
+                        constexpr int CH = 16 / BITS;  // codes of a half-word
+                        const int i0 = x / CH, i1 = (MT + x) / CH, j = x % CH;
+                        const uint32_t a0 = code_pair<TA, BITS>(u[0][i0 >> 1][i0 & 1], j, s2[0], b2[0]);
+                        const uint32_t a1 = code_pair<TA, BITS>(u[0][i1 >> 1][i1 & 1], j, s2[0], b2[0]);
+                        const uint32_t a2 = code_pair<TA, BITS>(u[1][i0 >> 1][i0 & 1], j, s2[1], b2[1]);
+                        const uint32_t a3 = code_pair<TA, BITS>(u[1][i1 >> 1][i1 & 1], j, s2[1], b2[1]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            Act<TA>::mma(o[n][x], a0, a1, a2, a3, pf[kt][n][0], pf[kt][n][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            pg_cur = pg_next;
+            pg_next = pg_far;
+            issue(K0{}, i + 2, pg_next, vs);  // the values' slot is free
+            pg_far = pages_of(i + 3);
+            ks = ks == 0 ? 2 : ks - 1;  // two units on, of three
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp's ring is free: the results of the warps meet there
+
+        // ---- join the warps
+        const bool whole = b0 == 0 && b1 == t.nblk;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = l[n][c];
+                uint32_t sn = seen[n][c];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    x += __shfl_xor_sync(0xffffffffu, x, d);
+                    sn |= __shfl_xor_sync(0xffffffffu, sn, d);
+                }
+                // only scores of -inf: the softmax is no number, unless other
+                // parts of the tile's keys hold larger ones
+                if (sn && m[n][c] == -INFINITY) x = __uint_as_float(0x7FC00000u);
+                if (g == 0) {
+                    s_ml[(warp * R + n * 8 + 2 * t4 + c) * 2] = m[n][c];
+                    s_ml[(warp * R + n * 8 + 2 * t4 + c) * 2 + 1] = x;
+                }
+#pragma unroll
+                for (int x2 = 0; x2 < MT; ++x2)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int dim = Q ? (D / 8) * g + h * (D / 16) + x2 : 16 * x2 + 8 * h + g;
+                        s_o[(warp * R + n * 8 + 2 * t4 + c) * (D + 4) + dim] = o[n][x2][2 * h + c];
+                    }
+            }
+        __syncthreads();
+        float *part = part_ptr(a, gridDim.x, part_floats<R, D>(), blockIdx.x, b0 == 0 ? 1 : 0);
+        for (int i = tid; i < R * (D / 4); i += kRowThreads) {
+            const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+            float mm = -INFINITY, ll = 0.0f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) mm = max_nan(mm, s_ml[(w * R + row) * 2]);
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) {
+                const float mw = s_ml[(w * R + row) * 2];
+                if (mw == -INFINITY && mm != -INFINITY) continue;
+                const float x = mw == -INFINITY ? 1.0f : ex2(mw - mm);
+                const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * (D + 4) + d);
+                ll += x * s_ml[(w * R + row) * 2 + 1];
+                acc.x += x * v.x;
+                acc.y += x * v.y;
+                acc.z += x * v.z;
+                acc.w += x * v.w;
+            }
+            if (!whole) {
+                *reinterpret_cast<float4 *>(part + row * D + d) = acc;
+                if (d == 0) {
+                    part[R * D + row * 2] = mm;
+                    part[R * D + row * 2 + 1] = ll;
+                }
+            } else if (row < t.rows) {
+                const int rr = t.rt * R + row, tok = rr / a.group;
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                uint2 v;
+                v.x = Act<TA>::pack2(acc.x * inv, acc.y * inv);
+                v.y = Act<TA>::pack2(acc.z * inv, acc.w * inv);
+                *reinterpret_cast<uint2 *>(a.out + ((int64_t)(t.row0 + tok) * a.q_heads + t.h * a.group + rr -
+                                                    tok * a.group) * D + d) = v;
+            }
+        }
+        if (tid == 0 && b0 == 0 && b1 < t.nblk) {
+            rec->out0 = t.row0;
+            rec->row = t.rt * R;
+            rec->rows_h = t.rows | t.h << 16;
+            rec->parts = sh.owner(cur.tile_begin + t.nblk - 1) - blockIdx.x + 1;
+        }
+        if (left > 0) {
+            __syncthreads();
+            next_tile<R, KS>(a, cur);
         }
     }
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-        a.out[((int64_t)r * a.q_heads + h) * D + lane + 32 * i] = any ? Act<TA>::from_f(o[i] / l) : (uint16_t)0;
 }
 
-template <typename TA, int BITS, int D>
-cudaError_t launch_rows(const AttnArgs &a, cudaStream_t st) {
-    const int64_t warps = (int64_t)a.r.n_rows * a.q_heads;
-    return launch_pdl(attn_rows_kernel<TA, BITS, D>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, a);
+// Joins the parts of the tiles that were cut: block (c, y) the tile that goes
+// on behind launch block c's run; row by row (rows split over y), a warp's
+// lanes the head dimension, the block's warps every 8th part.
+template <typename TA, int R, int D>
+__global__ void __launch_bounds__(256) attn_merge_kernel(const AttnArgs a, int grid) {
+    constexpr int V = D / 32;  // elements of a lane
+    __shared__ float s_m[8], s_l[8], s_o[8][D];
+    pdl_wait();
+    pdl_trigger();
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const MergeRec rec = reinterpret_cast<const MergeRec *>(a.scratch)[c];
+    if (rec.parts < 2) return;
+    const int rows = rec.rows_h & 0xFFFF, h = rec.rows_h >> 16;
+    const float *first = part_ptr(a, grid, part_floats<R, D>(), c, 1);
+    const size_t pf = part_floats<R, D>();
+    auto part = [&](int i) { return i == 0 ? first : first + (size_t)(2 * i - 1) * pf; };
+    const bool wide = rec.parts > 8;  // many parts: all warps on one row; few: a row each
+    for (int row = blockIdx.y * (wide ? 1 : 8) + (wide ? 0 : warp); row < rows; row += gridDim.y * (wide ? 1 : 8)) {
+        float mm = -INFINITY, ll = 0.0f, acc[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        const int i0 = wide ? warp : 0, step = wide ? 8 : 1;
+        for (int i = i0 + lane * step; i < rec.parts; i += 32 * step) mm = max_nan(mm, part(i)[R * D + row * 2]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) mm = max_nan(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+#pragma unroll 4
+        for (int i = i0; i < rec.parts; i += step) {
+            const float *p = part(i);
+            const float mi = p[R * D + row * 2], li = p[R * D + row * 2 + 1];
+            float x[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = p[row * D + v * 32 + lane];
+            if (mi == -INFINITY && mm != -INFINITY) continue;
+            const float w = mi == -INFINITY ? 1.0f : ex2(mi - mm);
+            ll += w * li;
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] += w * x[v];
+        }
+        if (wide) {
+            if (lane == 0) {
+                s_m[warp] = mm;
+                s_l[warp] = ll;
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) s_o[warp][v * 32 + lane] = acc[v];
+            __syncthreads();
+            if (warp == 0) {
+                mm = -INFINITY;
+                ll = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) mm = max_nan(mm, s_m[w]);
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+                for (int w = 0; w < 8; ++w) {
+                    if (s_m[w] == -INFINITY && mm != -INFINITY) continue;
+                    const float x = s_m[w] == -INFINITY ? 1.0f : ex2(s_m[w] - mm);
+                    ll += x * s_l[w];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[v] += x * s_o[w][v * 32 + lane];
+                }
+            }
+            __syncthreads();
+            if (warp != 0) continue;
+        }
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+        const int rr = rec.row + row, tok = rr / a.group;
+        uint16_t *out = a.out + ((int64_t)(rec.out0 + tok) * a.q_heads + h * a.group + rr - tok * a.group) * D;
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v * 32 + lane] = Act<TA>::from_f(acc[v] * inv);
+    }
+}
+
+template <typename TA, int BITS, int D, int GS, int NT>
+cudaError_t launch_rows_t(const AttnArgs &a, cudaStream_t st) {
+    using G = RowsGeo<BITS, D, GS, NT>;
+    auto kern = attn_rows_kernel<TA, BITS, D, GS, NT>;
+    // launch blocks that fit on an SM at once, by device; the whole launch is resident
+    static int per_sm[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    int fit = dev < 64 ? per_sm[dev] : 0;
+    if (fit == 0) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, kRowThreads, G::SMEM);
+        if (e != cudaSuccess) return e;
+        fit = min(max(fit, 1), kRowBlocksPerSm);
+        if (dev < 64) per_sm[dev] = fit;
+    }
+    const int grid = attn_num_sms() * fit;
+    e = launch_pdl(kern, dim3((unsigned)grid), dim3(kRowThreads), G::SMEM, st, a);
+    if (e != cudaSuccess) return e;
+    // few tiles, each cut into many parts: a merge block for each row
+    const int y = (long long)a.r.n_seqs * a.c.kv_heads * 8 < grid ? G::R : 1;
+    return launch_pdl(attn_merge_kernel<TA, G::R, D>, dim3((unsigned)grid, (unsigned)y), dim3(256), 0, st, a, grid);
+}
+
+template <typename TA, int BITS, int D, int GS>
+cudaError_t launch_nt(int nt, const AttnArgs &a, cudaStream_t st) {
+    return nt == 1 ? launch_rows_t<TA, BITS, D, GS, 1>(a, st) : launch_rows_t<TA, BITS, D, GS, 2>(a, st);
 }
 
 template <typename TA>
-cudaError_t launch_bits(int D, int bits, const AttnArgs &a, cudaStream_t st) {
-    if (D == 64) {
-        if (bits == 16) return launch_rows<TA, 16, 64>(a, st);
-        if (bits == 8) return launch_rows<TA, 8, 64>(a, st);
-        return launch_rows<TA, 4, 64>(a, st);
-    }
-    if (bits == 16) return launch_rows<TA, 16, 128>(a, st);
-    if (bits == 8) return launch_rows<TA, 8, 128>(a, st);
-    return launch_rows<TA, 4, 128>(a, st);
+cudaError_t launch_rows(int D, int bits, int gs, int nt, const AttnArgs &a, cudaStream_t st) {
+#define LMOE_ATTN_CASE(B, DD, GG) \
+    if (bits == B && D == DD && (B == 16 || gs == GG)) return launch_nt<TA, B, DD, GG>(nt, a, st);
+    LMOE_ATTN_CASE(16, 64, 64)
+    LMOE_ATTN_CASE(16, 128, 64)
+    LMOE_ATTN_CASE(8, 64, 32)
+    LMOE_ATTN_CASE(8, 64, 64)
+    LMOE_ATTN_CASE(8, 128, 32)
+    LMOE_ATTN_CASE(8, 128, 64)
+    LMOE_ATTN_CASE(8, 128, 128)
+    LMOE_ATTN_CASE(4, 64, 32)
+    LMOE_ATTN_CASE(4, 64, 64)
+    LMOE_ATTN_CASE(4, 128, 32)
+    LMOE_ATTN_CASE(4, 128, 64)
+    LMOE_ATTN_CASE(4, 128, 128)
+#undef LMOE_ATTN_CASE
+    return cudaErrorInvalidValue;
 }
+
+// tiles of 8 rows while the sequences have that many on average, else of 16
+int rows_nt(const KvRows &r, int group) { return (long long)r.n_rows * group <= 8ll * r.n_seqs ? 1 : 2; }
 
 }  // namespace
 
-size_t attention_scratch_bytes(const KvRows &, int, int, int) { return 0; }
+int attn_num_sms() {
+    static int sms[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (sms[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+        sms[dev] = n;
+    }
+    return sms[dev];
+}
 
-cudaError_t launch_attention(int act_f16, int head_dim, int bits, int, const AttnArgs &a, cudaStream_t st) {
-    return act_f16 ? launch_bits<__half>(head_dim, bits, a, st) : launch_bits<__nv_bfloat16>(head_dim, bits, a, st);
+size_t attention_scratch_bytes(const KvRows &r, int, int group, int D) {
+    if (r.n_rows == 0 || r.n_seqs == 0) return 0;
+    const int nt = rows_nt(r, group), grid = attn_num_sms() * kRowBlocksPerSm;
+    return (size_t)grid * (sizeof(MergeRec) + 2 * sizeof(float) * (size_t)(8 * nt) * (D + 2));
+}
+
+cudaError_t launch_attention(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st) {
+    const int nt = rows_nt(a.r, a.group);
+    return act_f16 ? launch_rows<__half>(head_dim, bits, group_size, nt, a, st)
+                   : launch_rows<__nv_bfloat16>(head_dim, bits, group_size, nt, a, st);
 }
 
 }  // namespace lmoe

@@ -1,0 +1,266 @@
+// Shared by the attention kernels: which keys a tile of rows sees, how the
+// work of a launch is cut over its blocks, and 16-bit pair arithmetic.
+#pragma once
+
+#include "lmoe_kernels.cuh"
+#include "lmoe_kv.cuh"
+
+namespace lmoe {
+
+// A tile is up to R consecutive rows of one sequence for one key/value head,
+// where the rows of a sequence are its tokens times the group's query heads
+// (row i = token i / group, head i % group).  Its keys are walked in blocks
+// of KS positions: first the blocks of the first tokens that stay visible
+// (sinks), then the blocks from the window's lower edge of its first token to
+// its last token's position.
+struct Tile {
+    int b, rt, h;       // sequence, row tile, key/value head
+    int row0;           // first row of the arrays that is the sequence's
+    int n;              // its token rows
+    int first;          // position of its token row 0 (may be negative)
+    int rows;           // rows of the tile, 1..R
+    int minpos, maxpos; // positions of the tile's first and last row
+    int hi;             // keys [0, hi) are looked at
+    int nsink, lo;      // sink blocks, first block of the rest
+    int nblk;           // blocks; at least 1, so a tile that sees nothing is written
+    __device__ __forceinline__ int block(int i) const { return i < nsink ? i : lo + i - nsink; }
+};
+
+template <int R, int KS>
+__device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
+    const int r0 = t.rt * R;
+    t.rows = min(R, t.n * a.group - r0);
+    t.minpos = t.first + r0 / a.group;
+    t.maxpos = t.first + (r0 + t.rows - 1) / a.group;
+    t.hi = max(0, t.maxpos + 1);
+    int low = 0;
+    if (a.window > 0) low = (int)max(0ll, (long long)t.minpos - a.window + 1);
+    t.lo = low / KS;
+    t.nsink = t.lo > 0 ? min((min(a.sinks, t.hi) + KS - 1) / KS, t.lo) : 0;
+    t.nblk = max(1, t.nsink + (t.hi + KS - 1) / KS - t.lo);
+}
+
+// Blocks of all tiles of sequence b (one head), and its rows.
+template <int R, int KS>
+__device__ __forceinline__ int seq_blocks(const AttnArgs &a, int b, Tile &t) {
+    t.b = b;
+    t.row0 = a.r.start(b);
+    t.n = max(0, a.r.start(b + 1) - t.row0);
+    t.first = max(a.r.lens[b], 0) - t.n;
+    int sum = 0;
+    const int nt = (t.n * a.group + R - 1) / R;
+    for (t.rt = 0; t.rt < nt; ++t.rt) {
+        tile_range<R, KS>(a, t);
+        sum += t.nblk;
+    }
+    return sum;
+}
+
+// The blocks of all (sequence, row tile, head), in that order, form one
+// stream; block c of the launch takes the c-th of `parts` equal runs of it.
+// So ragged batches stay level without the host knowing a length, and a tile
+// may be cut over several blocks of the launch; attn_merge_kernel joins those.
+struct Share {
+    long long total;  // blocks of the stream
+    int parts;        // launch blocks that take part
+    __device__ __forceinline__ long long begin(int c) const { return total * c / parts; }
+    __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * parts + total - 1) / total) - 1; }
+};
+
+// Position in the stream: the tile, and the block in it.
+struct Cursor {
+    Tile t;
+    int blk;
+    long long tile_begin;  // stream position of the tile's block 0
+};
+
+// Finds the launch block's run; every thread of the block calls it (NTHR
+// threads, smem of at least NTHR / 32 + 6 long longs).  False: no work.
+template <int R, int KS, int NTHR>
+__device__ __forceinline__ bool find_share(const AttnArgs &a, int minb, long long *sm, Share &sh, Cursor &cur) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NW = NTHR / 32;
+    Tile t;
+    long long carry = 0;
+    long long mine = 0;  // this thread's sequence of the first round
+    const int rounds = (a.r.n_seqs + NTHR - 1) / NTHR;
+    // total; with at most NTHR sequences one round finds everything
+    for (int k = 0; k < rounds; ++k) {
+        const int b = k * NTHR + tid;
+        const long long w = b < a.r.n_seqs ? (long long)seq_blocks<R, KS>(a, b, t) * a.c.kv_heads : 0;
+        if (k == 0) mine = w;
+        carry += w;
+    }
+    long long sum = carry;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sm[warp] = sum;
+    __syncthreads();
+    sh.total = 0;
+    for (int w = 0; w < NW; ++w) sh.total += sm[w];
+    __syncthreads();
+    if (sh.total == 0) return false;
+    sh.parts = (int)min((long long)gridDim.x, max(1ll, sh.total / minb));
+    if ((int)blockIdx.x >= sh.parts) return false;
+    const long long s = sh.begin(blockIdx.x);
+    // the sequence that holds stream position s
+    long long base = 0;
+    for (int k = 0; k < rounds; ++k) {
+        const int b = k * NTHR + tid;
+        const long long w = k == 0 ? mine : (b < a.r.n_seqs ? (long long)seq_blocks<R, KS>(a, b, t) * a.c.kv_heads : 0);
+        long long inc = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) sm[warp] = inc;
+        __syncthreads();
+        long long before = base;
+        for (int q = 0; q < NW; ++q) {
+            if (q < warp) before += sm[q];
+            base += sm[q];
+        }
+        before += inc - w;
+        if (w > 0 && before <= s && s < before + w) {
+            sm[NW] = b;
+            sm[NW + 1] = before;
+        }
+        __syncthreads();
+        if (s < base) break;
+    }
+    // its tile and head
+    Tile &ct = cur.t;
+    const int b = (int)sm[NW];
+    long long off = s - sm[NW + 1];
+    ct.b = b;
+    ct.row0 = a.r.start(b);
+    ct.n = max(0, a.r.start(b + 1) - ct.row0);
+    ct.first = max(a.r.lens[b], 0) - ct.n;
+    for (ct.rt = 0;; ++ct.rt) {
+        tile_range<R, KS>(a, ct);
+        const long long w = (long long)ct.nblk * a.c.kv_heads;
+        if (off < w) break;
+        off -= w;
+    }
+    ct.h = (int)(off / ct.nblk);
+    cur.blk = (int)(off % ct.nblk);
+    cur.tile_begin = s - cur.blk;
+    __syncthreads();
+    return true;
+}
+
+// The tile after cur's (there is one).
+template <int R, int KS>
+__device__ __forceinline__ void next_tile(const AttnArgs &a, Cursor &cur) {
+    Tile &t = cur.t;
+    cur.tile_begin += t.nblk;
+    cur.blk = 0;
+    if (++t.h < a.c.kv_heads) return;
+    t.h = 0;
+    if (++t.rt * (long long)R < (long long)t.n * a.group) {
+        tile_range<R, KS>(a, t);
+        return;
+    }
+    t.rt = 0;
+    do {
+        ++t.b;
+        t.row0 = a.r.start(t.b);
+        t.n = max(0, a.r.start(t.b + 1) - t.row0);
+    } while (t.n == 0);
+    t.first = max(a.r.lens[t.b], 0) - t.n;
+    tile_range<R, KS>(a, t);
+}
+
+// Scratch: one record for each launch block (the cut tile that begins in its
+// run, if any), then two partial results each: slot 0 of a launch block is
+// its part of a tile begun before it, slot 1 of the tile that goes on behind
+// it.  A partial: R rows of D fp32 sums, then R (maximum, sum) pairs.
+struct MergeRec {
+    int32_t parts;  // 0 or 1: nothing to merge
+    int32_t out0;   // first row of the sequence
+    int32_t row;    // first row of the tile in the sequence's rows
+    int32_t rows_h; // rows | head << 16
+};
+template <int R, int D>
+__host__ __device__ constexpr size_t part_floats() {
+    return (size_t)R * (D + 2);
+}
+__device__ __forceinline__ float *part_ptr(const AttnArgs &a, int grid, size_t floats, int c, int slot) {
+    return reinterpret_cast<float *>(a.scratch + (size_t)grid * sizeof(MergeRec)) + ((size_t)2 * c + slot) * floats;
+}
+
+// maximum that keeps a NaN
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ------------------------------------------------------------ packed 16-bit pairs
+template <typename TA>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
+    }
+    __device__ __forceinline__ static uint32_t mul(uint32_t a, uint32_t b) { return fma(a, b, 0x80008000u); }
+    // 8-bit codes: the code's bits are a bf16 subnormal, c * 2^-133;
+    // multiplied by 2^127 it is c * 2^-6 exactly, and the scale is taken times
+    // 2^6 (exact, no overflow: a scale is at most 2^129 / 255).  4-bit codes,
+    // whose scales may be larger: 0x4300 | c is 128 + c.
+    template <int BITS>
+    __device__ __forceinline__ static uint32_t scale(uint32_t s2) {
+        return BITS == 8 ? mul(s2, 0x42804280u) : s2;
+    }
+    __device__ __forceinline__ static uint32_t value8(uint32_t c, uint32_t s2, uint32_t b2) {
+        return fma(mul(c, 0x7F007F00u), s2, b2);
+    }
+    // code j of each half
+    __device__ __forceinline__ static uint32_t value4(uint32_t u, int j, uint32_t s2, uint32_t b2) {
+        return fma(fma(and_or(u >> (4 * j), 0x000F000Fu, 0x43004300u), 0x3F803F80u, 0xC300C300u), s2, b2);
+    }
+    static constexpr uint32_t kExpMask = 0x7F80u;
+};
+template <>
+struct Pair<__half> {
+    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
+    }
+    template <int BITS>
+    __device__ __forceinline__ static uint32_t scale(uint32_t s2) {
+        return s2;
+    }
+    // 0x6400 | c is 1024 + c
+    __device__ __forceinline__ static uint32_t value8(uint32_t c, uint32_t s2, uint32_t b2) {
+        return fma(fma(c | 0x64006400u, 0x3C003C00u, 0xE400E400u), s2, b2);
+    }
+    // code j of each half; at bits 4..7, 0x6400 | c << 4 is 1024 + 16 c
+    __device__ __forceinline__ static uint32_t value4(uint32_t u, int j, uint32_t s2, uint32_t b2) {
+        const uint32_t v = j < 2 ? u : u >> 8;
+        return j & 1 ? fma(fma(and_or(v, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD400D400u), s2, b2)
+                     : fma(fma(and_or(v, 0x000F000Fu, 0x64006400u), 0x3C003C00u, 0xE400E400u), s2, b2);
+    }
+    static constexpr uint32_t kExpMask = 0x7C00u;
+};
+
+// Value pair j of a word's two halves: 4-bit codes j = 0..3, 8-bit codes j = 0..1.
+template <typename TA, int BITS>
+__device__ __forceinline__ uint32_t code_pair(uint32_t u, int j, uint32_t s2, uint32_t b2) {
+    if constexpr (BITS == 4) return Pair<TA>::value4(u, j, s2, b2);
+    else return Pair<TA>::value8((j ? u >> 8 : u) & 0x00FF00FFu, s2, b2);
+}
+
+int attn_num_sms();
+
+}  // namespace lmoe

@@ -263,7 +263,7 @@ int check_cache(const lmoe_kv_cache *c, KvView *v) {
     if (!c || !c->k || !c->v || c->n_pages < 1 || c->page_size < 1 || c->kv_heads < 1) return LMOE_EINVAL;
     if (c->dtype != LMOE_BF16 && c->dtype != LMOE_F16) return LMOE_EUNSUPPORTED;
     if (c->head_dim != 64 && c->head_dim != 128) return LMOE_EUNSUPPORTED;
-    if (c->page_size % 16 != 0) return LMOE_EUNSUPPORTED;
+    if (c->page_size % 16 != 0 || c->kv_heads > 32767) return LMOE_EUNSUPPORTED;
     const bool quant = c->bits != 16;
     if (quant) {
         if (c->bits != 8 && c->bits != 4) return LMOE_EUNSUPPORTED;
