@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -25,8 +26,9 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-r
               "-Wno-deprecated-gpu-targets"]
 
 LMOE_SOURCES = ["lmoe_route.cu", "lmoe_gemv.cu", "lmoe_stream.cu", "lmoe_vec.cu", "lmoe_prefill.cu", "lmoe_ep.cu", "lmoe_api.cu",
-                "lmoe_kv.cu", "lmoe_attn.cu"]
-LMOE_DEPS = LMOE_SOURCES + ["lmoe_common.cuh", "lmoe_kernels.cuh", "lmoe_kv.cuh", "lmoe_attn.cuh"]
+                "lmoe_kv.cu", "lmoe_attn.cu", "lmoe_attn_chunk.cu"]
+KV_HEADERS = ["lmoe_kv.cuh", "lmoe_attn.cuh"]  # of the key/value cache's sources alone
+LMOE_DEPS = LMOE_SOURCES + ["lmoe_common.cuh", "lmoe_kernels.cuh", "lmoe_tc.cuh"] + KV_HEADERS
 LMOE_LIB = PKG / "liblmoe.so"
 CORE_LIB = PKG / "liblocali_core.so"
 
@@ -59,16 +61,21 @@ def build_lmoe(force: bool = False, verbose: bool = False) -> Path:
     nvcc = _nvcc()
     objdir = CSRC / "_build"
     objdir.mkdir(exist_ok=True)
-    headers = [CSRC / s for s in LMOE_DEPS if s.endswith(".cuh")] + [INCLUDE / "lmoe.h", Path(__file__)]
-    objs = []
+    headers = [CSRC / s for s in LMOE_DEPS if s.endswith(".cuh") and s not in KV_HEADERS]
+    headers += [INCLUDE / "lmoe.h", Path(__file__)]
+    kv_headers = [CSRC / s for s in KV_HEADERS]
+    objs, cmds = [], []
     for src in LMOE_SOURCES:
         obj = objdir / (Path(src).stem + ".o")
-        if force or verbose or _stale(obj, [CSRC / src, *headers]):
+        deps = [CSRC / src, *headers] + (kv_headers if src.startswith(("lmoe_kv", "lmoe_attn")) else [])
+        if force or verbose or _stale(obj, deps):
             cmd = [nvcc, *ARCH, *NVCC_FLAGS, f"-I{INCLUDE}", "-c", str(CSRC / src), "-o", str(obj)]
             if verbose:
                 cmd.insert(1, "-Xptxas=-v")
-            _run(cmd)
+            cmds.append(cmd)
         objs.append(str(obj))
+    with ThreadPoolExecutor(max_workers=max(1, min(4, os.cpu_count() or 1))) as pool:
+        list(pool.map(_run, cmds))
     tmp = LMOE_LIB.with_suffix(".so.tmp")
     _run([nvcc, *ARCH, "-shared", "-o", str(tmp), *objs, "-lcudart"])
     os.replace(tmp, LMOE_LIB)

@@ -47,6 +47,9 @@ struct RowsGeo {
 __device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -197,43 +200,51 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 
         // ---- this warp's blocks of [b0, b1), as units K, V, K, V, ...
         const int nb = b0 + warp < b1 ? (b1 - b0 - warp + kRowWarps - 1) / kRowWarps : 0;
-        // page of 16-position run `lane` of block i of the warp's; -2: no such
-        // positions, -1: no page
-        auto pages_of = [&](int i) -> int32_t {
-            int32_t pg = -2;
+        // Head row (of all pages') where 16-position run `lane` of block i of
+        // the warp's begins; -2: no such positions, -1: no page.
+        auto runs_of = [&](int i) -> long long {
+            long long r = -2;
             if (lane < KT && i < nb) {
                 const int p = t.block(b0 + warp + i * kRowWarps) * KS + lane * 16;
-                if (p < t.hi) pg = a.r.page(a.c, t.b, p);
+                if (p < t.hi) {
+                    const int32_t pg = a.r.page(a.c, t.b, p);
+                    r = pg < 0 ? -1 : a.c.row(pg, t.h, p % a.c.page_size);
+                }
             }
-            return pg;
+            return r;
         };
-        auto issue = [&](auto which, int i, int32_t pg, int slot) {
+        auto issue = [&](auto which, int i, long long runs, int slot) {
             constexpr int W = decltype(which)::value;
+            constexpr int RPI = 512 / RB;  // rows of one copy instruction of the warp
             if (i < nb) {
                 const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
                 const uint32_t u = ring + slot * G::UB;
-                const int slot0 = k0 % a.c.page_size;  // positions of a run are in one page, runs in turn
+                const int r0 = lane / (RB / 16), c0 = lane % (RB / 16);
+                const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, runs == -1);
 #pragma unroll
-                for (int it = 0; it < G::CB / 512; ++it) {
-                    const int ch = it * 32 + lane, row = ch / (RB / 16), c = ch % (RB / 16);
-                    const int32_t p = __shfl_sync(0xffffffffu, pg, row >> 4);
-                    int sl = slot0 + row;
-                    while (sl >= a.c.page_size) sl -= a.c.page_size;
-                    const bool in = p >= 0 && k0 + row < t.hi;
-                    const uint8_t *src = a.c.kv[W] + (in ? a.c.row(p, t.h, sl) * RB + c * 16 : 0);
-                    cp16z(u + unit_off<BITS, D, W>(row, c * 16), src, in ? 16 : 0);
+                for (int kt = 0; kt < KT; ++kt) {
+                    const long long run = __shfl_sync(0xffffffffu, runs, kt);
+                    const uint8_t *src = a.c.kv[W] + (run < 0 ? 0 : run * RB + lane * 16);
+#pragma unroll
+                    for (int it = 0; it < 16 / RPI; ++it) {
+                        const int row = kt * 16 + it * RPI + r0;
+                        const uint32_t dst = u + unit_off<BITS, D, W>(row, c0 * 16);
+                        if (all) cp16(dst, src + it * 512);
+                        else {
+                            const bool in = run >= 0 && k0 + row < t.hi;
+                            cp16z(dst, in ? src + it * 512 : a.c.kv[W], in ? 16 : 0);
+                        }
+                    }
                 }
                 if constexpr (Q) {
                     constexpr int CPR = 2 * NG;  // 16-byte chunks of a run's scales
                     static_assert(CPR * KT <= 32, "one chunk a lane");
                     const int run = min(lane / CPR, KT - 1), c = lane % CPR;
-                    const int32_t p = __shfl_sync(0xffffffffu, pg, run);
+                    const long long r = __shfl_sync(0xffffffffu, runs, run);
                     if (lane < CPR * KT) {
-                        int sl = slot0 + run * 16;
-                        while (sl >= a.c.page_size) sl -= a.c.page_size;
                         int bytes = min(16, max(0, (t.hi - k0 - run * 16) * NG * 2 - c * 16));
-                        if (p < 0) bytes = 0;
-                        const int64_t off = bytes ? a.c.row(p, t.h, sl) * NG + c * 8 : 0;
+                        if (r < 0) bytes = 0;
+                        const long long off = bytes ? r * NG + c * 8 : 0;
                         cp16z(u + G::CB + lane * 16, a.c.scale[W] + off, bytes);
                         cp16z(u + G::CB + G::SB + lane * 16, a.c.bias[W] + off, bytes);
                     }
@@ -243,7 +254,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
         };
         using K0 = std::integral_constant<int, 0>;
         using V1 = std::integral_constant<int, 1>;
-        int32_t pg_cur = pages_of(0), pg_next = pages_of(1), pg_far = pages_of(2);
+        long long pg_cur = runs_of(0), pg_next = runs_of(1), pg_far = runs_of(2);
         issue(K0{}, 0, pg_cur, 0);
         issue(V1{}, 0, pg_cur, 1);
         issue(K0{}, 1, pg_next, 2);
@@ -511,7 +522,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
             pg_cur = pg_next;
             pg_next = pg_far;
             issue(K0{}, i + 2, pg_next, vs);  // the values' slot is free
-            pg_far = pages_of(i + 3);
+            pg_far = runs_of(i + 3);
             ks = ks == 0 ? 2 : ks - 1;  // two units on, of three
         }
         cp_wait<0>();
@@ -688,7 +699,7 @@ cudaError_t launch_rows_t(const AttnArgs &a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     // few tiles, each cut into many parts: a merge block for each row
     const int y = (long long)a.r.n_seqs * a.c.kv_heads * 8 < grid ? G::R : 1;
-    return launch_pdl(attn_merge_kernel<TA, G::R, D>, dim3((unsigned)grid, (unsigned)y), dim3(256), 0, st, a, grid);
+    return launch_attn_merge(std::is_same<TA, __half>::value, G::R, D, grid, y, a, st);
 }
 
 template <typename TA, int BITS, int D, int GS>
@@ -719,6 +730,9 @@ cudaError_t launch_rows(int D, int bits, int gs, int nt, const AttnArgs &a, cuda
 // tiles of 8 rows while the sequences have that many on average, else of 16
 int rows_nt(const KvRows &r, int group) { return (long long)r.n_rows * group <= 8ll * r.n_seqs ? 1 : 2; }
 
+// Chunks on average: the tcgen05 kernel's tiles of 256 rows.
+bool use_chunk(const KvRows &r, int group) { return (long long)r.n_rows * group > 16ll * r.n_seqs; }
+
 }  // namespace
 
 int attn_num_sms() {
@@ -733,13 +747,31 @@ int attn_num_sms() {
     return sms[dev];
 }
 
+cudaError_t launch_attn_merge(int act_f16, int R, int D, int grid, int y, const AttnArgs &a, cudaStream_t st) {
+    const dim3 g((unsigned)grid, (unsigned)y), b(256);
+#define LMOE_MERGE_CASE(RR, DD)                                                                       \
+    if (R == RR && D == DD)                                                                           \
+        return act_f16 ? launch_pdl(attn_merge_kernel<__half, RR, DD>, g, b, 0, st, a, grid)          \
+                       : launch_pdl(attn_merge_kernel<__nv_bfloat16, RR, DD>, g, b, 0, st, a, grid);
+    LMOE_MERGE_CASE(8, 64)
+    LMOE_MERGE_CASE(8, 128)
+    LMOE_MERGE_CASE(16, 64)
+    LMOE_MERGE_CASE(16, 128)
+    LMOE_MERGE_CASE(256, 64)
+    LMOE_MERGE_CASE(256, 128)
+#undef LMOE_MERGE_CASE
+    return cudaErrorInvalidValue;
+}
+
 size_t attention_scratch_bytes(const KvRows &r, int, int group, int D) {
     if (r.n_rows == 0 || r.n_seqs == 0) return 0;
+    if (use_chunk(r, group)) return chunk_scratch_bytes(D);
     const int nt = rows_nt(r, group), grid = attn_num_sms() * kRowBlocksPerSm;
     return (size_t)grid * (sizeof(MergeRec) + 2 * sizeof(float) * (size_t)(8 * nt) * (D + 2));
 }
 
 cudaError_t launch_attention(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st) {
+    if (use_chunk(a.r, a.group)) return launch_attn_chunk(act_f16, head_dim, bits, group_size, a, st);
     const int nt = rows_nt(a.r, a.group);
     return act_f16 ? launch_rows<__half>(head_dim, bits, group_size, nt, a, st)
                    : launch_rows<__nv_bfloat16>(head_dim, bits, group_size, nt, a, st);

@@ -258,9 +258,14 @@ struct Pair<__half> {
 template <typename TA, int BITS>
 __device__ __forceinline__ uint32_t code_pair(uint32_t u, int j, uint32_t s2, uint32_t b2) {
     if constexpr (BITS == 4) return Pair<TA>::value4(u, j, s2, b2);
-    else return Pair<TA>::value8((j ? u >> 8 : u) & 0x00FF00FFu, s2, b2);
+    else return Pair<TA>::value8(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, s2, b2);
 }
 
 int attn_num_sms();
+// lmoe_attn.cu: joins the cut tiles of R rows of a launch of `grid` blocks; y: merge blocks for each
+cudaError_t launch_attn_merge(int act_f16, int R, int D, int grid, int y, const AttnArgs &a, cudaStream_t st);
+// lmoe_attn_chunk.cu
+size_t chunk_scratch_bytes(int head_dim);
+cudaError_t launch_attn_chunk(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st);
 
 }  // namespace lmoe

@@ -1,0 +1,756 @@
+// Attention of chunks (many rows of a sequence) over the paged key/value
+// cache, on the 5th-generation tensor cores.
+//
+// A tile is 256 rows (tokens x query heads of one key/value head) as two
+// sub-tiles of 128, the M of a tcgen05.mma; its keys are walked in blocks of
+// 128 positions.  Per block and sub-tile t:
+//   S_t = Q_t K^T            (Q_t, K in shared memory; S_t in tensor memory)
+//   P_t = exp2(S_t c - m_t)  (one thread per row; P_t over S_t, in 16 bits)
+//   O_t += P_t V             (P_t from tensor memory, V in shared memory)
+// One block per SM; the stream of (tile, head, key block) is cut evenly over
+// the launch as in lmoe_attn.cu.  Warp roles:
+//   0-3, 4-7   softmax and output of sub-tile 0 and 1
+//   8-11       keys into shared memory; 12-15 values: 16-bit rows by cp.async,
+//              codes through registers, dequantised to the 16-bit type on the
+//              way, both into the 128-byte-swizzled operand layout
+//   16, 17     one thread each issues the MMAs of sub-tile 0, 1
+// The sub-tiles run apart, so one's softmax overlaps the other's MMAs.  The
+// running maximum of a row moves only when a score passes it by 2^8: until
+// then terms may exceed 1, which costs nothing in fp32 and leaves the sums in
+// tensor memory untouched (a row's result is the quotient either way).
+//
+// V is the MN-major B operand (head dimension contiguous), so keys and values
+// share one layout: [D / 64][128 positions][128 bytes], 16-byte chunk c of
+// position r at c ^ (r & 7).
+//
+// Bound by the tensor pipe (4 D flops per row and key) and, close to it, by
+// the 16 exponentials a cycle of an SM (one per row and key).
+#include "lmoe_attn.cuh"
+#include "lmoe_tc.cuh"
+
+namespace lmoe {
+
+namespace {
+
+constexpr int kCkRows = 256, kCkKeys = 128, kCkSub = 128;
+constexpr int kCkThreads = 18 * 32;
+constexpr int kCkKWarp = 8, kCkVWarp = 12, kCkMmaWarp = 16;
+constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
+constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
+
+template <int BITS, int D, int GS>
+struct ChunkGeo {
+    static constexpr int HALVES = D / 64;
+    static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
+    static constexpr int NG = BITS == 16 ? 1 : D / GS;
+    static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
+    static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
+    static constexpr int SMEM = 1024 + 6 * TILE + SCALES + 1024;
+};
+
+// Walks the key blocks of a launch block's run, tile by tile.
+struct Walk {
+    Cursor cur;
+    long long left;
+    int b0, b1;  // blocks of the current tile that are this launch block's
+    __device__ __forceinline__ void begin(const Cursor &c, long long n) {
+        cur = c;
+        left = n;
+        open();
+    }
+    __device__ __forceinline__ void open() {
+        b0 = cur.blk;
+        b1 = (int)min((long long)cur.t.nblk, b0 + left);
+        left -= b1 - b0;
+    }
+    __device__ __forceinline__ bool next(const AttnArgs &a) {
+        if (left <= 0) return false;
+        next_tile<kCkRows, kCkKeys>(a, cur);
+        open();
+        return true;
+    }
+};
+
+// every row of the tile sees every position of the block at k0
+__device__ __forceinline__ bool block_full(const AttnArgs &a, int k0, int minpos, int maxpos) {
+    return k0 + kCkKeys - 1 <= minpos &&
+           (a.window == 0 || k0 > (long long)maxpos - a.window || k0 + kCkKeys <= a.sinks);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// the registers pass through, so no use of them moves above the wait
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Shared-memory descriptor of an MN-major operand, 128-byte swizzle: 64
+// elements of MN by 8 of K are one 1024-byte atom, the next 8 of K 1024 bytes
+// on, the next 64 of MN 16 KB on.
+__device__ __forceinline__ uint64_t mn128_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+// fp32 accumulator, M = 128, N = n, A K-major, B K-major or MN-major
+__device__ __forceinline__ uint32_t attn_idesc(int n, bool f16, bool b_mn) {
+    const uint32_t fmt = f16 ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(128 >> 4) << 24);
+}
+
+// bits of [lo, hi) in the 32 positions from kb
+__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int kb) {
+    const int l = min(max(lo - kb, 0), 32), h = min(max(hi - kb, 0), 32);
+    return h > l ? (0xFFFFFFFFu >> (32 - (h - l))) << l : 0u;
+}
+
+// byte offset of 16-byte chunk c of row r in an operand tile
+__device__ __forceinline__ uint32_t op_off(int r, int c) {
+    return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void cpa16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <typename TA>
+__device__ __forceinline__ bool nonfinite2(uint32_t x) {
+    return (x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask || (x >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
+}
+
+// 8 codes -> 8 values as 16-bit pairs in order
+template <typename TA, int BITS>
+__device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, uint32_t s2, uint32_t b2) {
+    uint32_t v[4];
+    if constexpr (BITS == 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = Pair<TA>::value8(__byte_perm(i < 2 ? w0 : w1, 0u, i & 1 ? 0x4342 : 0x4140), s2, b2);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // codes 2i, 2i + 1 are the low nibbles of bytes i of the word and of it shifted
+            v[i] = Pair<TA>::value4(__byte_perm(w0, w0 >> 4, i | (4 + i) << 8), 0, s2, b2);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <typename TA, int BITS, int D, int GS>
+__global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArgs a) {
+    using G = ChunkGeo<BITS, D, GS>;
+    constexpr int CH = D / 8;   // 16-byte chunks of an operand row
+    constexpr int RB = D * BITS / 8;
+    constexpr bool Q = BITS != 16;
+    constexpr int NG = G::NG;
+    constexpr bool F16 = std::is_same<TA, __half>::value;
+    extern __shared__ __align__(1024) uint8_t raw[];
+    __shared__ long long s_plan[kCkThreads / 32 + 6];
+    __shared__ __align__(16) uint32_t s_bad[4][4];  // block u & 3: the key warps' runs without a page
+    __shared__ uint32_t s_poison[4][kPoison][4];    // tile & 3, its n-th block seen in part: rows taken out
+    __shared__ int s_pblk[4][kPoison];
+    __shared__ uint64_t bars[16];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_abort;
+    uint8_t *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t sb = smem_u32(smem);
+    uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *sfull = bars + 8,
+             *pfull = bars + 10, *qfull = bars + 12, *ofull = bars + 14;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&kfull[i], 4);
+            mbar_init(&kempty[i], 2);
+            mbar_init(&vfull[i], 4);
+            mbar_init(&vempty[i], 2);
+            mbar_init(&sfull[i], 1);
+            mbar_init(&pfull[i], 4);
+            mbar_init(&qfull[i], 4);
+            mbar_init(&ofull[i], 1);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+    if (blockIdx.x == 0) a.r.validate(threadIdx.x, kCkThreads);
+    MergeRec *rec = reinterpret_cast<MergeRec *>(a.scratch) + blockIdx.x;
+    if (threadIdx.x == 0) rec->parts = 0;
+    Share sh;
+    Cursor first;
+    if (!find_share<kCkRows, kCkKeys, kCkThreads>(a, kCkMinBlocks, s_plan, sh, first)) return;
+    const long long run = sh.begin(blockIdx.x + 1) - sh.begin(blockIdx.x);
+    if (warp == kCkMmaWarp) {
+        tmem_alloc(&s_tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    // tensor memory columns: S_0 (P_0), S_1 (P_1), O_0, O_1
+    auto tm_s = [&](int t) { return tmem + (uint32_t)(t * 128); };
+    auto tm_o = [&](int t) { return tmem + (uint32_t)(256 + t * D); };
+
+    // a wait that gave up: the error is latched and every role leaves
+    auto wait = [&](uint64_t *bar, uint32_t ph) -> bool {
+        if (pf_wait(bar, ph)) return true;
+        s_abort = 1;
+        set_error(a.r.err, kErrCuda);
+        return false;
+    };
+    Walk w;
+    w.begin(first, run);
+
+    if (warp < kCkKWarp) {
+        // ---------------------------------------------------- softmax and output
+        const int t = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;  // row of the sub-tile
+        const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+        const uint32_t qs = sb + G::OFF_Q + t * G::TILE;
+        const float sc = a.scale_log2;
+        // the row's query into the operand tile (zeros where there is none)
+        auto load_q = [&](const Tile &ti) {
+            const int row = ti.rt * kCkRows + t * kCkSub + r;
+            const bool in = row < ti.n * a.group;
+            const int tok = in ? row / a.group : 0;
+            const uint16_t *src = a.q + (int64_t)(ti.row0 + tok) * a.q_tok_stride +
+                                  (int64_t)(ti.h * a.group + (in ? row - tok * a.group : 0)) * a.q_head_stride;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) cpa16(qs + op_off(r, c), in ? src + c * 8 : a.q, in ? 16 : 0);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        load_q(w.cur.t);
+        int u = 0, act = 0, segs = 0, active_segs = 0;
+        bool ok = true;
+        while (ok && !s_abort) {
+            const Tile ti = w.cur.t;
+            const int b0 = w.b0, b1 = w.b1;
+            const long long tile_begin = w.cur.tile_begin;
+            const bool more = w.next(a);  // w: the tile after this one
+            if (t == 1 && ti.rows <= kCkSub) {
+                // no rows: only pass the tiles of keys and values on
+                if (r == 0)
+                    for (int i = b0; i < b1 && ok; ++i) {
+                        const int s = (u + i - b0) & 1, ph = (u + i - b0) >> 1 & 1;
+                        ok = wait(&kfull[s], ph);
+                        if (ok) mbar_arrive(&kempty[s]);
+                        ok = ok && wait(&vfull[s], ph);
+                        if (ok) mbar_arrive(&vempty[s]);
+                    }
+                u += b1 - b0;
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");  // before the same rows are written again
+                if (more) load_q(w.cur.t);
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&qfull[t]);
+                const int row = ti.rt * kCkRows + t * kCkSub + r;
+                const bool in = row < ti.n * a.group;
+                const int p = in ? ti.first + row / a.group : -1;
+                const int see_hi = p + 1, see_lo = a.window ? (int)max(0ll, (long long)p - a.window + 1) : 0;
+                const int see_sink = min(a.sinks, see_hi);
+                // positions of the sub-tile's first and last row
+                const int lastrow = min(ti.rows, (t + 1) * kCkSub) - 1;
+                const int smin = ti.first + (ti.rt * kCkRows + t * kCkSub) / a.group;
+                const int smax = ti.first + (ti.rt * kCkRows + lastrow) / a.group;
+                float m = -INFINITY;
+                float l0 = 0.0f, l1 = 0.0f;
+                bool seen = false;
+                int parts = 0;
+                for (int i = b0; i < b1; ++i, ++u, ++act) {
+                    const int k0 = ti.block(i) * kCkKeys;
+                    ok = __all_sync(0xffffffffu, wait(&sfull[t], act & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (r == 0) {  // the MMAs before S_t's end are done: the keys, and the values before
+                        mbar_arrive(&kempty[u & 1]);
+                        if (i > b0) mbar_arrive(&vempty[(u - 1) & 1]);
+                    }
+                    if (i == b1 - 1 && more) load_q(w.cur.t);  // Q_t is free
+                    const uint4 bw = *reinterpret_cast<const uint4 *>(s_bad[u & 3]);
+                    const uint32_t bad = bw.x | bw.y << 2 | bw.z << 4 | bw.w << 6;
+                    const bool full = !bad && block_full(a, k0, smin, smax);
+                    if (!block_full(a, k0, ti.minpos, ti.maxpos)) ++parts;
+                    auto mask = [&](int c) -> uint32_t {
+                        const int kb = k0 + 32 * c;
+                        uint32_t x = range_bits(see_lo, see_hi, kb) | range_bits(0, see_sink, kb);
+                        if (bad >> (2 * c) & 1u) x &= 0xFFFF0000u;
+                        if (bad >> (2 * c) & 2u) x &= 0x0000FFFFu;
+                        return x;
+                    };
+                    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(tm_s(t) + lanes + 32 * c, v);
+                        tmem_wait_ld32(v);
+                        if (!full) {
+                            const uint32_t mk = mask(c);
+                            seen |= mk != 0;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            x0 = max_nan(x0, __uint_as_float(v[e]));
+                            x1 = max_nan(x1, __uint_as_float(v[e + 1]));
+                        }
+                    }
+                    if (full) seen = true;
+                    const float x = max_nan(x0, x1) * sc;
+                    const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float f = move ? ex2(m - x) : 1.0f;
+                        if (move) m = x;
+                        l0 *= f;
+                        l1 *= f;
+                        if (i > b0) {  // the sums so far
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t v[32];
+                                tmem_ld32(tm_o(t) + lanes + 32 * c, v);
+                                tmem_wait_ld32(v);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                                tmem_st32(tm_o(t) + lanes + 32 * c, v);
+                            }
+                        }
+                    }
+                    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32], pk[16];
+                        tmem_ld32(tm_s(t) + lanes + 32 * c, v);
+                        tmem_wait_ld32(v);
+                        const uint32_t mk = full ? 0xFFFFFFFFu : mask(c);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float p0 = ex2(fmaf(__uint_as_float(v[e]), sc, -mu));
+                            float p1 = ex2(fmaf(__uint_as_float(v[e + 1]), sc, -mu));
+                            if (!full) {
+                                if (!(mk >> e & 1u)) p0 = 0.0f;
+                                if (!(mk >> (e + 1) & 1u)) p1 = 0.0f;
+                            }
+                            l0 += p0;
+                            l1 += p1;
+                            pk[e / 2] = Act<TA>::pack2(p0, p1);
+                        }
+                        tmem_st16(tm_s(t) + lanes + 16 * c, pk);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pfull[t]);
+                }
+                if (!ok) break;
+                // ---- the tile's result
+                ok = __all_sync(0xffffffffu, wait(&ofull[t], active_segs & 1));
+                ++active_segs;
+                if (!ok) break;
+                tc_fence_after();
+                if (r == 0) mbar_arrive(&vempty[(u - 1) & 1]);
+                float l = l0 + l1;
+                // only scores of -inf: the softmax is no number, unless other
+                // parts of the tile's keys hold larger ones
+                if (m == -INFINITY && seen) l = __uint_as_float(0x7FC00000u);
+                const bool whole = b0 == 0 && b1 == ti.nblk;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int tok = in ? row / a.group : 0;
+                uint16_t *out = a.out + ((int64_t)(ti.row0 + tok) * a.q_heads + ti.h * a.group + row - tok * a.group) * D;
+                float *part = part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) +
+                              (t * kCkSub + r) * D;
+                bool poisoned = false;
+                for (int n = 0; n < parts; ++n)
+                    poisoned |= (s_poison[segs & 3][n][0] | s_poison[segs & 3][n][1] | s_poison[segs & 3][n][2] |
+                                 s_poison[segs & 3][n][3]) != 0;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(tm_o(t) + lanes + 32 * c, v);
+                    tmem_wait_ld32(v);
+                    if (poisoned) {
+                        // values that are no numbers, taken out of blocks that
+                        // only some rows see: added for those that do
+                        for (int n = 0; n < parts; ++n)
+                            for (int k = 0; k < kCkKeys; ++k) {
+                                if (!(s_poison[segs & 3][n][k >> 5] >> (k & 31) & 1u)) continue;
+                                const int j = s_pblk[segs & 3][n] * kCkKeys + k;
+                                if (!(j < see_hi && (j >= see_lo || j < see_sink))) continue;
+                                const int32_t pg = a.r.page(a.c, ti.b, j);
+                                if (pg < 0) continue;
+                                const int64_t kr = a.c.row(pg, ti.h, j % a.c.page_size);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    const int d = 32 * c + e;
+                                    float y;
+                                    if constexpr (Q) {
+                                        const uint32_t by = a.c.kv[1][kr * RB + d * BITS / 8];
+                                        const uint32_t code = BITS == 8 ? by : by >> (4 * (d & 1)) & 15u;
+                                        y = fmaf(Act<TA>::to_f(a.c.scale[1][kr * NG + d / GS]), (float)code,
+                                                 Act<TA>::to_f(a.c.bias[1][kr * NG + d / GS]));
+                                    } else {
+                                        y = Act<TA>::to_f(reinterpret_cast<const uint16_t *>(a.c.kv[1])[kr * D + d]);
+                                    }
+                                    if (!(fabsf(y) <= 3.402823466e38f))
+                                        v[e] = __float_as_uint(__uint_as_float(v[e]) + y);
+                                }
+                            }
+                    }
+                    if (whole) {
+                        if (in) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint4 o;
+                                uint32_t *ov = &o.x;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    ov[k] = Act<TA>::pack2(__uint_as_float(v[e + 2 * k]) * inv,
+                                                           __uint_as_float(v[e + 2 * k + 1]) * inv);
+                                *reinterpret_cast<uint4 *>(out + 32 * c + e) = o;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<uint4 *>(part + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                }
+                if (!whole) {
+                    float2 *ml = reinterpret_cast<float2 *>(part - (t * kCkSub + r) * D + kCkRows * D);
+                    ml[t * kCkSub + r] = make_float2(m, l);
+                }
+                if (t == 0 && r == 0 && b0 == 0 && b1 < ti.nblk) {
+                    rec->out0 = ti.row0;
+                    rec->row = ti.rt * kCkRows;
+                    rec->rows_h = ti.rows | ti.h << 16;
+                    rec->parts = sh.owner(tile_begin + ti.nblk - 1) - blockIdx.x + 1;
+                }
+                // O_t is read: the next tile's first P_t says so
+                tc_fence_before();
+            }
+            ++segs;
+            if (!more) break;
+        }
+    } else if (warp < kCkMmaWarp) {
+        // ---------------------------------------------------- keys and values
+        const int which = warp >= kCkVWarp, lw = (warp - kCkKWarp) & 3;
+        uint64_t *fullb = which ? vfull : kfull, *emptyb = which ? vempty : kempty;
+        const uint32_t base = sb + (which ? G::OFF_V : G::OFF_K);
+        constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of a warp's 32
+        const int rr = lane / LPR, cc = lane % LPR;
+        int i = w.b0, segs = 0, parts = 0;
+        bool have = true;
+        // the block at hand: head row of 16-position run 0, 1 of the warp's (-2: none, -1: no page), its facts
+        struct Unit {
+            long long r0, r1;
+            int k0, hi, seg, part;  // part: its number among the blocks seen in part, -1: seen in full
+        };
+        auto unit = [&]() -> Unit {
+            Unit x;
+            const Tile &ti = w.cur.t;
+            x.k0 = ti.block(i) * kCkKeys;
+            x.hi = ti.hi;
+            x.seg = segs;
+            x.part = block_full(a, x.k0, ti.minpos, ti.maxpos) ? -1 : parts++;
+            long long r = -2;
+            const int p = x.k0 + lw * 32 + lane * 16;
+            if (lane < 2 && p < ti.hi) {
+                const int32_t pg = a.r.page(a.c, ti.b, p);
+                r = pg < 0 ? -1 : a.c.row(pg, ti.h, p % a.c.page_size);
+            }
+            x.r0 = __shfl_sync(0xffffffffu, r, 0);
+            x.r1 = __shfl_sync(0xffffffffu, r, 1);
+            return x;
+        };
+        auto step = [&]() {
+            if (++i < w.b1) return;
+            have = w.next(a);
+            i = w.b0;
+            ++segs;
+            parts = 0;
+        };
+        // head row of the warp's row x, -1 where there is nothing to read
+        auto row_of = [&](const Unit &n, int x) -> long long {
+            const long long r = x < 16 ? n.r0 : n.r1;
+            return r >= 0 && n.k0 + lw * 32 + x < n.hi ? r + (x & 15) : -1;
+        };
+        auto facts = [&](const Unit &n, int u, uint32_t taken) {
+            if (lane == 0) {
+                if (!which) s_bad[u & 3][lw] = (n.r0 == -1) | (n.r1 == -1) << 1;
+                else if (n.part >= 0) {
+                    s_poison[n.seg & 3][n.part][lw] = taken;
+                    if (lw == 0) s_pblk[n.seg & 3][n.part] = n.k0 / kCkKeys;
+                }
+            }
+        };
+        bool ok = true;
+        if constexpr (Q) {
+            constexpr int WPC = BITS == 8 ? 2 : 1;  // code words of a chunk
+            uint32_t code[IT][WPC];
+            uint32_t sbp[NG];  // (scale, bias) of row `lane`
+            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + (warp - kCkKWarp) * 32 * NG;
+            auto fetch = [&](const Unit &n, int x) {
+                const long long r = row_of(n, x * RPI + rr);
+                const uint8_t *src = a.c.kv[which] + r * RB + cc * BITS;
+                if constexpr (BITS == 8) {
+                    const uint2 v = r >= 0 ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
+                    code[x][0] = v.x;
+                    code[x][1] = v.y;
+                } else {
+                    code[x][0] = r >= 0 ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+                }
+            };
+            auto fetch_scales = [&](const Unit &n) {
+                const long long r = row_of(n, lane);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    sbp[g] = r >= 0 ? (uint32_t)a.c.scale[which][r * NG + g] | (uint32_t)a.c.bias[which][r * NG + g] << 16 : 0u;
+            };
+            Unit n = unit();
+            fetch_scales(n);
+#pragma unroll
+            for (int x = 0; x < IT; ++x) fetch(n, x);
+            step();
+            for (int u = 0; !s_abort; ++u) {
+                ok = __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1));
+                if (!ok) break;
+                uint32_t taken = 0;
+                {
+                    bool no = false;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        // in a block that only some rows see, values that are no numbers are taken out
+                        if (which && n.part >= 0 && nonfinite2<TA>(sbp[g])) {
+                            no = true;
+                            sbp[g] = 0;
+                        }
+                        const uint32_t s = Pair<TA>::template scale<BITS>(sbp[g]) & 0xFFFFu;
+                        spair[lane * NG + g] = s | (sbp[g] & 0xFFFF0000u);
+                    }
+                    taken = __ballot_sync(0xffffffffu, no);
+                }
+                facts(n, u, taken);
+                __syncwarp();
+                const bool next = have;
+                Unit nx = n;
+                if (next) {
+                    nx = unit();
+                    fetch_scales(nx);
+                }
+                const uint32_t dst = base + (u & 1) * G::TILE;
+#pragma unroll
+                for (int x = 0; x < IT; ++x) {
+                    const int row = lw * 32 + x * RPI + rr;
+                    const uint32_t sbv = spair[(x * RPI + rr) * NG + cc * 8 / GS];
+                    const uint4 v = dequant8<TA, BITS>(code[x][0], code[x][WPC - 1], __byte_perm(sbv, 0u, 0x1010),
+                                                       __byte_perm(sbv, 0u, 0x3232));
+                    sts128v(dst + op_off(row, cc), v.x, v.y, v.z, v.w);
+                    if (next) fetch(nx, x);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&fullb[u & 1]);
+                if (!next) break;
+                n = nx;
+                step();
+            }
+        } else {
+            Unit prev;
+            auto finish = [&](const Unit &n, int u) {
+                uint32_t taken = 0;
+                if (which && n.part >= 0) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (int x = 0; x < IT; ++x) {
+                        const int row = x * RPI + rr;
+                        const uint32_t at = base + (u & 1) * G::TILE + op_off(lw * 32 + row, cc);
+                        uint4 v = lds128(at);
+                        uint32_t *vv = &v.x;
+                        bool no = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (nonfinite2<TA>(vv[k])) {
+                                no = true;
+                                if ((vv[k] & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) vv[k] &= 0xFFFF0000u;
+                                if ((vv[k] >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) vv[k] &= 0xFFFFu;
+                            }
+                        if (no) sts128v(at, v.x, v.y, v.z, v.w);
+                        const uint32_t bl = __ballot_sync(0xffffffffu, no);
+#pragma unroll
+                        for (int y = 0; y < RPI; ++y)
+                            if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken |= 1u << (x * RPI + y);
+                    }
+                }
+                facts(n, u, taken);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&fullb[u & 1]);
+            };
+            int u = 0;
+            for (; have && !s_abort; ++u) {
+                const Unit n = unit();
+                step();
+                ok = __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1));
+                if (!ok) break;
+                const uint32_t dst = base + (u & 1) * G::TILE;
+#pragma unroll
+                for (int x = 0; x < IT; ++x) {
+                    const int row = x * RPI + rr;
+                    const long long r = row_of(n, row);
+                    cpa16(dst + op_off(lw * 32 + row, cc), r >= 0 ? a.c.kv[which] + r * RB + cc * 16 : a.c.kv[which],
+                          r >= 0 ? 16 : 0);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (u > 0) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    finish(prev, u - 1);
+                }
+                prev = n;
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (ok && u > 0) finish(prev, u - 1);
+        }
+    } else if (lane == 0) {
+        // ---------------------------------------------------- MMAs of sub-tile t
+        const int t = warp - kCkMmaWarp;
+        const uint32_t id_s = attn_idesc(kCkKeys, F16, false), id_o = attn_idesc(D, F16, true);
+        const uint64_t qd = sw128_desc(sb + G::OFF_Q + t * G::TILE);
+        auto scores = [&](int u) {
+            const uint64_t kd = sw128_desc(sb + G::OFF_K + (u & 1) * G::TILE);
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                const uint64_t o = (uint64_t)((s >> 2) * (16384 >> 4) + (s & 3) * 2);
+                umma_f16(tm_s(t), qd + o, kd + o, id_s, s ? 1u : 0u);
+            }
+            umma_commit(&sfull[t]);
+        };
+        int u = 0, act = 0, active_segs = 0;
+        bool ok = true;
+        while (ok && !s_abort) {
+            const int nb = w.b1 - w.b0;
+            if (t == 1 && w.cur.t.rows <= kCkSub) {
+                u += nb;
+            } else {
+                ok = wait(&qfull[t], active_segs & 1) && wait(&kfull[u & 1], u >> 1 & 1);
+                ++active_segs;
+                if (!ok) break;
+                tc_fence_after();
+                scores(u);
+                for (int j = 0; j < nb; ++j, ++u, ++act) {
+                    ok = wait(&vfull[u & 1], u >> 1 & 1) && wait(&pfull[t], act & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = mn128_desc(sb + G::OFF_V + (u & 1) * G::TILE);
+#pragma unroll
+                    for (int s = 0; s < kCkKeys / 16; ++s)
+                        umma_f16_ts(tm_o(t), tm_s(t) + 8 * s, vd + (uint64_t)(s * (2048 >> 4)), id_o, j || s ? 1u : 0u);
+                    if (j + 1 < nb) {
+                        ok = wait(&kfull[(u + 1) & 1], (u + 1) >> 1 & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(u + 1);
+                    } else {
+                        umma_commit(&ofull[t]);
+                    }
+                }
+            }
+            if (!ok || !w.next(a)) break;
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    if (s_abort && warp >= kCkMmaWarp && lane == 0) {
+        // a wait gave up: nothing may still write tensor memory when it is freed
+        uint64_t *b = &sfull[warp - kCkMmaWarp];
+        umma_commit(b);
+        const long long t0 = clock64();
+        while (clock64() - t0 < 10000000ll) {
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kCkMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename TA, int BITS, int D, int GS>
+cudaError_t launch_chunk_t(const AttnArgs &a, cudaStream_t st) {
+    using G = ChunkGeo<BITS, D, GS>;
+    auto kern = attn_chunk_kernel<TA, BITS, D, GS>;
+    static bool configured[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured[dev] = true;
+    }
+    const int grid = attn_num_sms();
+    e = launch_pdl(kern, dim3((unsigned)grid), dim3(kCkThreads), G::SMEM, st, a);
+    if (e != cudaSuccess) return e;
+    return launch_attn_merge(std::is_same<TA, __half>::value, kCkRows, D, grid, 8, a, st);
+}
+
+template <typename TA>
+cudaError_t launch_chunk_bits(int D, int bits, int gs, const AttnArgs &a, cudaStream_t st) {
+#define LMOE_ATTN_CASE(B, DD, GG) \
+    if (bits == B && D == DD && (B == 16 || gs == GG)) return launch_chunk_t<TA, B, DD, GG>(a, st);
+    LMOE_ATTN_CASE(16, 64, 64)
+    LMOE_ATTN_CASE(16, 128, 64)
+    LMOE_ATTN_CASE(8, 64, 32)
+    LMOE_ATTN_CASE(8, 64, 64)
+    LMOE_ATTN_CASE(8, 128, 32)
+    LMOE_ATTN_CASE(8, 128, 64)
+    LMOE_ATTN_CASE(8, 128, 128)
+    LMOE_ATTN_CASE(4, 64, 32)
+    LMOE_ATTN_CASE(4, 64, 64)
+    LMOE_ATTN_CASE(4, 128, 32)
+    LMOE_ATTN_CASE(4, 128, 64)
+    LMOE_ATTN_CASE(4, 128, 128)
+#undef LMOE_ATTN_CASE
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+size_t chunk_scratch_bytes(int D) {
+    return (size_t)attn_num_sms() * (sizeof(MergeRec) + 2 * sizeof(float) * (size_t)kCkRows * (D + 2));
+}
+
+cudaError_t launch_attn_chunk(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st) {
+    return act_f16 ? launch_chunk_bits<__half>(head_dim, bits, group_size, a, st)
+                   : launch_chunk_bits<__nv_bfloat16>(head_dim, bits, group_size, a, st);
+}
+
+}  // namespace lmoe

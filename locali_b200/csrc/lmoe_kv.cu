@@ -8,6 +8,7 @@
 // once.
 #include "../../include/lmoe.h"
 
+#include <cmath>
 #include <cstring>
 
 #include "lmoe_kernels.cuh"
@@ -392,7 +393,8 @@ int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, i
     a.out = static_cast<uint16_t *>(out);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    // a scale of zero (all terms equal) as one that no score makes visible: 0 times a hidden score's -inf is no number
+    a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 2e-38f);
     a.window = window > 0 ? window : 0;
     a.sinks = window > 0 ? sinks : 0;
     a.scratch = static_cast<uint8_t *>(scratch);

@@ -379,10 +379,11 @@ def test_rows_behind_the_last_sequence(built, rows):
     case = Case([100, 64], [rows, rows], bits=8, gs=32, d=64, hk=2)
     c, n = case.cache, case.n
     q = torch.randn(n + 37, 4, 64, device="cuda").to(torch.bfloat16)
-    want = c.attend(q[:n], case.table, case.lens, case.start)
     out = torch.full_like(q, 7.0)
     c.attend(q, case.table, case.lens, case.start, out=out)
-    assert torch.equal(out[:n], want) and (out[n:] == 7).all()
+    # the number of rows may choose another kernel than q[:n] alone: held to the oracle, not to those bits
+    attend_and_check(case, 4, q=q[:n], got=out[:n])
+    assert (out[n:] == 7).all()
     k, v = c.read(case.table, case.lens, case.start, rows=n)
     o = tuple(torch.full((n + 37, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
     c.read(case.table, case.lens, case.start, out=o)
