@@ -10,10 +10,10 @@
 // One block per SM; the stream of (tile, head, key block) is cut evenly over
 // the launch as in lmoe_attn.cu.  Warp roles:
 //   0-3, 4-7   softmax and output of sub-tile 0 and 1
-//   8-11       keys into shared memory; 12-15 values: 16-bit rows by cp.async,
-//              codes through registers, dequantised to the 16-bit type on the
-//              way, both into the 128-byte-swizzled operand layout
-//   16, 17     one thread each issues the MMAs of sub-tile 0, 1
+//   8-11       keys and values into shared memory: 16-bit rows by cp.async,
+//              codes through registers (one tile ahead), dequantised to the
+//              16-bit type on the way, into the 128-byte-swizzled operand layout
+//   12, 13     one thread each issues the MMAs of sub-tile 0, 1
 // The sub-tiles run apart, so one's softmax overlaps the other's MMAs.  The
 // running maximum of a row moves only when a score passes it by 2^8: until
 // then terms may exceed 1, which costs nothing in fp32 and leaves the sums in
@@ -33,18 +33,17 @@ namespace lmoe {
 namespace {
 
 constexpr int kCkRows = 256, kCkKeys = 128, kCkSub = 128;
-constexpr int kCkThreads = 18 * 32;
-constexpr int kCkKWarp = 8, kCkVWarp = 12, kCkMmaWarp = 16;
+constexpr int kCkThreads = 16 * 32;  // 14 warps work; 128 registers a thread
+constexpr int kCkLoadWarp = 8, kCkMmaWarp = 12;
 constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
 constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
 
 template <int BITS, int D, int GS>
 struct ChunkGeo {
-    static constexpr int HALVES = D / 64;
     static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
     static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
-    static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
+    static constexpr int SCALES = BITS == 16 ? 0 : 4 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
     static constexpr int SMEM = 1024 + 6 * TILE + SCALES + 1024;
 };
 
@@ -161,6 +160,111 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, uint32_t s2,
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// packed fp32 pairs
+__device__ __forceinline__ uint64_t pack_f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float &x, float &y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// largest of three, keeping a NaN
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
+// Largest visible score of the thread's row, S at `ts`; two of the four reads
+// of 32 columns are in flight at a time.  FULL: all are visible, else mask(c)
+// has the bits of columns 32 c .. 32 c + 31.
+template <bool FULL, class F>
+__device__ __forceinline__ float row_max(uint32_t ts, F &&mask, bool &seen) {
+    float x0 = -INFINITY, x1 = -INFINITY;
+    auto take = [&](uint32_t (&v)[32], int c) {
+        if constexpr (!FULL) {
+            const uint32_t mk = mask(c);
+            seen |= mk != 0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            x0 = max3_nan(x0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            x1 = max3_nan(x1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+        }
+    };
+    uint32_t v[32], y[32];
+    tmem_ld32(ts, v);
+    tmem_wait_ld32(v);
+    tmem_ld32(ts + 32, y);
+    take(v, 0);
+    tmem_wait_ld32(y);
+    tmem_ld32(ts + 64, v);
+    take(y, 1);
+    tmem_wait_ld32(v);
+    tmem_ld32(ts + 96, y);
+    take(v, 2);
+    tmem_wait_ld32(y);
+    take(y, 3);
+    if (FULL) seen = true;
+    return max_nan(x0, x1);
+}
+
+// Terms exp2(S sc - mu) over S, as 16-bit pairs for the tensor core (32
+// columns of S become 16, behind the reads); returns their sum in fp32.
+template <typename TA, bool FULL, class F>
+__device__ __forceinline__ float row_terms(uint32_t ts, F &&mask, float sc, float mu) {
+    const uint64_t sc2 = pack_f2(sc, sc), mu2 = pack_f2(-mu, -mu);
+    uint64_t sum = 0;
+    auto take = [&](uint32_t (&v)[32], int c) {
+        const uint32_t mk = FULL ? 0u : mask(c);
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            float p0, p1;
+            unpack_f2(fma_f2(pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, mu2), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            if constexpr (!FULL) {
+                if (!(mk >> e & 1u)) p0 = 0.0f;
+                if (!(mk >> (e + 1) & 1u)) p1 = 0.0f;
+            }
+            sum = add_f2(sum, pack_f2(p0, p1));
+            pk[e / 2] = Act<TA>::pack2(p0, p1);
+        }
+        tmem_st16(ts + 16 * c, pk);
+    };
+    uint32_t v[32], y[32];
+    tmem_ld32(ts, v);
+    tmem_wait_ld32(v);
+    tmem_ld32(ts + 32, y);
+    tmem_wait_ld32(y);  // read before columns 16.. are written over
+    take(v, 0);
+    tmem_ld32(ts + 64, v);
+    take(y, 1);
+    tmem_wait_ld32(v);
+    tmem_ld32(ts + 96, y);
+    take(v, 2);
+    tmem_wait_ld32(y);
+    take(y, 3);
+    float s0, s1;
+    unpack_f2(sum, s0, s1);
+    return s0 + s1;
+}
+
 template <typename TA, int BITS, int D, int GS>
 __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArgs a) {
     using G = ChunkGeo<BITS, D, GS>;
@@ -227,7 +331,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     Walk w;
     w.begin(first, run);
 
-    if (warp < kCkKWarp) {
+    if (warp < kCkLoadWarp) {
         // ---------------------------------------------------- softmax and output
         const int t = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;  // row of the sub-tile
         const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
@@ -281,7 +385,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const int smin = ti.first + (ti.rt * kCkRows + t * kCkSub) / a.group;
                 const int smax = ti.first + (ti.rt * kCkRows + lastrow) / a.group;
                 float m = -INFINITY;
-                float l0 = 0.0f, l1 = 0.0f;
+                float l = 0.0f;
                 bool seen = false;
                 int parts = 0;
                 for (int i = b0; i < b1; ++i, ++u, ++act) {
@@ -305,33 +409,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         if (bad >> (2 * c) & 2u) x &= 0x0000FFFFu;
                         return x;
                     };
-                    float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(tm_s(t) + lanes + 32 * c, v);
-                        tmem_wait_ld32(v);
-                        if (!full) {
-                            const uint32_t mk = mask(c);
-                            seen |= mk != 0;
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            x0 = max_nan(x0, __uint_as_float(v[e]));
-                            x1 = max_nan(x1, __uint_as_float(v[e + 1]));
-                        }
-                    }
-                    if (full) seen = true;
-                    const float x = max_nan(x0, x1) * sc;
+                    const float x = (full ? row_max<true>(tm_s(t) + lanes, mask, seen)
+                                          : row_max<false>(tm_s(t) + lanes, mask, seen)) * sc;
                     const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
                     if (__any_sync(0xffffffffu, move)) {
                         const float f = move ? ex2(m - x) : 1.0f;
                         if (move) m = x;
-                        l0 *= f;
-                        l1 *= f;
+                        l *= f;
                         if (i > b0) {  // the sums so far
 #pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
@@ -345,26 +429,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         }
                     }
                     const float mu = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32], pk[16];
-                        tmem_ld32(tm_s(t) + lanes + 32 * c, v);
-                        tmem_wait_ld32(v);
-                        const uint32_t mk = full ? 0xFFFFFFFFu : mask(c);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float p0 = ex2(fmaf(__uint_as_float(v[e]), sc, -mu));
-                            float p1 = ex2(fmaf(__uint_as_float(v[e + 1]), sc, -mu));
-                            if (!full) {
-                                if (!(mk >> e & 1u)) p0 = 0.0f;
-                                if (!(mk >> (e + 1) & 1u)) p1 = 0.0f;
-                            }
-                            l0 += p0;
-                            l1 += p1;
-                            pk[e / 2] = Act<TA>::pack2(p0, p1);
-                        }
-                        tmem_st16(tm_s(t) + lanes + 16 * c, pk);
-                    }
+                    l += full ? row_terms<TA, true>(tm_s(t) + lanes, mask, sc, mu)
+                              : row_terms<TA, false>(tm_s(t) + lanes, mask, sc, mu);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -377,7 +443,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 if (!ok) break;
                 tc_fence_after();
                 if (r == 0) mbar_arrive(&vempty[(u - 1) & 1]);
-                float l = l0 + l1;
                 // only scores of -inf: the softmax is no number, unless other
                 // parts of the tile's keys hold larger ones
                 if (m == -INFINITY && seen) l = __uint_as_float(0x7FC00000u);
@@ -461,11 +526,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         }
     } else if (warp < kCkMmaWarp) {
         // ---------------------------------------------------- keys and values
-        const int which = warp >= kCkVWarp, lw = (warp - kCkKWarp) & 3;
-        uint64_t *fullb = which ? vfull : kfull, *emptyb = which ? vempty : kempty;
-        const uint32_t base = sb + (which ? G::OFF_V : G::OFF_K);
+        const int lw = warp - kCkLoadWarp;  // rows 32 lw .. of a block
         constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of a warp's 32
         const int rr = lane / LPR, cc = lane % LPR;
+        const int64_t lane_off = (int64_t)rr * RB + cc * BITS;  // the lane's part of a round's rows
         int i = w.b0, segs = 0, parts = 0;
         bool have = true;
         // the block at hand: head row of 16-position run 0, 1 of the warp's (-2: none, -1: no page), its facts
@@ -502,96 +566,142 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             const long long r = x < 16 ? n.r0 : n.r1;
             return r >= 0 && n.k0 + lw * 32 + x < n.hi ? r + (x & 15) : -1;
         };
-        auto facts = [&](const Unit &n, int u, uint32_t taken) {
+        // all of the warp's 32 rows are there
+        auto whole = [&](const Unit &n) { return n.r0 >= 0 && n.r1 >= 0 && n.k0 + lw * 32 + 32 <= n.hi; };
+        auto dst_of = [&](auto which, int u) {
+            return sb + (decltype(which)::value ? G::OFF_V : G::OFF_K) + (u & 1) * G::TILE;
+        };
+        auto empty = [&](auto which, int u) -> bool {
+            uint64_t *b = decltype(which)::value ? vempty : kempty;
+            return __all_sync(0xffffffffu, wait(&b[u & 1], (u >> 1 & 1) ^ 1));
+        };
+        // the tile is in place; taken: rows of the warp's with values taken out
+        auto done = [&](auto which, const Unit &n, int u, uint32_t taken) {
+            constexpr bool V = decltype(which)::value;
             if (lane == 0) {
-                if (!which) s_bad[u & 3][lw] = (n.r0 == -1) | (n.r1 == -1) << 1;
+                if (!V) s_bad[u & 3][lw] = (n.r0 == -1) | (n.r1 == -1) << 1;
                 else if (n.part >= 0) {
                     s_poison[n.seg & 3][n.part][lw] = taken;
                     if (lw == 0) s_pblk[n.seg & 3][n.part] = n.k0 / kCkKeys;
                 }
             }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(V ? &vfull[u & 1] : &kfull[u & 1]);
         };
-        bool ok = true;
+        using Keys = std::integral_constant<bool, false>;
+        using Values = std::integral_constant<bool, true>;
         if constexpr (Q) {
             constexpr int WPC = BITS == 8 ? 2 : 1;  // code words of a chunk
             uint32_t code[IT][WPC];
             uint32_t sbp[NG];  // (scale, bias) of row `lane`
-            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + (warp - kCkKWarp) * 32 * NG;
-            auto fetch = [&](const Unit &n, int x) {
-                const long long r = row_of(n, x * RPI + rr);
-                const uint8_t *src = a.c.kv[which] + r * RB + cc * BITS;
+            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + lw * 32 * NG;
+            // round x of a tile: rows x RPI + rr; `run`: the lane's part of the rows of round 0 (or 16 / RPI)
+            auto fetch = [&](const uint8_t *run, bool in, int x) {
+                const uint8_t *src = run + (x * RPI % 16) * RB;
                 if constexpr (BITS == 8) {
-                    const uint2 v = r >= 0 ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
+                    const uint2 v = in ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
                     code[x][0] = v.x;
                     code[x][1] = v.y;
                 } else {
-                    code[x][0] = r >= 0 ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+                    code[x][0] = in ? *reinterpret_cast<const uint32_t *>(src) : 0u;
                 }
             };
-            auto fetch_scales = [&](const Unit &n) {
+            auto fetch_part = [&](auto which, const Unit &n, int x) {
+                const long long r = x * RPI < 16 ? n.r0 : n.r1;
+                fetch(a.c.kv[decltype(which)::value] + lane_off + r * RB, row_of(n, x * RPI + rr) >= 0, x);
+            };
+            auto fetch_scales = [&](auto which, const Unit &n) {
+                constexpr int W = decltype(which)::value;
                 const long long r = row_of(n, lane);
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
-                    sbp[g] = r >= 0 ? (uint32_t)a.c.scale[which][r * NG + g] | (uint32_t)a.c.bias[which][r * NG + g] << 16 : 0u;
+                    sbp[g] = r >= 0 ? (uint32_t)a.c.scale[W][r * NG + g] | (uint32_t)a.c.bias[W][r * NG + g] << 16 : 0u;
             };
-            Unit n = unit();
-            fetch_scales(n);
+            // writes tile u (codes and scales are in registers) and fetches the next one behind it
+            auto tile = [&](auto which, const Unit &n, int u, auto nwhich, const Unit &nx, bool next) -> bool {
+                constexpr bool V = decltype(which)::value;
+                constexpr int NW = decltype(nwhich)::value;
+                if (!empty(which, u)) return false;
+                bool no = false;
 #pragma unroll
-            for (int x = 0; x < IT; ++x) fetch(n, x);
-            step();
-            for (int u = 0; !s_abort; ++u) {
-                ok = __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1));
-                if (!ok) break;
-                uint32_t taken = 0;
-                {
-                    bool no = false;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        // in a block that only some rows see, values that are no numbers are taken out
-                        if (which && n.part >= 0 && nonfinite2<TA>(sbp[g])) {
-                            no = true;
-                            sbp[g] = 0;
-                        }
-                        const uint32_t s = Pair<TA>::template scale<BITS>(sbp[g]) & 0xFFFFu;
-                        spair[lane * NG + g] = s | (sbp[g] & 0xFFFF0000u);
+                for (int g = 0; g < NG; ++g) {
+                    // in a block that only some rows see, values that are no numbers are taken out
+                    if (V && n.part >= 0 && nonfinite2<TA>(sbp[g])) {
+                        no = true;
+                        sbp[g] = 0;
                     }
-                    taken = __ballot_sync(0xffffffffu, no);
+                    const uint32_t s = Pair<TA>::template scale<BITS>(sbp[g]) & 0xFFFFu;
+                    spair[lane * NG + g] = s | (sbp[g] & 0xFFFF0000u);
                 }
-                facts(n, u, taken);
+                const uint32_t taken = __ballot_sync(0xffffffffu, no);
                 __syncwarp();
-                const bool next = have;
-                Unit nx = n;
-                if (next) {
-                    nx = unit();
-                    fetch_scales(nx);
-                }
-                const uint32_t dst = base + (u & 1) * G::TILE;
-#pragma unroll
-                for (int x = 0; x < IT; ++x) {
-                    const int row = lw * 32 + x * RPI + rr;
-                    const uint32_t sbv = spair[(x * RPI + rr) * NG + cc * 8 / GS];
+                if (next) fetch_scales(nwhich, nx);
+                const uint32_t dst = dst_of(which, u);
+                const uint32_t *sp = spair + rr * NG + cc * 8 / GS;
+                auto put = [&](int x) {
+                    const uint32_t sbv = sp[x * RPI * NG];
                     const uint4 v = dequant8<TA, BITS>(code[x][0], code[x][WPC - 1], __byte_perm(sbv, 0u, 0x1010),
                                                        __byte_perm(sbv, 0u, 0x3232));
-                    sts128v(dst + op_off(row, cc), v.x, v.y, v.z, v.w);
-                    if (next) fetch(nx, x);
+                    sts128v(dst + op_off(lw * 32 + x * RPI + rr, cc), v.x, v.y, v.z, v.w);
+                };
+                // each round's registers are filled for the next tile as they come free
+                if (next && whole(nx)) {
+                    const uint8_t *p0 = a.c.kv[NW] + lane_off + nx.r0 * RB, *p1 = a.c.kv[NW] + lane_off + nx.r1 * RB;
+#pragma unroll
+                    for (int x = 0; x < IT; ++x) {
+                        put(x);
+                        fetch(x * RPI < 16 ? p0 : p1, true, x);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < IT; ++x) {
+                        put(x);
+                        if (next) fetch_part(nwhich, nx, x);
+                    }
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&fullb[u & 1]);
-                if (!next) break;
-                n = nx;
+                done(which, n, u, taken);
+                return true;
+            };
+            Unit n = unit();
+            fetch_scales(Keys{}, n);
+#pragma unroll
+            for (int x = 0; x < IT; ++x) fetch_part(Keys{}, n, x);
+            for (int u = 0; !s_abort; ++u) {
+                if (!tile(Keys{}, n, u, Values{}, n, true)) break;
                 step();
+                const bool next = have;
+                const Unit nx = next ? unit() : n;
+                if (!tile(Values{}, n, u, Keys{}, nx, next) || !next) break;
+                n = nx;
             }
         } else {
-            Unit prev;
-            auto finish = [&](const Unit &n, int u) {
+            auto copy = [&](auto which, const Unit &n, int u) {
+                const uint8_t *kv = a.c.kv[decltype(which)::value];
+                const uint32_t dst = dst_of(which, u);
+                if (whole(n)) {
+                    const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
+#pragma unroll
+                    for (int x = 0; x < IT; ++x)
+                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
+                } else {
+#pragma unroll 1
+                    for (int x = 0; x < IT; ++x) {
+                        const long long r = row_of(n, x * RPI + rr);
+                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv, r >= 0 ? 16 : 0);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            // the copies of a tile have landed
+            auto finish = [&](auto which, const Unit &n, int u) {
                 uint32_t taken = 0;
-                if (which && n.part >= 0) {
+                if (decltype(which)::value && n.part >= 0) {
                     __syncwarp();
 #pragma unroll 1
                     for (int x = 0; x < IT; ++x) {
                         const int row = x * RPI + rr;
-                        const uint32_t at = base + (u & 1) * G::TILE + op_off(lw * 32 + row, cc);
+                        const uint32_t at = dst_of(which, u) + op_off(lw * 32 + row, cc);
                         uint4 v = lds128(at);
                         uint32_t *vv = &v.x;
                         bool no = false;
@@ -609,36 +719,34 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                             if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken |= 1u << (x * RPI + y);
                     }
                 }
-                facts(n, u, taken);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&fullb[u & 1]);
+                done(which, n, u, taken);
             };
+            // one tile is in flight while the one before it is completed
+            Unit prev{};
             int u = 0;
+            bool ok = true;
             for (; have && !s_abort; ++u) {
                 const Unit n = unit();
                 step();
-                ok = __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1));
+                ok = empty(Keys{}, u);
                 if (!ok) break;
-                const uint32_t dst = base + (u & 1) * G::TILE;
-#pragma unroll
-                for (int x = 0; x < IT; ++x) {
-                    const int row = x * RPI + rr;
-                    const long long r = row_of(n, row);
-                    cpa16(dst + op_off(lw * 32 + row, cc), r >= 0 ? a.c.kv[which] + r * RB + cc * 16 : a.c.kv[which],
-                          r >= 0 ? 16 : 0);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                copy(Keys{}, n, u);
                 if (u > 0) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    finish(prev, u - 1);
+                    finish(Values{}, prev, u - 1);
                 }
+                ok = empty(Values{}, u);
+                if (!ok) break;
+                copy(Values{}, n, u);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                finish(Keys{}, n, u);
                 prev = n;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (ok && u > 0) finish(prev, u - 1);
+            if (ok && u > 0) finish(Values{}, prev, u - 1);
         }
-    } else if (lane == 0) {
+    }
+    if (warp >= kCkMmaWarp && warp < kCkMmaWarp + 2 && lane == 0) {
         // ---------------------------------------------------- MMAs of sub-tile t
         const int t = warp - kCkMmaWarp;
         const uint32_t id_s = attn_idesc(kCkKeys, F16, false), id_o = attn_idesc(D, F16, true);
@@ -687,7 +795,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
-    if (s_abort && warp >= kCkMmaWarp && lane == 0) {
+    if (s_abort && warp >= kCkMmaWarp && warp < kCkMmaWarp + 2 && lane == 0) {
         // a wait gave up: nothing may still write tensor memory when it is freed
         uint64_t *b = &sfull[warp - kCkMmaWarp];
         umma_commit(b);
