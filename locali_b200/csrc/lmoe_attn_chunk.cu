@@ -14,7 +14,13 @@
 //              codes through registers (one tile ahead), dequantised to the
 //              16-bit type on the way, into the 128-byte-swizzled operand layout
 //   12, 13     one thread each issues the MMAs of sub-tile 0, 1
-// The sub-tiles run apart, so one's softmax overlaps the other's MMAs.  The
+//   14         walks the launch block's tiles and lays what the others need to
+//              know of them into a ring in shared memory
+// The sub-tiles issue their MMAs (P V of a block, then S of the next) in turn,
+// which keeps them half a block apart: one's softmax overlaps the other's
+// MMAs.  Issued as they came, the MMAs of both interleaved and ended together,
+// and the two softmaxes then shared the exponential unit while the tensor pipe
+// waited.  The
 // running maximum of a row moves only when a score passes it by 2^8: until
 // then terms may exceed 1, which costs nothing in fp32 and leaves the sums in
 // tensor memory untouched (a row's result is the quotient either way).
@@ -33,8 +39,9 @@ namespace lmoe {
 namespace {
 
 constexpr int kCkRows = 256, kCkKeys = 128, kCkSub = 128;
-constexpr int kCkThreads = 16 * 32;  // 14 warps work; 128 registers a thread
-constexpr int kCkLoadWarp = 8, kCkMmaWarp = 12;
+constexpr int kCkThreads = 16 * 32;  // 15 warps work; 128 registers a thread
+constexpr int kCkLoadWarp = 8, kCkMmaWarp = 12, kCkWalkWarp = 14;
+constexpr int kSegs = 8;  // tiles in the ring: the loader is at most 3 ahead of the output
 constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
 constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
 
@@ -47,27 +54,12 @@ struct ChunkGeo {
     static constexpr int SMEM = 1024 + 6 * TILE + SCALES + 1024;
 };
 
-// Walks the key blocks of a launch block's run, tile by tile.
-struct Walk {
-    Cursor cur;
-    long long left;
-    int b0, b1;  // blocks of the current tile that are this launch block's
-    __device__ __forceinline__ void begin(const Cursor &c, long long n) {
-        cur = c;
-        left = n;
-        open();
-    }
-    __device__ __forceinline__ void open() {
-        b0 = cur.blk;
-        b1 = (int)min((long long)cur.t.nblk, b0 + left);
-        left -= b1 - b0;
-    }
-    __device__ __forceinline__ bool next(const AttnArgs &a) {
-        if (left <= 0) return false;
-        next_tile<kCkRows, kCkKeys>(a, cur);
-        open();
-        return true;
-    }
+// A tile, and the blocks of it that are this launch block's.
+struct Seg {
+    Tile t;
+    int b0, b1;
+    int more;   // another one follows
+    int parts;  // launch blocks that share the tile, if it begins here and goes on behind; else 0
 };
 
 // every row of the tile sees every position of the block at k0
@@ -223,6 +215,71 @@ __device__ __forceinline__ float row_max(uint32_t ts, F &&mask, bool &seen) {
     return max_nan(x0, x1);
 }
 
+// Terms over S with the running maximum m as it is, in one read of S; nothing
+// is written (again = true) when a score of a row of the warp passes its
+// maximum by more than 2^8 or is no number.
+template <typename TA, bool FULL, class F>
+__device__ __forceinline__ float row_try(uint32_t ts, F &&mask, float sc, float m, float &x, bool &seen, bool &again) {
+    const float mu = m == -INFINITY ? 0.0f : m;
+    const uint64_t sc2 = pack_f2(sc, sc), mu2 = pack_f2(-mu, -mu);
+    uint64_t sum = 0;
+    float x0 = -INFINITY, x1 = -INFINITY;
+    uint32_t pk[64];
+    bool any = FULL;
+    auto take = [&](uint32_t (&v)[16], int c) {  // columns 16 c ..
+        uint32_t mk = 0;
+        if constexpr (!FULL) {
+            mk = mask(c >> 1) >> (16 * (c & 1)) & 0xFFFFu;
+            any |= mk != 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            x0 = max3_nan(x0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            x1 = max3_nan(x1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            float p0, p1;
+            unpack_f2(fma_f2(pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, mu2), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            sum = add_f2(sum, pack_f2(p0, p1));
+            pk[8 * c + e / 2] = Act<TA>::pack2(p0, p1);
+        }
+    };
+    uint32_t v[16], y[16];
+    tmem_ld16(ts, v);
+    tmem_wait_ld(v);
+#pragma unroll
+    for (int c = 0; c < 8; c += 2) {
+        tmem_ld16(ts + 16 * (c + 1), y);
+        take(v, c);
+        tmem_wait_ld(y);
+        if (c < 6) tmem_ld16(ts + 16 * (c + 2), v);
+        take(y, c + 1);
+        if (c < 6) tmem_wait_ld(v);
+    }
+    x = max_nan(x0, x1) * sc;
+    const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
+    again = __any_sync(0xffffffffu, move);
+    if (!again) {
+        seen |= any;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t z[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) z[e] = pk[32 * h + e];
+            tmem_st32(ts + 32 * h, z);
+        }
+    }
+    float s0, s1;
+    unpack_f2(sum, s0, s1);
+    return s0 + s1;
+}
+
 // Terms exp2(S sc - mu) over S, as 16-bit pairs for the tensor core (32
 // columns of S become 16, behind the reads); returns their sum in fp32.
 template <typename TA, bool FULL, class F>
@@ -278,13 +335,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     __shared__ __align__(16) uint32_t s_bad[4][4];  // block u & 3: the key warps' runs without a page
     __shared__ uint32_t s_poison[4][kPoison][4];    // tile & 3, its n-th block seen in part: rows taken out
     __shared__ int s_pblk[4][kPoison];
-    __shared__ uint64_t bars[16];
+    __shared__ uint64_t bars[18 + 2 * kSegs];
+    __shared__ Seg s_seg[kSegs];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     uint8_t *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
     uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *sfull = bars + 8,
-             *pfull = bars + 10, *qfull = bars + 12, *ofull = bars + 14;
+             *pfull = bars + 10, *qfull = bars + 12, *ofull = bars + 14, *turn = bars + 16,
+             *gfull = bars + 18, *gempty = gfull + kSegs;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -296,6 +355,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             mbar_init(&pfull[i], 4);
             mbar_init(&qfull[i], 4);
             mbar_init(&ofull[i], 1);
+            mbar_init(&turn[i], 1);
+        }
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(&gfull[i], 1);
+            mbar_init(&gempty[i], kCkWalkWarp);
         }
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -328,8 +392,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         set_error(a.r.err, kErrCuda);
         return false;
     };
-    Walk w;
-    w.begin(first, run);
+    // the launch block's n-th tile; let go (by one lane of each warp) when nothing more of it is needed
+    auto seg = [&](int n) -> const Seg & { return s_seg[n % kSegs]; };
+    auto seg_ready = [&](int n) -> bool { return wait(&gfull[n % kSegs], n / kSegs & 1); };
+    auto seg_done = [&](int n) { mbar_arrive(&gempty[n % kSegs]); };
 
     if (warp < kCkLoadWarp) {
         // ---------------------------------------------------- softmax and output
@@ -348,14 +414,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             for (int c = 0; c < CH; ++c) cpa16(qs + op_off(r, c), in ? src + c * 8 : a.q, in ? 16 : 0);
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        load_q(w.cur.t);
-        int u = 0, act = 0, segs = 0, active_segs = 0;
-        bool ok = true;
-        while (ok && !s_abort) {
-            const Tile ti = w.cur.t;
-            const int b0 = w.b0, b1 = w.b1;
-            const long long tile_begin = w.cur.tile_begin;
-            const bool more = w.next(a);  // w: the tile after this one
+        int u = 0, act = 0, active_segs = 0;
+        bool ok = __all_sync(0xffffffffu, seg_ready(0));
+        if (ok) load_q(seg(0).t);
+        for (int n = 0; ok && !s_abort; ++n) {
+            const Seg &sg = seg(n);
+            const Tile &ti = sg.t;
+            const int b0 = sg.b0, b1 = sg.b1, more = sg.more;
             if (t == 1 && ti.rows <= kCkSub) {
                 // no rows: only pass the tiles of keys and values on
                 if (r == 0)
@@ -367,9 +432,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         if (ok) mbar_arrive(&vempty[s]);
                     }
                 u += b1 - b0;
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, ok && (!more || seg_ready(n + 1)));
                 asm volatile("cp.async.wait_group 0;" ::: "memory");  // before the same rows are written again
-                if (more) load_q(w.cur.t);
+                if (ok && more) load_q(seg(n + 1).t);
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 fence_proxy_async();
@@ -382,6 +447,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const int see_sink = min(a.sinks, see_hi);
                 // positions of the sub-tile's first and last row
                 const int lastrow = min(ti.rows, (t + 1) * kCkSub) - 1;
+                const int nsink = ti.nsink, lo = ti.lo - nsink;
+                const int tmin = ti.minpos, tmax = ti.maxpos;
                 const int smin = ti.first + (ti.rt * kCkRows + t * kCkSub) / a.group;
                 const int smax = ti.first + (ti.rt * kCkRows + lastrow) / a.group;
                 float m = -INFINITY;
@@ -389,7 +456,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 bool seen = false;
                 int parts = 0;
                 for (int i = b0; i < b1; ++i, ++u, ++act) {
-                    const int k0 = ti.block(i) * kCkKeys;
+                    const int k0 = (i < nsink ? i : lo + i) * kCkKeys;
                     ok = __all_sync(0xffffffffu, wait(&sfull[t], act & 1));
                     if (!ok) break;
                     tc_fence_after();
@@ -397,11 +464,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         mbar_arrive(&kempty[u & 1]);
                         if (i > b0) mbar_arrive(&vempty[(u - 1) & 1]);
                     }
-                    if (i == b1 - 1 && more) load_q(w.cur.t);  // Q_t is free
+                    if (i == b1 - 1 && more) {  // Q_t is free
+                        ok = __all_sync(0xffffffffu, seg_ready(n + 1));
+                        if (!ok) break;
+                        load_q(seg(n + 1).t);
+                    }
                     const uint4 bw = *reinterpret_cast<const uint4 *>(s_bad[u & 3]);
                     const uint32_t bad = bw.x | bw.y << 2 | bw.z << 4 | bw.w << 6;
                     const bool full = !bad && block_full(a, k0, smin, smax);
-                    if (!block_full(a, k0, ti.minpos, ti.maxpos)) ++parts;
+                    if (!block_full(a, k0, tmin, tmax)) ++parts;
                     auto mask = [&](int c) -> uint32_t {
                         const int kb = k0 + 32 * c;
                         uint32_t x = range_bits(see_lo, see_hi, kb) | range_bits(0, see_sink, kb);
@@ -409,10 +480,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         if (bad >> (2 * c) & 2u) x &= 0x0000FFFFu;
                         return x;
                     };
-                    const float x = (full ? row_max<true>(tm_s(t) + lanes, mask, seen)
-                                          : row_max<false>(tm_s(t) + lanes, mask, seen)) * sc;
-                    const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
-                    if (__any_sync(0xffffffffu, move)) {
+                    // with the maximum as it is, unless a score of the block passes it
+                    const uint32_t ts = tm_s(t) + lanes;
+                    bool again = true;
+                    if (i > b0) {
+                        float x;
+                        const float sum = full ? row_try<TA, true>(ts, mask, sc, m, x, seen, again)
+                                               : row_try<TA, false>(ts, mask, sc, m, x, seen, again);
+                        if (!again) l += sum;
+                    }
+                    if (again) {
+                        const float x = (full ? row_max<true>(ts, mask, seen) : row_max<false>(ts, mask, seen)) * sc;
+                        const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
                         const float f = move ? ex2(m - x) : 1.0f;
                         if (move) m = x;
                         l *= f;
@@ -427,10 +506,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                                 tmem_st32(tm_o(t) + lanes + 32 * c, v);
                             }
                         }
+                        const float mu = m == -INFINITY ? 0.0f : m;
+                        l += full ? row_terms<TA, true>(ts, mask, sc, mu) : row_terms<TA, false>(ts, mask, sc, mu);
                     }
-                    const float mu = m == -INFINITY ? 0.0f : m;
-                    l += full ? row_terms<TA, true>(tm_s(t) + lanes, mask, sc, mu)
-                              : row_terms<TA, false>(tm_s(t) + lanes, mask, sc, mu);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -453,9 +531,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 float *part = part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) +
                               (t * kCkSub + r) * D;
                 bool poisoned = false;
-                for (int n = 0; n < parts; ++n)
-                    poisoned |= (s_poison[segs & 3][n][0] | s_poison[segs & 3][n][1] | s_poison[segs & 3][n][2] |
-                                 s_poison[segs & 3][n][3]) != 0;
+                for (int pi = 0; pi < parts; ++pi)
+                    poisoned |= (s_poison[n & 3][pi][0] | s_poison[n & 3][pi][1] | s_poison[n & 3][pi][2] | s_poison[n & 3][pi][3]) != 0;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t v[32];
@@ -464,10 +541,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     if (poisoned) {
                         // values that are no numbers, taken out of blocks that
                         // only some rows see: added for those that do
-                        for (int n = 0; n < parts; ++n)
+                        for (int pi = 0; pi < parts; ++pi)
                             for (int k = 0; k < kCkKeys; ++k) {
-                                if (!(s_poison[segs & 3][n][k >> 5] >> (k & 31) & 1u)) continue;
-                                const int j = s_pblk[segs & 3][n] * kCkKeys + k;
+                                if (!(s_poison[n & 3][pi][k >> 5] >> (k & 31) & 1u)) continue;
+                                const int j = s_pblk[n & 3][pi] * kCkKeys + k;
                                 if (!(j < see_hi && (j >= see_lo || j < see_sink))) continue;
                                 const int32_t pg = a.r.page(a.c, ti.b, j);
                                 if (pg < 0) continue;
@@ -512,16 +589,17 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     float2 *ml = reinterpret_cast<float2 *>(part - (t * kCkSub + r) * D + kCkRows * D);
                     ml[t * kCkSub + r] = make_float2(m, l);
                 }
-                if (t == 0 && r == 0 && b0 == 0 && b1 < ti.nblk) {
+                if (t == 0 && r == 0 && sg.parts) {
                     rec->out0 = ti.row0;
                     rec->row = ti.rt * kCkRows;
                     rec->rows_h = ti.rows | ti.h << 16;
-                    rec->parts = sh.owner(tile_begin + ti.nblk - 1) - blockIdx.x + 1;
+                    rec->parts = sg.parts;
                 }
                 // O_t is read: the next tile's first P_t says so
                 tc_fence_before();
             }
-            ++segs;
+            __syncwarp();
+            if (lane == 0) seg_done(n);
             if (!more) break;
         }
     } else if (warp < kCkMmaWarp) {
@@ -530,36 +608,64 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of a warp's 32
         const int rr = lane / LPR, cc = lane % LPR;
         const int64_t lane_off = (int64_t)rr * RB + cc * BITS;  // the lane's part of a round's rows
-        int i = w.b0, segs = 0, parts = 0;
+        // the walk: block i of tile n, in blocks [.., b1)
+        int i = 0, b1 = 0, n_seg = -1, parts = 0, more = 1;
         bool have = true;
-        // the block at hand: head row of 16-position run 0, 1 of the warp's (-2: none, -1: no page), its facts
+        // A block of the walk: head row of 16-position run 0, 1 of the warp's
+        // (-2: none, -1: no page), its facts.  Lanes 0 and 1 look the pages
+        // up; a block's page ids are asked for while the one before it is
+        // worked on (ask), and looked at when they have come (take).
         struct Unit {
             long long r0, r1;
             int k0, hi, seg, part;  // part: its number among the blocks seen in part, -1: seen in full
         };
-        auto unit = [&]() -> Unit {
-            Unit x;
-            const Tile &ti = w.cur.t;
-            x.k0 = ti.block(i) * kCkKeys;
-            x.hi = ti.hi;
-            x.seg = segs;
-            x.part = block_full(a, x.k0, ti.minpos, ti.maxpos) ? -1 : parts++;
-            long long r = -2;
-            const int p = x.k0 + lw * 32 + lane * 16;
+        Unit ahead{};
+        int32_t a_page = 0;
+        int a_slot = 0, a_head = 0;  // a_slot < 0: the lane has no run
+        bool asked = false;
+        auto ask = [&]() {
+            if (i == b1) {
+                if (n_seg >= 0) {
+                    __syncwarp();
+                    if (lane == 0) seg_done(n_seg);
+                }
+                have = more && __all_sync(0xffffffffu, seg_ready(n_seg + 1));
+                if (have) {
+                    const Seg &sg = seg(++n_seg);
+                    i = sg.b0;
+                    b1 = sg.b1;
+                    more = sg.more;
+                    parts = 0;
+                }
+            }
+            asked = have;
+            if (!have) return;
+            const Tile &ti = seg(n_seg).t;
+            ahead.k0 = ti.block(i) * kCkKeys;
+            ahead.hi = ti.hi;
+            ahead.seg = n_seg;
+            ahead.part = block_full(a, ahead.k0, ti.minpos, ti.maxpos) ? -1 : parts++;
+            const int p = ahead.k0 + lw * 32 + lane * 16;
+            a_slot = -1;
+            a_head = ti.h;
             if (lane < 2 && p < ti.hi) {
-                const int32_t pg = a.r.page(a.c, ti.b, p);
-                r = pg < 0 ? -1 : a.c.row(pg, ti.h, p % a.c.page_size);
+                const int e = p / a.c.page_size;
+                a_slot = p - e * a.c.page_size;
+                a_page = e < a.r.table_width ? a.r.table[(int64_t)ti.b * a.r.table_stride + e] : -1;
+            }
+            ++i;
+        };
+        auto take = [&]() -> Unit {
+            Unit x = ahead;
+            long long r = -2;
+            if (a_slot >= 0) {
+                const bool in = a_page >= 0 && a_page < a.c.n_pages;
+                if (!in) set_error(a.r.err, kErrIndex);
+                r = in ? a.c.row(a_page, a_head, a_slot) : -1;
             }
             x.r0 = __shfl_sync(0xffffffffu, r, 0);
             x.r1 = __shfl_sync(0xffffffffu, r, 1);
             return x;
-        };
-        auto step = [&]() {
-            if (++i < w.b1) return;
-            have = w.next(a);
-            i = w.b0;
-            ++segs;
-            parts = 0;
         };
         // head row of the warp's row x, -1 where there is nothing to read
         auto row_of = [&](const Unit &n, int x) -> long long {
@@ -663,15 +769,17 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 done(which, n, u, taken);
                 return true;
             };
-            Unit n = unit();
+            ask();
+            Unit n = take();
             fetch_scales(Keys{}, n);
 #pragma unroll
             for (int x = 0; x < IT; ++x) fetch_part(Keys{}, n, x);
+            ask();
             for (int u = 0; !s_abort; ++u) {
                 if (!tile(Keys{}, n, u, Values{}, n, true)) break;
-                step();
-                const bool next = have;
-                const Unit nx = next ? unit() : n;
+                const bool next = asked;
+                const Unit nx = next ? take() : n;
+                ask();
                 if (!tile(Values{}, n, u, Keys{}, nx, next) || !next) break;
                 n = nx;
             }
@@ -725,9 +833,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             Unit prev{};
             int u = 0;
             bool ok = true;
-            for (; have && !s_abort; ++u) {
-                const Unit n = unit();
-                step();
+            ask();
+            for (; asked && !s_abort; ++u) {
+                const Unit n = take();
+                ask();
                 ok = empty(Keys{}, u);
                 if (!ok) break;
                 copy(Keys{}, n, u);
@@ -758,39 +867,59 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const uint64_t o = (uint64_t)((s >> 2) * (16384 >> 4) + (s & 3) * 2);
                 umma_f16(tm_s(t), qd + o, kd + o, id_s, s ? 1u : 0u);
             }
-            umma_commit(&sfull[t]);
         };
         int u = 0, act = 0, active_segs = 0;
         bool ok = true;
-        while (ok && !s_abort) {
-            const int nb = w.b1 - w.b0;
-            if (t == 1 && w.cur.t.rows <= kCkSub) {
-                u += nb;
+        for (int n = 0; !s_abort; ++n) {
+            if (!seg_ready(n)) break;
+            const int nb = seg(n).b1 - seg(n).b0, rows = seg(n).t.rows, more = seg(n).more;
+            seg_done(n);
+            if (t == 1 && rows <= kCkSub) {
+                for (int j = 0; j < nb && ok; ++j, ++u) {  // only pass the turn on
+                    ok = wait(&turn[1], u & 1);
+                    if (ok) mbar_arrive(&turn[0]);
+                }
             } else {
                 ok = wait(&qfull[t], active_segs & 1) && wait(&kfull[u & 1], u >> 1 & 1);
                 ++active_segs;
                 if (!ok) break;
                 tc_fence_after();
                 scores(u);
+                umma_commit(&sfull[t]);
                 for (int j = 0; j < nb; ++j, ++u, ++act) {
-                    ok = wait(&vfull[u & 1], u >> 1 & 1) && wait(&pfull[t], act & 1);
+                    const bool last = j + 1 == nb;
+                    ok = wait(&vfull[u & 1], u >> 1 & 1) && (last || wait(&kfull[(u + 1) & 1], (u + 1) >> 1 & 1)) &&
+                         wait(&pfull[t], act & 1) && wait(&turn[t], t ? u & 1 : (u & 1) ^ 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = mn128_desc(sb + G::OFF_V + (u & 1) * G::TILE);
 #pragma unroll
                     for (int s = 0; s < kCkKeys / 16; ++s)
                         umma_f16_ts(tm_o(t), tm_s(t) + 8 * s, vd + (uint64_t)(s * (2048 >> 4)), id_o, j || s ? 1u : 0u);
-                    if (j + 1 < nb) {
-                        ok = wait(&kfull[(u + 1) & 1], (u + 1) >> 1 & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(u + 1);
-                    } else {
-                        umma_commit(&ofull[t]);
-                    }
+                    if (!last) scores(u + 1);
+                    mbar_arrive(&turn[t ^ 1]);
+                    umma_commit(last ? &ofull[t] : &sfull[t]);
                 }
             }
-            if (!ok || !w.next(a)) break;
+            if (!ok || !more) break;
+        }
+    } else if (warp == kCkWalkWarp && lane == 0) {
+        // ---------------------------------------------------- the walk
+        long long left = run;
+        for (int n = 0; !s_abort; ++n) {
+            if (n >= kSegs && !wait(&gempty[n % kSegs], (n / kSegs - 1) & 1)) break;
+            Seg &sg = s_seg[n % kSegs];
+            sg.t = first.t;
+            sg.b0 = first.blk;
+            sg.b1 = (int)min((long long)first.t.nblk, first.blk + left);
+            left -= sg.b1 - sg.b0;
+            sg.more = left > 0;
+            sg.parts = sg.b0 == 0 && sg.b1 < first.t.nblk
+                           ? sh.owner(first.tile_begin + first.t.nblk - 1) - (int)blockIdx.x + 1
+                           : 0;
+            mbar_arrive(&gfull[n % kSegs]);
+            if (left <= 0) break;
+            next_tile<kCkRows, kCkKeys>(a, first);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
