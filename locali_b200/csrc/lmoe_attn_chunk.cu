@@ -10,8 +10,8 @@
 // One block per SM; the stream of (tile, head, key block) is cut evenly over
 // the launch as in lmoe_attn.cu.  Warp roles:
 //   0-3, 4-7   softmax and output of sub-tile 0 and 1
-//   8-11       keys and values into shared memory: 16-bit rows by cp.async,
-//              codes through registers (one tile ahead), dequantised to the
+//   8, 9       keys into shared memory, 10, 11 values: 16-bit rows by cp.async,
+//              codes through registers (32 rows ahead), dequantised to the
 //              16-bit type on the way, into the 128-byte-swizzled operand layout
 //   12, 13     one thread each issues the MMAs of sub-tile 0, 1
 //   14         walks the launch block's tiles and lays what the others need to
@@ -43,6 +43,9 @@ constexpr int kCkThreads = 16 * 32;  // 15 warps work; 128 registers a thread
 constexpr int kCkLoadWarp = 8, kCkMmaWarp = 12, kCkWalkWarp = 14;
 constexpr int kSegs = 8;  // tiles in the ring: the loader is at most 3 ahead of the output
 constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
+// Output staging of a warp: 32 rows of 64 bytes, 80 apart (no bank conflicts).  A lane holds a whole row, and rows
+// stored straight from lanes touch 32 lines an instruction (an epilogue took 10k cycles).
+constexpr int kStgRow = 80, kStgWarp = 32 * kStgRow;
 constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
 
 template <int BITS, int D, int GS>
@@ -51,7 +54,8 @@ struct ChunkGeo {
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
     static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
     static constexpr int SCALES = BITS == 16 ? 0 : 4 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
-    static constexpr int SMEM = 1024 + 6 * TILE + SCALES + 1024;
+    static constexpr int OFF_STG = OFF_X + SCALES;                   // output staging of the softmax warps
+    static constexpr int SMEM = 1024 + OFF_STG + 8 * kStgWarp;
 };
 
 // A tile, and the blocks of it that are this launch block's.
@@ -178,16 +182,37 @@ __device__ __forceinline__ float max3_nan(float x, float y, float z) {
     return r;
 }
 
-// Largest visible score of the thread's row, S at `ts`; two of the four reads
-// of 32 columns are in flight at a time.  FULL: all are visible, else mask(c)
-// has the bits of columns 32 c .. 32 c + 31.
-template <bool FULL, class F>
+// tcgen05.ld and st of one column
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r)
+                 : "r"(taddr)
+                 : "memory");
+    return __uint_as_float(r);
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+                 "r"(__float_as_uint(v))
+                 : "memory");
+}
+
+// Largest visible score of the thread's row, S at `ts`; mask(c) has the bits
+// of columns 32 c .. 32 c + 31.  Not unrolled: it runs for a tile's first
+// block and for blocks seen in part, and unrolled code that runs so seldom is
+// fetched anew each time.
+template <class F>
 __device__ __forceinline__ float row_max(uint32_t ts, F &&mask, bool &seen) {
     float x0 = -INFINITY, x1 = -INFINITY;
-    auto take = [&](uint32_t (&v)[32], int c) {
-        if constexpr (!FULL) {
-            const uint32_t mk = mask(c);
-            seen |= mk != 0;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t mk = mask(c);
+        if (!__any_sync(0xffffffffu, mk != 0)) continue;
+        seen |= mk != 0;
+        uint32_t v[32];
+        tmem_ld32(ts + 32 * c, v);
+        tmem_wait_ld32(v);
+        if (!__all_sync(0xffffffffu, mk == 0xFFFFFFFFu)) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
                 if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
@@ -197,44 +222,60 @@ __device__ __forceinline__ float row_max(uint32_t ts, F &&mask, bool &seen) {
             x0 = max3_nan(x0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
             x1 = max3_nan(x1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
         }
-    };
-    uint32_t v[32], y[32];
-    tmem_ld32(ts, v);
-    tmem_wait_ld32(v);
-    tmem_ld32(ts + 32, y);
-    take(v, 0);
-    tmem_wait_ld32(y);
-    tmem_ld32(ts + 64, v);
-    take(y, 1);
-    tmem_wait_ld32(v);
-    tmem_ld32(ts + 96, y);
-    take(v, 2);
-    tmem_wait_ld32(y);
-    take(y, 3);
-    if (FULL) seen = true;
+    }
     return max_nan(x0, x1);
 }
 
-// Terms over S with the running maximum m as it is, in one read of S; nothing
-// is written (again = true) when a score of a row of the warp passes its
-// maximum by more than 2^8 or is no number.
-template <typename TA, bool FULL, class F>
-__device__ __forceinline__ float row_try(uint32_t ts, F &&mask, float sc, float m, float &x, bool &seen, bool &again) {
+// Terms exp2(S sc - mu) over S, as 16-bit pairs for the tensor core (32
+// columns of S become 16, behind the reads); returns their sum in fp32.
+template <typename TA, class F>
+__device__ __forceinline__ float row_terms(uint32_t ts, F &&mask, float sc, float mu) {
+    const uint64_t sc2 = pack_f2(sc, sc), mu2 = pack_f2(-mu, -mu);
+    uint64_t sum = 0;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t mk = mask(c);
+        uint32_t pk[16];
+        if (!__any_sync(0xffffffffu, mk != 0)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+        } else {
+            uint32_t v[32];
+            tmem_ld32(ts + 32 * c, v);
+            tmem_wait_ld32(v);
+            if (!__all_sync(0xffffffffu, mk == 0xFFFFFFFFu)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (!(mk >> e & 1u)) v[e] = 0xFF800000u;  // sc > 0: its term is 0
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                float p0, p1;
+                unpack_f2(fma_f2(pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, mu2), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                sum = add_f2(sum, pack_f2(p0, p1));
+                pk[e / 2] = Act<TA>::pack2(p0, p1);
+            }
+        }
+        tmem_st16(ts + 16 * c, pk);
+    }
+    float s0, s1;
+    unpack_f2(sum, s0, s1);
+    return s0 + s1;
+}
+
+// Terms over an S seen in full with the running maximum m as it is, in one
+// read; nothing is written (again = true) when a score of a row of the warp
+// passes its maximum by more than 2^8 or is no number.
+template <typename TA>
+__device__ __forceinline__ float row_try(uint32_t ts, float sc, float m, bool &again) {
     const float mu = m == -INFINITY ? 0.0f : m;
     const uint64_t sc2 = pack_f2(sc, sc), mu2 = pack_f2(-mu, -mu);
     uint64_t sum = 0;
     float x0 = -INFINITY, x1 = -INFINITY;
     uint32_t pk[64];
-    bool any = FULL;
     auto take = [&](uint32_t (&v)[16], int c) {  // columns 16 c ..
-        uint32_t mk = 0;
-        if constexpr (!FULL) {
-            mk = mask(c >> 1) >> (16 * (c & 1)) & 0xFFFFu;
-            any |= mk != 0;
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (!(mk >> e & 1u)) v[e] = 0xFF800000u;
-        }
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             x0 = max3_nan(x0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
@@ -262,11 +303,9 @@ __device__ __forceinline__ float row_try(uint32_t ts, F &&mask, float sc, float 
         take(y, c + 1);
         if (c < 6) tmem_wait_ld(v);
     }
-    x = max_nan(x0, x1) * sc;
-    const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
-    again = __any_sync(0xffffffffu, move);
+    const float x = max_nan(x0, x1) * sc;
+    again = __any_sync(0xffffffffu, !(x <= m + 8.0f) && !(x == -INFINITY));
     if (!again) {
-        seen |= any;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t z[32];
@@ -410,8 +449,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             const int tok = in ? row / a.group : 0;
             const uint16_t *src = a.q + (int64_t)(ti.row0 + tok) * a.q_tok_stride +
                                   (int64_t)(ti.h * a.group + (in ? row - tok * a.group : 0)) * a.q_head_stride;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) cpa16(qs + op_off(r, c), in ? src + c * 8 : a.q, in ? 16 : 0);
+            // CH lanes a row, 32 / CH rows at a time
+            const uint32_t ins = __ballot_sync(0xffffffffu, in);
+            const int cc = lane % CH;
+#pragma unroll 4
+            for (int x = lane / CH; x < 32; x += 32 / CH) {
+                const uint16_t *p = reinterpret_cast<const uint16_t *>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), x));
+                const bool ok = ins >> x & 1u;
+                cpa16(qs + op_off(q4 * 32 + x, cc), ok ? p + cc * 8 : a.q, ok ? 16 : 0);
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         int u = 0, act = 0, active_segs = 0;
@@ -474,6 +521,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     const bool full = !bad && block_full(a, k0, smin, smax);
                     if (!block_full(a, k0, tmin, tmax)) ++parts;
                     auto mask = [&](int c) -> uint32_t {
+                        if (full) return 0xFFFFFFFFu;
                         const int kb = k0 + 32 * c;
                         uint32_t x = range_bits(see_lo, see_hi, kb) | range_bits(0, see_sink, kb);
                         if (bad >> (2 * c) & 1u) x &= 0xFFFF0000u;
@@ -483,31 +531,31 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     // with the maximum as it is, unless a score of the block passes it
                     const uint32_t ts = tm_s(t) + lanes;
                     bool again = true;
-                    if (i > b0) {
-                        float x;
-                        const float sum = full ? row_try<TA, true>(ts, mask, sc, m, x, seen, again)
-                                               : row_try<TA, false>(ts, mask, sc, m, x, seen, again);
+                    if (full && i > b0) {
+                        seen = true;
+                        const float sum = row_try<TA>(ts, sc, m, again);
                         if (!again) l += sum;
                     }
                     if (again) {
-                        const float x = (full ? row_max<true>(ts, mask, seen) : row_max<false>(ts, mask, seen)) * sc;
+                        const float x = row_max(ts, mask, seen) * sc;
                         const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
-                        const float f = move ? ex2(m - x) : 1.0f;
-                        if (move) m = x;
-                        l *= f;
-                        if (i > b0) {  // the sums so far
+                        if (__any_sync(0xffffffffu, move)) {
+                            const float f = move ? ex2(m - x) : 1.0f;
+                            if (move) m = x;
+                            l *= f;
+                            if (i > b0) {  // the sums so far
 #pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t v[32];
-                                tmem_ld32(tm_o(t) + lanes + 32 * c, v);
-                                tmem_wait_ld32(v);
+                                for (int c = 0; c < D / 32; ++c) {
+                                    uint32_t v[32];
+                                    tmem_ld32(tm_o(t) + lanes + 32 * c, v);
+                                    tmem_wait_ld32(v);
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                                tmem_st32(tm_o(t) + lanes + 32 * c, v);
+                                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                                    tmem_st32(tm_o(t) + lanes + 32 * c, v);
+                                }
                             }
                         }
-                        const float mu = m == -INFINITY ? 0.0f : m;
-                        l += full ? row_terms<TA, true>(ts, mask, sc, mu) : row_terms<TA, false>(ts, mask, sc, mu);
+                        l += row_terms<TA>(ts, mask, sc, m == -INFINITY ? 0.0f : m);
                     }
                     tmem_wait_st();
                     tc_fence_before();
@@ -526,67 +574,86 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 if (m == -INFINITY && seen) l = __uint_as_float(0x7FC00000u);
                 const bool whole = b0 == 0 && b1 == ti.nblk;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int tok = in ? row / a.group : 0;
-                uint16_t *out = a.out + ((int64_t)(ti.row0 + tok) * a.q_heads + ti.h * a.group + row - tok * a.group) * D;
-                float *part = part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) +
-                              (t * kCkSub + r) * D;
                 bool poisoned = false;
                 for (int pi = 0; pi < parts; ++pi)
                     poisoned |= (s_poison[n & 3][pi][0] | s_poison[n & 3][pi][1] | s_poison[n & 3][pi][2] | s_poison[n & 3][pi][3]) != 0;
+                if (poisoned) {
+                    // values that are no numbers, taken out of blocks that
+                    // only some rows see: added for those that do
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(tm_o(t) + lanes + 32 * c, v);
-                    tmem_wait_ld32(v);
-                    if (poisoned) {
-                        // values that are no numbers, taken out of blocks that
-                        // only some rows see: added for those that do
-                        for (int pi = 0; pi < parts; ++pi)
-                            for (int k = 0; k < kCkKeys; ++k) {
-                                if (!(s_poison[n & 3][pi][k >> 5] >> (k & 31) & 1u)) continue;
-                                const int j = s_pblk[n & 3][pi] * kCkKeys + k;
-                                if (!(j < see_hi && (j >= see_lo || j < see_sink))) continue;
-                                const int32_t pg = a.r.page(a.c, ti.b, j);
-                                if (pg < 0) continue;
-                                const int64_t kr = a.c.row(pg, ti.h, j % a.c.page_size);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    const int d = 32 * c + e;
-                                    float y;
-                                    if constexpr (Q) {
-                                        const uint32_t by = a.c.kv[1][kr * RB + d * BITS / 8];
-                                        const uint32_t code = BITS == 8 ? by : by >> (4 * (d & 1)) & 15u;
-                                        y = fmaf(Act<TA>::to_f(a.c.scale[1][kr * NG + d / GS]), (float)code,
-                                                 Act<TA>::to_f(a.c.bias[1][kr * NG + d / GS]));
-                                    } else {
-                                        y = Act<TA>::to_f(reinterpret_cast<const uint16_t *>(a.c.kv[1])[kr * D + d]);
-                                    }
-                                    if (!(fabsf(y) <= 3.402823466e38f))
-                                        v[e] = __float_as_uint(__uint_as_float(v[e]) + y);
-                                }
+                    for (int x = 0; x < parts * kCkKeys; ++x) {
+                        const int pi = x / kCkKeys, k = x % kCkKeys;
+                        if (!(s_poison[n & 3][pi][k >> 5] >> (k & 31) & 1u)) continue;
+                        const int j = s_pblk[n & 3][pi] * kCkKeys + k;
+                        const bool sees = j < see_hi && (j >= see_lo || j < see_sink);
+                        const int32_t pg = a.r.page(a.c, ti.b, j);
+                        if (pg < 0) continue;
+                        const int64_t kr = a.c.row(pg, ti.h, j % a.c.page_size);
+#pragma unroll 1
+                        for (int d = 0; d < D; ++d) {
+                            float y;
+                            if constexpr (Q) {
+                                const uint32_t by = a.c.kv[1][kr * RB + d * BITS / 8];
+                                const uint32_t code = BITS == 8 ? by : by >> (4 * (d & 1)) & 15u;
+                                y = fmaf(Act<TA>::to_f(a.c.scale[1][kr * NG + d / GS]), (float)code,
+                                         Act<TA>::to_f(a.c.bias[1][kr * NG + d / GS]));
+                            } else {
+                                y = Act<TA>::to_f(reinterpret_cast<const uint16_t *>(a.c.kv[1])[kr * D + d]);
                             }
-                    }
-                    if (whole) {
-                        if (in) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint4 o;
-                                uint32_t *ov = &o.x;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    ov[k] = Act<TA>::pack2(__uint_as_float(v[e + 2 * k]) * inv,
-                                                           __uint_as_float(v[e + 2 * k + 1]) * inv);
-                                *reinterpret_cast<uint4 *>(out + 32 * c + e) = o;
-                            }
+                            if (fabsf(y) <= 3.402823466e38f) continue;  // the same for all lanes
+                            const float o = tmem_ld1(tm_o(t) + lanes + d);
+                            tmem_st1(tm_o(t) + lanes + d, sees ? o + y : o);
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4 *>(part + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
                 }
+                // rows go out through the staging, 4 lanes a row of 64 bytes
+                const uint32_t stg = sb + G::OFF_STG + warp * kStgWarp;
+                const int tok = in ? row / a.group : 0;
+                uint8_t *mine = whole ? reinterpret_cast<uint8_t *>(
+                                            a.out + ((int64_t)(ti.row0 + tok) * a.q_heads + ti.h * a.group + row - tok * a.group) * D)
+                                      : reinterpret_cast<uint8_t *>(
+                                            part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) +
+                                            (t * kCkSub + r) * D);
+                uint8_t *dst[4];
+                const uint32_t ins = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    dst[x] = reinterpret_cast<uint8_t *>(__shfl_sync(
+                                 0xffffffffu, reinterpret_cast<unsigned long long>(mine), 8 * x + (lane >> 2))) +
+                             (lane & 3) * 16;
+                const int cols = whole ? 32 : 16;  // columns of 64 bytes
+#pragma unroll 1
+                for (int c = 0; c < D; c += cols) {
+                    uint4 o[4];
+                    uint32_t *ov = &o[0].x;
+                    if (whole) {
+                        uint32_t v[32];
+                        tmem_ld32(tm_o(t) + lanes + c, v);
+                        tmem_wait_ld32(v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            ov[e] = Act<TA>::pack2(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv);
+                    } else {
+                        uint32_t v[16];
+                        tmem_ld16(tm_o(t) + lanes + c, v);
+                        tmem_wait_ld(v);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) ov[e] = v[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sts128v(stg + lane * kStgRow + e * 16, o[e].x, o[e].y, o[e].z, o[e].w);
+                    __syncwarp();
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint4 v = lds128(stg + (8 * x + (lane >> 2)) * kStgRow + (lane & 3) * 16);
+                        if (ins >> (8 * x + (lane >> 2)) & 1u) *reinterpret_cast<uint4 *>(dst[x]) = v;
+                        dst[x] += 64;
+                    }
+                    __syncwarp();
+                }
                 if (!whole) {
-                    float2 *ml = reinterpret_cast<float2 *>(part - (t * kCkSub + r) * D + kCkRows * D);
+                    float2 *ml = reinterpret_cast<float2 *>(
+                        part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) + kCkRows * D);
                     ml[t * kCkSub + r] = make_float2(m, l);
                 }
                 if (t == 0 && r == 0 && sg.parts) {
@@ -604,19 +671,22 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         }
     } else if (warp < kCkMmaWarp) {
         // ---------------------------------------------------- keys and values
-        const int lw = warp - kCkLoadWarp;  // rows 32 lw .. of a block
-        constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of a warp's 32
+        const int which = (warp - kCkLoadWarp) >> 1, lw = (warp - kCkLoadWarp) & 1;  // rows 64 lw .. of a block
+        uint64_t *fullb = which ? vfull : kfull, *emptyb = which ? vempty : kempty;
+        const uint8_t *const kv = a.c.kv[which];
+        const uint32_t base = sb + (which ? G::OFF_V : G::OFF_K);
+        constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of 32 rows
         const int rr = lane / LPR, cc = lane % LPR;
         const int64_t lane_off = (int64_t)rr * RB + cc * BITS;  // the lane's part of a round's rows
         // the walk: block i of tile n, in blocks [.., b1)
         int i = 0, b1 = 0, n_seg = -1, parts = 0, more = 1;
         bool have = true;
-        // A block of the walk: head row of 16-position run 0, 1 of the warp's
-        // (-2: none, -1: no page), its facts.  Lanes 0 and 1 look the pages
-        // up; a block's page ids are asked for while the one before it is
-        // worked on (ask), and looked at when they have come (take).
+        // A block of the walk: lane x < 4 has the head row where 16-position
+        // run x of the warp's 64 begins (-2: none, -1: no page).  A block's
+        // page ids are asked for while the one before it is worked on (ask),
+        // and looked at when they have come (take).
         struct Unit {
-            long long r0, r1;
+            long long run;
             int k0, hi, seg, part;  // part: its number among the blocks seen in part, -1: seen in full
         };
         Unit ahead{};
@@ -645,10 +715,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             ahead.hi = ti.hi;
             ahead.seg = n_seg;
             ahead.part = block_full(a, ahead.k0, ti.minpos, ti.maxpos) ? -1 : parts++;
-            const int p = ahead.k0 + lw * 32 + lane * 16;
+            const int p = ahead.k0 + lw * 64 + lane * 16;
             a_slot = -1;
             a_head = ti.h;
-            if (lane < 2 && p < ti.hi) {
+            if (lane < 4 && p < ti.hi) {
                 const int e = p / a.c.page_size;
                 a_slot = p - e * a.c.page_size;
                 a_page = e < a.r.table_width ? a.r.table[(int64_t)ti.b * a.r.table_stride + e] : -1;
@@ -657,202 +727,202 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         };
         auto take = [&]() -> Unit {
             Unit x = ahead;
-            long long r = -2;
+            x.run = -2;
             if (a_slot >= 0) {
                 const bool in = a_page >= 0 && a_page < a.c.n_pages;
                 if (!in) set_error(a.r.err, kErrIndex);
-                r = in ? a.c.row(a_page, a_head, a_slot) : -1;
+                x.run = in ? a.c.row(a_page, a_head, a_slot) : -1;
             }
-            x.r0 = __shfl_sync(0xffffffffu, r, 0);
-            x.r1 = __shfl_sync(0xffffffffu, r, 1);
             return x;
         };
-        // head row of the warp's row x, -1 where there is nothing to read
-        auto row_of = [&](const Unit &n, int x) -> long long {
+        // head rows of the two runs of half h (32 rows) of the warp's
+        struct Half {
+            long long r0, r1;
+            int left;  // rows in front of the end
+        };
+        auto half = [&](const Unit &n, int h) -> Half {
+            return Half{__shfl_sync(0xffffffffu, n.run, 2 * h), __shfl_sync(0xffffffffu, n.run, 2 * h + 1),
+                        n.hi - n.k0 - lw * 64 - h * 32};
+        };
+        // head row of row x of a half, -1 where there is nothing to read
+        auto row_of = [&](const Half &n, int x) -> long long {
             const long long r = x < 16 ? n.r0 : n.r1;
-            return r >= 0 && n.k0 + lw * 32 + x < n.hi ? r + (x & 15) : -1;
+            return r >= 0 && x < n.left ? r + (x & 15) : -1;
         };
-        // all of the warp's 32 rows are there
-        auto whole = [&](const Unit &n) { return n.r0 >= 0 && n.r1 >= 0 && n.k0 + lw * 32 + 32 <= n.hi; };
-        auto dst_of = [&](auto which, int u) {
-            return sb + (decltype(which)::value ? G::OFF_V : G::OFF_K) + (u & 1) * G::TILE;
-        };
-        auto empty = [&](auto which, int u) -> bool {
-            uint64_t *b = decltype(which)::value ? vempty : kempty;
-            return __all_sync(0xffffffffu, wait(&b[u & 1], (u >> 1 & 1) ^ 1));
-        };
-        // the tile is in place; taken: rows of the warp's with values taken out
-        auto done = [&](auto which, const Unit &n, int u, uint32_t taken) {
-            constexpr bool V = decltype(which)::value;
+        auto whole = [&](const Half &n) { return n.r0 >= 0 && n.r1 >= 0 && n.left >= 32; };
+        auto empty = [&](int u) -> bool { return __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1)); };
+        // half h is in place; taken: its rows with values taken out
+        auto done = [&](const Unit &n, int u, int h, uint32_t taken) {
+            const uint32_t bad = __ballot_sync(0xffffffffu, n.run == -1);
             if (lane == 0) {
-                if (!V) s_bad[u & 3][lw] = (n.r0 == -1) | (n.r1 == -1) << 1;
+                if (!which) s_bad[u & 3][2 * lw + h] = bad >> (2 * h) & 3u;
                 else if (n.part >= 0) {
-                    s_poison[n.seg & 3][n.part][lw] = taken;
+                    s_poison[n.seg & 3][n.part][2 * lw + h] = taken;
                     if (lw == 0) s_pblk[n.seg & 3][n.part] = n.k0 / kCkKeys;
                 }
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(V ? &vfull[u & 1] : &kfull[u & 1]);
+            if (lane == 0) mbar_arrive(&fullb[u & 1]);
         };
-        using Keys = std::integral_constant<bool, false>;
-        using Values = std::integral_constant<bool, true>;
         if constexpr (Q) {
             constexpr int WPC = BITS == 8 ? 2 : 1;  // code words of a chunk
-            uint32_t code[IT][WPC];
-            uint32_t sbp[NG];  // (scale, bias) of row `lane`
-            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + lw * 32 * NG;
-            // round x of a tile: rows x RPI + rr; `run`: the lane's part of the rows of round 0 (or 16 / RPI)
-            auto fetch = [&](const uint8_t *run, bool in, int x) {
-                const uint8_t *src = run + (x * RPI % 16) * RB;
-                if constexpr (BITS == 8) {
-                    const uint2 v = in ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
-                    code[x][0] = v.x;
-                    code[x][1] = v.y;
-                } else {
-                    code[x][0] = in ? *reinterpret_cast<const uint32_t *>(src) : 0u;
-                }
+            // Codes and (scale, bias) pairs of a half.  Two of them: all loads
+            // of the next half are issued before this one is worked on.  (Loads
+            // issued between its rounds share the few scoreboards with the
+            // loads it waits for, which made every round wait a full latency.)
+            struct Raw {
+                uint32_t code[IT][WPC];
+                uint32_t sbp[NG];
             };
-            auto fetch_part = [&](auto which, const Unit &n, int x) {
-                const long long r = x * RPI < 16 ? n.r0 : n.r1;
-                fetch(a.c.kv[decltype(which)::value] + lane_off + r * RB, row_of(n, x * RPI + rr) >= 0, x);
-            };
-            auto fetch_scales = [&](auto which, const Unit &n) {
-                constexpr int W = decltype(which)::value;
+            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + (warp - kCkLoadWarp) * 32 * NG;
+            auto fetch = [&](Raw &w, const Half &n) {
                 const long long r = row_of(n, lane);
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
-                    sbp[g] = r >= 0 ? (uint32_t)a.c.scale[W][r * NG + g] | (uint32_t)a.c.bias[W][r * NG + g] << 16 : 0u;
+                    w.sbp[g] = r >= 0 ? (uint32_t)a.c.scale[which][r * NG + g] | (uint32_t)a.c.bias[which][r * NG + g] << 16 : 0u;
+                const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
+                const bool all = whole(n);
+#pragma unroll
+                for (int x = 0; x < IT; ++x) {
+                    const uint8_t *src = (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB;
+                    const bool in = all || row_of(n, x * RPI + rr) >= 0;
+                    if constexpr (BITS == 8) {
+                        const uint2 v = in ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
+                        w.code[x][0] = v.x;
+                        w.code[x][1] = v.y;
+                    } else {
+                        w.code[x][0] = in ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+                    }
+                }
             };
-            // writes tile u (codes and scales are in registers) and fetches the next one behind it
-            auto tile = [&](auto which, const Unit &n, int u, auto nwhich, const Unit &nx, bool next) -> bool {
-                constexpr bool V = decltype(which)::value;
-                constexpr int NW = decltype(nwhich)::value;
-                if (!empty(which, u)) return false;
+            // half h of block u into its place, four rounds at a time so that their reads and arithmetic overlap
+            auto put = [&](Raw &w, const Unit &n, int u, int h) {
                 bool no = false;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     // in a block that only some rows see, values that are no numbers are taken out
-                    if (V && n.part >= 0 && nonfinite2<TA>(sbp[g])) {
+                    if (which && n.part >= 0 && nonfinite2<TA>(w.sbp[g])) {
                         no = true;
-                        sbp[g] = 0;
+                        w.sbp[g] = 0;
                     }
-                    const uint32_t s = Pair<TA>::template scale<BITS>(sbp[g]) & 0xFFFFu;
-                    spair[lane * NG + g] = s | (sbp[g] & 0xFFFF0000u);
+                    const uint32_t s = Pair<TA>::template scale<BITS>(w.sbp[g]) & 0xFFFFu;
+                    spair[lane * NG + g] = s | (w.sbp[g] & 0xFFFF0000u);
                 }
                 const uint32_t taken = __ballot_sync(0xffffffffu, no);
                 __syncwarp();
-                if (next) fetch_scales(nwhich, nx);
-                const uint32_t dst = dst_of(which, u);
+                const uint32_t dst = base + (u & 1) * G::TILE;
                 const uint32_t *sp = spair + rr * NG + cc * 8 / GS;
-                auto put = [&](int x) {
-                    const uint32_t sbv = sp[x * RPI * NG];
-                    const uint4 v = dequant8<TA, BITS>(code[x][0], code[x][WPC - 1], __byte_perm(sbv, 0u, 0x1010),
-                                                       __byte_perm(sbv, 0u, 0x3232));
-                    sts128v(dst + op_off(lw * 32 + x * RPI + rr, cc), v.x, v.y, v.z, v.w);
-                };
-                // each round's registers are filled for the next tile as they come free
-                if (next && whole(nx)) {
-                    const uint8_t *p0 = a.c.kv[NW] + lane_off + nx.r0 * RB, *p1 = a.c.kv[NW] + lane_off + nx.r1 * RB;
 #pragma unroll
-                    for (int x = 0; x < IT; ++x) {
-                        put(x);
-                        fetch(x * RPI < 16 ? p0 : p1, true, x);
-                    }
-                } else {
+                for (int x0 = 0; x0 < IT; x0 += 4) {
+                    uint32_t sv[4];
+                    uint4 v[4];
 #pragma unroll
-                    for (int x = 0; x < IT; ++x) {
-                        put(x);
-                        if (next) fetch_part(nwhich, nx, x);
-                    }
+                    for (int x = 0; x < 4; ++x) sv[x] = sp[(x0 + x) * RPI * NG];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        v[x] = dequant8<TA, BITS>(w.code[x0 + x][0], w.code[x0 + x][WPC - 1],
+                                                  __byte_perm(sv[x], 0u, 0x1010), __byte_perm(sv[x], 0u, 0x3232));
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        sts128v(dst + op_off(lw * 64 + h * 32 + (x0 + x) * RPI + rr, cc), v[x].x, v[x].y, v[x].z, v[x].w);
                 }
-                done(which, n, u, taken);
-                return true;
+                done(n, u, h, taken);
             };
+            Raw w0, w1;
             ask();
             Unit n = take();
-            fetch_scales(Keys{}, n);
-#pragma unroll
-            for (int x = 0; x < IT; ++x) fetch_part(Keys{}, n, x);
+            fetch(w0, half(n, 0));
             ask();
             for (int u = 0; !s_abort; ++u) {
-                if (!tile(Keys{}, n, u, Values{}, n, true)) break;
+                fetch(w1, half(n, 1));
+                if (!empty(u)) break;
+                put(w0, n, u, 0);
                 const bool next = asked;
                 const Unit nx = next ? take() : n;
+                if (next) fetch(w0, half(nx, 0));
                 ask();
-                if (!tile(Values{}, n, u, Keys{}, nx, next) || !next) break;
+                put(w1, n, u, 1);
+                if (!next) break;
                 n = nx;
             }
         } else {
-            auto copy = [&](auto which, const Unit &n, int u) {
-                const uint8_t *kv = a.c.kv[decltype(which)::value];
-                const uint32_t dst = dst_of(which, u);
-                if (whole(n)) {
-                    const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
+            auto copy = [&](const Unit &n, int u) {
+                const uint32_t dst = base + (u & 1) * G::TILE;
 #pragma unroll
-                    for (int x = 0; x < IT; ++x)
-                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
-                } else {
+                for (int h = 0; h < 2; ++h) {
+                    const Half hf = half(n, h);
+                    if (whole(hf)) {
+                        const uint8_t *p0 = kv + lane_off + hf.r0 * RB, *p1 = kv + lane_off + hf.r1 * RB;
+#pragma unroll
+                        for (int x = 0; x < IT; ++x)
+                            cpa16(dst + op_off(lw * 64 + h * 32 + x * RPI + rr, cc),
+                                  (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
+                    } else {
 #pragma unroll 1
-                    for (int x = 0; x < IT; ++x) {
-                        const long long r = row_of(n, x * RPI + rr);
-                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv, r >= 0 ? 16 : 0);
+                        for (int x = 0; x < IT; ++x) {
+                            const long long r = row_of(hf, x * RPI + rr);
+                            cpa16(dst + op_off(lw * 64 + h * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv,
+                                  r >= 0 ? 16 : 0);
+                        }
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            // the copies of a tile have landed
-            auto finish = [&](auto which, const Unit &n, int u) {
-                uint32_t taken = 0;
-                if (decltype(which)::value && n.part >= 0) {
+            // the copies of a block have landed
+            auto finish = [&](const Unit &n, int u) {
+                uint32_t taken[2] = {0, 0};
+                if (which && n.part >= 0) {
                     __syncwarp();
 #pragma unroll 1
-                    for (int x = 0; x < IT; ++x) {
+                    for (int x = 0; x < 2 * IT; ++x) {
                         const int row = x * RPI + rr;
-                        const uint32_t at = dst_of(which, u) + op_off(lw * 32 + row, cc);
+                        const uint32_t at = base + (u & 1) * G::TILE + op_off(lw * 64 + row, cc);
                         uint4 v = lds128(at);
-                        uint32_t *vv = &v.x;
-                        bool no = false;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (nonfinite2<TA>(vv[k])) {
-                                no = true;
-                                if ((vv[k] & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) vv[k] &= 0xFFFF0000u;
-                                if ((vv[k] >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) vv[k] &= 0xFFFFu;
-                            }
-                        if (no) sts128v(at, v.x, v.y, v.z, v.w);
+                        const bool no = nonfinite2<TA>(v.x) || nonfinite2<TA>(v.y) || nonfinite2<TA>(v.z) || nonfinite2<TA>(v.w);
                         const uint32_t bl = __ballot_sync(0xffffffffu, no);
+                        if (bl == 0) continue;
+                        if (no) {
+                            auto out = [](uint32_t y) {
+                                if ((y & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) y &= 0xFFFF0000u;
+                                if ((y >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) y &= 0xFFFFu;
+                                return y;
+                            };
+                            sts128v(at, out(v.x), out(v.y), out(v.z), out(v.w));
+                        }
 #pragma unroll
                         for (int y = 0; y < RPI; ++y)
-                            if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken |= 1u << (x * RPI + y);
+                            if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken[x >= IT] |= 1u << ((x * RPI + y) & 31);
                     }
                 }
-                done(which, n, u, taken);
+                done(n, u, 0, taken[0]);
+                done(n, u, 1, taken[1]);
             };
-            // one tile is in flight while the one before it is completed
+            // one block is in flight while the one before it is completed,
+            // unless its place is still taken: then that one first
             Unit prev{};
+            bool pending = false;
             int u = 0;
-            bool ok = true;
             ask();
             for (; asked && !s_abort; ++u) {
                 const Unit n = take();
                 ask();
-                ok = empty(Keys{}, u);
-                if (!ok) break;
-                copy(Keys{}, n, u);
-                if (u > 0) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    finish(Values{}, prev, u - 1);
+                if (pending && !__all_sync(0xffffffffu, mbar_test(&emptyb[u & 1], (u >> 1 & 1) ^ 1))) {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    finish(prev, u - 1);
+                    pending = false;
                 }
-                ok = empty(Values{}, u);
-                if (!ok) break;
-                copy(Values{}, n, u);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-                finish(Keys{}, n, u);
+                if (!empty(u)) break;
+                copy(n, u);
+                if (pending) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    finish(prev, u - 1);
+                }
                 prev = n;
+                pending = true;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (ok && u > 0) finish(Values{}, prev, u - 1);
+            if (pending && !asked) finish(prev, u - 1);
         }
     }
     if (warp >= kCkMmaWarp && warp < kCkMmaWarp + 2 && lane == 0) {

@@ -98,19 +98,6 @@ __device__ __forceinline__ uint32_t idesc_f16(int n, bool f16) {
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPfM >> 4) << 24);
 }
 
-// Non-blocking test of an mbarrier phase (try_wait may suspend the thread for
-// hundreds of cycles when the phase is not complete yet).
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; "
-        "selp.u32 %0, 1, 0, p; }"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
 // 2-D tiled TMA load (no multicast): box at (x, y) of `map` -> shared memory,
 // completion counted in bytes on `bar`
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {

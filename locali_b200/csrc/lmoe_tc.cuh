@@ -87,6 +87,19 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
            ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
+// Non-blocking test of an mbarrier phase (try_wait may suspend the thread for
+// hundreds of cycles when the phase is not complete yet).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // Pipeline wait of the warp roles: mbarrier.try_wait suspends the thread
 // in hardware until the phase completes (or a short time limit passes), so a
 // plain loop keeps hand-off latency low; bounded like mbar_wait.
