@@ -10,12 +10,15 @@
 // One block per SM; the stream of (tile, head, key block) is cut evenly over
 // the launch as in lmoe_attn.cu.  Warp roles:
 //   0-3, 4-7   softmax and output of sub-tile 0 and 1
-//   8, 9       keys into shared memory, 10, 11 values: 16-bit rows by cp.async,
-//              codes through registers (32 rows ahead), dequantised to the
-//              16-bit type on the way, into the 128-byte-swizzled operand layout
-//   12, 13     one thread each issues the MMAs of sub-tile 0, 1
-//   14         walks the launch block's tiles and lays what the others need to
+//   8-11       keys into shared memory, 12-15 values: 16-bit rows by cp.async,
+//              codes through registers, dequantised to the 16-bit type on the
+//              way, into the 128-byte-swizzled operand layout
+//   16, 17     one thread each issues the MMAs of sub-tile 0, 1
+//   18         walks the launch block's tiles and lays what the others need to
 //              know of them into a ring in shared memory
+//   19         looks up the pages of the next key blocks for the loaders
+// Register budgets differ (setmaxnreg): a softmax thread holds the 64 packed
+// terms of its row.
 // The sub-tiles issue their MMAs (P V of a block, then S of the next) in turn,
 // which keeps them half a block apart: one's softmax overlaps the other's
 // MMAs.  Issued as they came, the MMAs of both interleaved and ended together,
@@ -39,9 +42,13 @@ namespace lmoe {
 namespace {
 
 constexpr int kCkRows = 256, kCkKeys = 128, kCkSub = 128;
-constexpr int kCkThreads = 16 * 32;  // 15 warps work; 128 registers a thread
-constexpr int kCkLoadWarp = 8, kCkMmaWarp = 12, kCkWalkWarp = 14;
-constexpr int kSegs = 8;  // tiles in the ring: the loader is at most 3 ahead of the output
+constexpr int kCkThreads = 20 * 32;
+constexpr int kCkLoadWarp = 8, kCkMmaWarp = 16, kCkWalkWarp = 18, kCkLookWarp = 19;
+// Registers a thread after the split: 256 x 136 + 256 x 80 + 128 x 48 = 61440, the 640 x 96 of the launch.
+constexpr int kRegSoftmax = 136, kRegLoad = 80, kRegRest = 48;
+static_assert(256 * kRegSoftmax + 256 * kRegLoad + 128 * kRegRest <= kCkThreads * 96, "registers");
+constexpr int kLook = 4;  // key blocks looked up ahead
+constexpr int kSegs = 16;  // tiles in the ring: the look-up is at most 7 blocks ahead of the output
 constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
 // Output staging of a warp: 32 rows of 64 bytes, 80 apart (no bank conflicts).  A lane holds a whole row, and rows
 // stored straight from lanes touch 32 lines an instruction (an epilogue took 10k cycles).
@@ -53,7 +60,7 @@ struct ChunkGeo {
     static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
     static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
-    static constexpr int SCALES = BITS == 16 ? 0 : 4 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
+    static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
     static constexpr int OFF_STG = OFF_X + SCALES;                   // output staging of the softmax warps
     static constexpr int SMEM = 1024 + OFF_STG + 8 * kStgWarp;
 };
@@ -64,6 +71,15 @@ struct Seg {
     int b0, b1;
     int more;   // another one follows
     int parts;  // launch blocks that share the tile, if it begins here and goes on behind; else 0
+};
+
+// A key block as the loaders need it: the head row where each 16-position run
+// begins (-2: none, -1: no page).
+struct Look {
+    long long run[kCkKeys / 16];
+    int left;  // positions in front of the end
+    int blk, seg;
+    int part;  // its number among the tile's blocks seen in part; -1: seen in full, -2: no block, the walk is over
 };
 
 // every row of the tile sees every position of the block at k0
@@ -371,10 +387,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     constexpr bool F16 = std::is_same<TA, __half>::value;
     extern __shared__ __align__(1024) uint8_t raw[];
     __shared__ long long s_plan[kCkThreads / 32 + 6];
-    __shared__ __align__(16) uint32_t s_bad[4][4];  // block u & 3: the key warps' runs without a page
-    __shared__ uint32_t s_poison[4][kPoison][4];    // tile & 3, its n-th block seen in part: rows taken out
+    __shared__ uint32_t s_bad[8];  // block u & 7: its runs without a page
+    __shared__ uint32_t s_poison[4][kPoison][4];  // tile & 3, its n-th block seen in part: rows taken out
     __shared__ int s_pblk[4][kPoison];
-    __shared__ uint64_t bars[18 + 2 * kSegs];
+    __shared__ Look s_look[kLook];
+    __shared__ uint64_t bars[18 + 2 * kSegs + 2 * kLook];
     __shared__ Seg s_seg[kSegs];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     const uint32_t sb = smem_u32(smem);
     uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *sfull = bars + 8,
              *pfull = bars + 10, *qfull = bars + 12, *ofull = bars + 14, *turn = bars + 16,
-             *gfull = bars + 18, *gempty = gfull + kSegs;
+             *gfull = bars + 18, *gempty = gfull + kSegs, *lfull = gempty + kSegs, *lempty = lfull + kLook;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -398,7 +415,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         }
         for (int i = 0; i < kSegs; ++i) {
             mbar_init(&gfull[i], 1);
-            mbar_init(&gempty[i], kCkWalkWarp);
+            mbar_init(&gempty[i], 11);  // 8 softmax warps, 2 MMA warps, the look-up
+        }
+        for (int i = 0; i < kLook; ++i) {
+            mbar_init(&lfull[i], 1);
+            mbar_init(&lempty[i], 8);
         }
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -437,6 +458,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     auto seg_done = [&](int n) { mbar_arrive(&gempty[n % kSegs]); };
 
     if (warp < kCkLoadWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoftmax));
         // ---------------------------------------------------- softmax and output
         const int t = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;  // row of the sub-tile
         const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
@@ -516,8 +538,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         if (!ok) break;
                         load_q(seg(n + 1).t);
                     }
-                    const uint4 bw = *reinterpret_cast<const uint4 *>(s_bad[u & 3]);
-                    const uint32_t bad = bw.x | bw.y << 2 | bw.z << 4 | bw.w << 6;
+                    const uint32_t bad = s_bad[u & 7];
                     const bool full = !bad && block_full(a, k0, smin, smax);
                     if (!block_full(a, k0, tmin, tmax)) ++parts;
                     auto mask = [&](int c) -> uint32_t {
@@ -670,96 +691,41 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             if (!more) break;
         }
     } else if (warp < kCkMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegLoad));
         // ---------------------------------------------------- keys and values
-        const int which = (warp - kCkLoadWarp) >> 1, lw = (warp - kCkLoadWarp) & 1;  // rows 64 lw .. of a block
+        const int which = (warp - kCkLoadWarp) >> 2, lw = warp & 3;  // rows 32 lw .. of a block
         uint64_t *fullb = which ? vfull : kfull, *emptyb = which ? vempty : kempty;
         const uint8_t *const kv = a.c.kv[which];
         const uint32_t base = sb + (which ? G::OFF_V : G::OFF_K);
-        constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of 32 rows
+        constexpr int LPR = CH, RPI = 32 / LPR, IT = 32 / RPI;  // lanes of a row; rows and rounds of a warp's 32
         const int rr = lane / LPR, cc = lane % LPR;
         const int64_t lane_off = (int64_t)rr * RB + cc * BITS;  // the lane's part of a round's rows
-        // the walk: block i of tile n, in blocks [.., b1)
-        int i = 0, b1 = 0, n_seg = -1, parts = 0, more = 1;
-        bool have = true;
-        // A block of the walk: lane x < 4 has the head row where 16-position
-        // run x of the warp's 64 begins (-2: none, -1: no page).  A block's
-        // page ids are asked for while the one before it is worked on (ask),
-        // and looked at when they have come (take).
+        // the warp's share of a block
         struct Unit {
-            long long run;
-            int k0, hi, seg, part;  // part: its number among the blocks seen in part, -1: seen in full
+            long long r0, r1;  // head rows of its two runs
+            int left, blk, seg, part;
         };
-        Unit ahead{};
-        int32_t a_page = 0;
-        int a_slot = 0, a_head = 0;  // a_slot < 0: the lane has no run
-        bool asked = false;
-        auto ask = [&]() {
-            if (i == b1) {
-                if (n_seg >= 0) {
-                    __syncwarp();
-                    if (lane == 0) seg_done(n_seg);
-                }
-                have = more && __all_sync(0xffffffffu, seg_ready(n_seg + 1));
-                if (have) {
-                    const Seg &sg = seg(++n_seg);
-                    i = sg.b0;
-                    b1 = sg.b1;
-                    more = sg.more;
-                    parts = 0;
-                }
-            }
-            asked = have;
-            if (!have) return;
-            const Tile &ti = seg(n_seg).t;
-            ahead.k0 = ti.block(i) * kCkKeys;
-            ahead.hi = ti.hi;
-            ahead.seg = n_seg;
-            ahead.part = block_full(a, ahead.k0, ti.minpos, ti.maxpos) ? -1 : parts++;
-            const int p = ahead.k0 + lw * 64 + lane * 16;
-            a_slot = -1;
-            a_head = ti.h;
-            if (lane < 4 && p < ti.hi) {
-                const int e = p / a.c.page_size;
-                a_slot = p - e * a.c.page_size;
-                a_page = e < a.r.table_width ? a.r.table[(int64_t)ti.b * a.r.table_stride + e] : -1;
-            }
-            ++i;
+        auto look = [&](int u) -> Unit {
+            Unit n{-2, -2, 0, 0, 0, -2};
+            if (!__all_sync(0xffffffffu, wait(&lfull[u % kLook], u / kLook & 1))) return n;
+            const Look &e = s_look[u % kLook];
+            n = Unit{e.run[2 * lw], e.run[2 * lw + 1], e.left - 32 * lw, e.blk, e.seg, e.part};
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&lempty[u % kLook]);
+            return n;
         };
-        auto take = [&]() -> Unit {
-            Unit x = ahead;
-            x.run = -2;
-            if (a_slot >= 0) {
-                const bool in = a_page >= 0 && a_page < a.c.n_pages;
-                if (!in) set_error(a.r.err, kErrIndex);
-                x.run = in ? a.c.row(a_page, a_head, a_slot) : -1;
-            }
-            return x;
-        };
-        // head rows of the two runs of half h (32 rows) of the warp's
-        struct Half {
-            long long r0, r1;
-            int left;  // rows in front of the end
-        };
-        auto half = [&](const Unit &n, int h) -> Half {
-            return Half{__shfl_sync(0xffffffffu, n.run, 2 * h), __shfl_sync(0xffffffffu, n.run, 2 * h + 1),
-                        n.hi - n.k0 - lw * 64 - h * 32};
-        };
-        // head row of row x of a half, -1 where there is nothing to read
-        auto row_of = [&](const Half &n, int x) -> long long {
+        // head row of the warp's row x, -1 where there is nothing to read
+        auto row_of = [&](const Unit &n, int x) -> long long {
             const long long r = x < 16 ? n.r0 : n.r1;
             return r >= 0 && x < n.left ? r + (x & 15) : -1;
         };
-        auto whole = [&](const Half &n) { return n.r0 >= 0 && n.r1 >= 0 && n.left >= 32; };
+        auto whole = [&](const Unit &n) { return n.r0 >= 0 && n.r1 >= 0 && n.left >= 32; };
         auto empty = [&](int u) -> bool { return __all_sync(0xffffffffu, wait(&emptyb[u & 1], (u >> 1 & 1) ^ 1)); };
-        // half h is in place; taken: its rows with values taken out
-        auto done = [&](const Unit &n, int u, int h, uint32_t taken) {
-            const uint32_t bad = __ballot_sync(0xffffffffu, n.run == -1);
-            if (lane == 0) {
-                if (!which) s_bad[u & 3][2 * lw + h] = bad >> (2 * h) & 3u;
-                else if (n.part >= 0) {
-                    s_poison[n.seg & 3][n.part][2 * lw + h] = taken;
-                    if (lw == 0) s_pblk[n.seg & 3][n.part] = n.k0 / kCkKeys;
-                }
+        // the share is in place; taken: its rows with values taken out
+        auto done = [&](const Unit &n, int u, uint32_t taken) {
+            if (which && n.part >= 0 && lane == 0) {
+                s_poison[n.seg & 3][n.part][lw] = taken;
+                if (lw == 0) s_pblk[n.seg & 3][n.part] = n.blk;
             }
             fence_proxy_async();
             __syncwarp();
@@ -767,117 +733,114 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         };
         if constexpr (Q) {
             constexpr int WPC = BITS == 8 ? 2 : 1;  // code words of a chunk
-            // Codes and (scale, bias) pairs of a half.  Two of them: all loads
-            // of the next half are issued before this one is worked on.  (Loads
-            // issued between its rounds share the few scoreboards with the
-            // loads it waits for, which made every round wait a full latency.)
-            struct Raw {
-                uint32_t code[IT][WPC];
-                uint32_t sbp[NG];
-            };
-            uint32_t *spair = reinterpret_cast<uint32_t *>(smem + G::OFF_X) + (warp - kCkLoadWarp) * 32 * NG;
-            auto fetch = [&](Raw &w, const Half &n) {
+            uint32_t code[IT][WPC];
+            uint32_t sc[(NG + 1) / 2], bi[(NG + 1) / 2];  // of row `lane`, two groups a word
+            bool in_lane = false;                        // row `lane` is there
+            // (scale, scale), (bias, bias) of the rows' groups
+            uint2 *spair = reinterpret_cast<uint2 *>(smem + G::OFF_X) + (warp - kCkLoadWarp) * 32 * NG;
+            // all loads of a share, issued as soon as the one before it is in place
+            auto fetch = [&](const Unit &n) {
                 const long long r = row_of(n, lane);
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-                    w.sbp[g] = r >= 0 ? (uint32_t)a.c.scale[which][r * NG + g] | (uint32_t)a.c.bias[which][r * NG + g] << 16 : 0u;
+                const uint16_t *ps = a.c.scale[which] + (r < 0 ? 0 : r * NG), *pb = a.c.bias[which] + (r < 0 ? 0 : r * NG);
+                if constexpr (NG == 1) {
+                    sc[0] = *ps;
+                    bi[0] = *pb;
+                } else if constexpr (NG == 2) {
+                    sc[0] = *reinterpret_cast<const uint32_t *>(ps);
+                    bi[0] = *reinterpret_cast<const uint32_t *>(pb);
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(ps), y = *reinterpret_cast<const uint2 *>(pb);
+                    sc[0] = x.x;
+                    sc[(NG - 1) / 2] = x.y;
+                    bi[0] = y.x;
+                    bi[(NG - 1) / 2] = y.y;
+                }
+                in_lane = r >= 0;
                 const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
-                const bool all = whole(n);
-#pragma unroll
-                for (int x = 0; x < IT; ++x) {
+                auto get = [&](int x, bool in) {
                     const uint8_t *src = (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB;
-                    const bool in = all || row_of(n, x * RPI + rr) >= 0;
                     if constexpr (BITS == 8) {
                         const uint2 v = in ? *reinterpret_cast<const uint2 *>(src) : make_uint2(0u, 0u);
-                        w.code[x][0] = v.x;
-                        w.code[x][1] = v.y;
+                        code[x][0] = v.x;
+                        code[x][1] = v.y;
                     } else {
-                        w.code[x][0] = in ? *reinterpret_cast<const uint32_t *>(src) : 0u;
+                        code[x][0] = in ? *reinterpret_cast<const uint32_t *>(src) : 0u;
                     }
+                };
+                if (whole(n)) {
+#pragma unroll
+                    for (int x = 0; x < IT; ++x) get(x, true);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < IT; ++x) get(x, row_of(n, x * RPI + rr) >= 0);
                 }
             };
-            // half h of block u into its place, four rounds at a time so that their reads and arithmetic overlap
-            auto put = [&](Raw &w, const Unit &n, int u, int h) {
+            // the share into its place, four rounds at a time so that their reads and arithmetic overlap
+            auto put = [&](const Unit &n, int u) {
                 bool no = false;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
+                    uint32_t x = in_lane ? __byte_perm(sc[g / 2], bi[g / 2], g & 1 ? 0x7632 : 0x5410) : 0u;
                     // in a block that only some rows see, values that are no numbers are taken out
-                    if (which && n.part >= 0 && nonfinite2<TA>(w.sbp[g])) {
+                    if (which && n.part >= 0 && nonfinite2<TA>(x)) {
                         no = true;
-                        w.sbp[g] = 0;
+                        x = 0;
                     }
-                    const uint32_t s = Pair<TA>::template scale<BITS>(w.sbp[g]) & 0xFFFFu;
-                    spair[lane * NG + g] = s | (w.sbp[g] & 0xFFFF0000u);
+                    spair[lane * NG + g] = make_uint2(Pair<TA>::template scale<BITS>(__byte_perm(x, 0u, 0x1010)),
+                                                      __byte_perm(x, 0u, 0x3232));
                 }
                 const uint32_t taken = __ballot_sync(0xffffffffu, no);
                 __syncwarp();
                 const uint32_t dst = base + (u & 1) * G::TILE;
-                const uint32_t *sp = spair + rr * NG + cc * 8 / GS;
+                const uint2 *sp = spair + rr * NG + cc * 8 / GS;
 #pragma unroll
                 for (int x0 = 0; x0 < IT; x0 += 4) {
-                    uint32_t sv[4];
+                    uint2 sv[4];
                     uint4 v[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) sv[x] = sp[(x0 + x) * RPI * NG];
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        v[x] = dequant8<TA, BITS>(w.code[x0 + x][0], w.code[x0 + x][WPC - 1],
-                                                  __byte_perm(sv[x], 0u, 0x1010), __byte_perm(sv[x], 0u, 0x3232));
+                        v[x] = dequant8<TA, BITS>(code[x0 + x][0], code[x0 + x][WPC - 1], sv[x].x, sv[x].y);
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        sts128v(dst + op_off(lw * 64 + h * 32 + (x0 + x) * RPI + rr, cc), v[x].x, v[x].y, v[x].z, v[x].w);
+                        sts128v(dst + op_off(lw * 32 + (x0 + x) * RPI + rr, cc), v[x].x, v[x].y, v[x].z, v[x].w);
                 }
-                done(n, u, h, taken);
+                done(n, u, taken);
             };
-            Raw w0, w1;
-            ask();
-            Unit n = take();
-            fetch(w0, half(n, 0));
-            ask();
-            for (int u = 0; !s_abort; ++u) {
-                fetch(w1, half(n, 1));
+            Unit n = look(0);
+            if (n.part > -2) fetch(n);
+            for (int u = 0; n.part > -2 && !s_abort; ++u) {
                 if (!empty(u)) break;
-                put(w0, n, u, 0);
-                const bool next = asked;
-                const Unit nx = next ? take() : n;
-                if (next) fetch(w0, half(nx, 0));
-                ask();
-                put(w1, n, u, 1);
-                if (!next) break;
-                n = nx;
+                put(n, u);
+                n = look(u + 1);
+                if (n.part > -2) fetch(n);
             }
         } else {
             auto copy = [&](const Unit &n, int u) {
                 const uint32_t dst = base + (u & 1) * G::TILE;
+                if (whole(n)) {
+                    const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const Half hf = half(n, h);
-                    if (whole(hf)) {
-                        const uint8_t *p0 = kv + lane_off + hf.r0 * RB, *p1 = kv + lane_off + hf.r1 * RB;
-#pragma unroll
-                        for (int x = 0; x < IT; ++x)
-                            cpa16(dst + op_off(lw * 64 + h * 32 + x * RPI + rr, cc),
-                                  (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
-                    } else {
+                    for (int x = 0; x < IT; ++x)
+                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
+                } else {
 #pragma unroll 1
-                        for (int x = 0; x < IT; ++x) {
-                            const long long r = row_of(hf, x * RPI + rr);
-                            cpa16(dst + op_off(lw * 64 + h * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv,
-                                  r >= 0 ? 16 : 0);
-                        }
+                    for (int x = 0; x < IT; ++x) {
+                        const long long r = row_of(n, x * RPI + rr);
+                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv, r >= 0 ? 16 : 0);
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            // the copies of a block have landed
+            // the copies of a share have landed
             auto finish = [&](const Unit &n, int u) {
-                uint32_t taken[2] = {0, 0};
+                uint32_t taken = 0;
                 if (which && n.part >= 0) {
                     __syncwarp();
 #pragma unroll 1
-                    for (int x = 0; x < 2 * IT; ++x) {
-                        const int row = x * RPI + rr;
-                        const uint32_t at = base + (u & 1) * G::TILE + op_off(lw * 64 + row, cc);
+                    for (int x = 0; x < IT; ++x) {
+                        const uint32_t at = base + (u & 1) * G::TILE + op_off(lw * 32 + x * RPI + rr, cc);
                         uint4 v = lds128(at);
                         const bool no = nonfinite2<TA>(v.x) || nonfinite2<TA>(v.y) || nonfinite2<TA>(v.z) || nonfinite2<TA>(v.w);
                         const uint32_t bl = __ballot_sync(0xffffffffu, no);
@@ -892,27 +855,26 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         }
 #pragma unroll
                         for (int y = 0; y < RPI; ++y)
-                            if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken[x >= IT] |= 1u << ((x * RPI + y) & 31);
+                            if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken |= 1u << (x * RPI + y);
                     }
                 }
-                done(n, u, 0, taken[0]);
-                done(n, u, 1, taken[1]);
+                done(n, u, taken);
             };
-            // one block is in flight while the one before it is completed,
-            // unless its place is still taken: then that one first
+            // One share is in flight while the one before it is completed,
+            // unless its place is still taken: then that one first.
             Unit prev{};
-            bool pending = false;
+            bool pending = false, ok = true;
             int u = 0;
-            ask();
-            for (; asked && !s_abort; ++u) {
-                const Unit n = take();
-                ask();
+            for (; !s_abort; ++u) {
+                const Unit n = look(u);
+                if (n.part == -2) break;
                 if (pending && !__all_sync(0xffffffffu, mbar_test(&emptyb[u & 1], (u >> 1 & 1) ^ 1))) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     finish(prev, u - 1);
                     pending = false;
                 }
-                if (!empty(u)) break;
+                ok = empty(u);
+                if (!ok) break;
                 copy(n, u);
                 if (pending) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -922,8 +884,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 pending = true;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (pending && !asked) finish(prev, u - 1);
+            if (pending && ok) finish(prev, u - 1);
         }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegRest));
     }
     if (warp >= kCkMmaWarp && warp < kCkMmaWarp + 2 && lane == 0) {
         // ---------------------------------------------------- MMAs of sub-tile t
@@ -991,6 +955,73 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
             if (left <= 0) break;
             next_tile<kCkRows, kCkKeys>(a, first);
         }
+    } else if (warp == kCkLookWarp) {
+        // ---------------------------------------------------- the pages of the key blocks
+        // lane x < 8: run x of the block; the page ids of a block are asked
+        // for before those of the one in front of it are looked at
+        int u = 0;
+        Look e;  // the block asked for (run: not used)
+        int32_t page = -1;
+        int slot = -1, head = 0;
+        e.part = -2;
+        auto give = [&]() -> bool {
+            if (u >= kLook && !__all_sync(0xffffffffu, wait(&lempty[u % kLook], (u / kLook - 1) & 1))) return false;
+            long long run = -2;
+            if (slot >= 0) {
+                const bool in = page >= 0 && page < a.c.n_pages;
+                if (!in) set_error(a.r.err, kErrIndex);
+                run = in ? a.c.row(page, head, slot) : -1;
+            }
+            const uint32_t bad = __ballot_sync(0xffffffffu, run == -1);
+            Look &x = s_look[u % kLook];
+            if (lane < kCkKeys / 16) x.run[lane] = run;
+            if (lane == 0) {
+                x.left = e.left;
+                x.blk = e.blk;
+                x.seg = e.seg;
+                x.part = e.part;
+                s_bad[u & 7] = bad;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&lfull[u % kLook]);
+            ++u;
+            return true;
+        };
+        bool asked = false, ok = true;
+        for (int n = 0, more = 1; more && ok && !s_abort; ++n) {
+            ok = __all_sync(0xffffffffu, seg_ready(n));
+            if (!ok) break;
+            const Seg &sg = seg(n);
+            const Tile ti = sg.t;
+            const int b0 = sg.b0, b1 = sg.b1;
+            more = sg.more;
+            __syncwarp();
+            if (lane == 0) seg_done(n);
+            int parts = 0;
+            for (int i = b0; i < b1 && ok; ++i) {
+                const int blk = ti.block(i), p = blk * kCkKeys + lane * 16;
+                int32_t pg = -1;
+                int sl = -1;
+                if (lane < kCkKeys / 16 && p < ti.hi) {
+                    const int en = p / a.c.page_size;
+                    sl = p - en * a.c.page_size;
+                    if (en < a.r.table_width) pg = a.r.table[(int64_t)ti.b * a.r.table_stride + en];
+                }
+                if (asked) ok = give();
+                asked = true;
+                page = pg;
+                slot = sl;
+                head = ti.h;
+                e.left = ti.hi - blk * kCkKeys;
+                e.blk = blk;
+                e.seg = n;
+                e.part = block_full(a, blk * kCkKeys, ti.minpos, ti.maxpos) ? -1 : parts++;
+            }
+        }
+        if (ok && asked) ok = give();
+        e.part = -2;
+        slot = -1;
+        if (ok) give();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
