@@ -28,6 +28,7 @@ namespace {
 constexpr int kRowWarps = 4;
 constexpr int kRowThreads = kRowWarps * 32;
 constexpr int kRowBlocksPerSm = 4;  // at most
+constexpr int kRowTile = 2;         // what a tile costs besides its key blocks, in key blocks
 
 template <int BITS, int D, int GS, int NT>
 struct RowsGeo {
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
     constexpr int R = G::R, KS = G::KS, KT = G::KT, MT = G::MT, QS = G::QS, NG = G::NG, RB = G::RB;
     constexpr bool Q = BITS != 16;
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ long long s_plan[kRowWarps + 6];
+    __shared__ long long s_plan[kRowWarps + 4];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(sm) + warp * (G::NU * G::UB);
     float *s_o = reinterpret_cast<float *>(sm);
@@ -125,18 +126,16 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
     pdl_trigger();
     if (blockIdx.x == 0) a.r.validate(tid, kRowThreads);
     Share sh;
-    Cursor cur;
+    Cursor<R, KS, kRowTile> cur;
     // a run of at least one key block for each warp
-    const bool work = find_share<R, KS, kRowThreads>(a, kRowWarps, s_plan, sh, cur);
+    const bool work = find_share<R, KS, kRowTile, kRowThreads, false>(a, kRowTile + kRowWarps, s_plan, sh, cur);
     if (tid == 0) rec->parts = 0;
     if (!work) return;
-    long long left = sh.begin(blockIdx.x + 1) - sh.begin(blockIdx.x);
     const float sc = a.scale_log2;
 
-    while (left > 0) {
+    for (;;) {
         const Tile &t = cur.t;
-        const int b0 = cur.blk, b1 = (int)min((long long)t.nblk, b0 + left);
-        left -= b1 - b0;
+        const int b0 = cur.b0, b1 = cur.b1;
 
         // ---- the tile's rows as the column operand of S^T, in the order of K's words
         uint32_t qf[NT][QS][2];
@@ -145,7 +144,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
         for (int n = 0; n < NT; ++n) {
             const int row = t.rt * R + n * 8 + g;  // in the sequence's rows
             const bool in = row < t.n * a.group;
-            const int tok = row / a.group;
+            const int tok = a.per_group(row);
             const uint16_t *q = a.q + (int64_t)(t.row0 + tok) * a.q_tok_stride +
                                 (int64_t)(t.h * a.group + row - tok * a.group) * a.q_head_stride;
 #pragma unroll
@@ -179,7 +178,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int rc = t.rt * R + n * 8 + 2 * t4 + c;
-                pos[n][c] = rc < t.n * a.group ? t.first + rc / a.group : -1;
+                pos[n][c] = rc < t.n * a.group ? t.first + a.per_group(rc) : -1;
             }
         }
         float o[NT][MT][4], m[NT][2], l[NT][2];
@@ -583,7 +582,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                     part[R * D + row * 2 + 1] = ll;
                 }
             } else if (row < t.rows) {
-                const int rr = t.rt * R + row, tok = rr / a.group;
+                const int rr = t.rt * R + row, tok = a.per_group(rr);
                 const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
                 uint2 v;
                 v.x = Act<TA>::pack2(acc.x * inv, acc.y * inv);
@@ -592,16 +591,15 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                                                     tok * a.group) * D + d) = v;
             }
         }
-        if (tid == 0 && b0 == 0 && b1 < t.nblk) {
+        const int shared = cur.shared(sh, blockIdx.x);
+        if (tid == 0 && shared) {
             rec->out0 = t.row0;
             rec->row = t.rt * R;
             rec->rows_h = t.rows | t.h << 16;
-            rec->parts = sh.owner(cur.tile_begin + t.nblk - 1) - blockIdx.x + 1;
+            rec->parts = shared;
         }
-        if (left > 0) {
-            __syncthreads();
-            next_tile<R, KS>(a, cur);
-        }
+        __syncthreads();
+        if (!cur.next(a)) break;
     }
 }
 
@@ -670,7 +668,7 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const AttnArgs a, int g
             if (warp != 0) continue;
         }
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-        const int rr = rec.row + row, tok = rr / a.group;
+        const int rr = rec.row + row, tok = a.per_group(rr);
         uint16_t *out = a.out + ((int64_t)(rec.out0 + tok) * a.q_heads + h * a.group + rr - tok * a.group) * D;
 #pragma unroll
         for (int v = 0; v < V; ++v) out[v * 32 + lane] = Act<TA>::from_f(acc[v] * inv);

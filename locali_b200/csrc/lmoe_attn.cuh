@@ -30,8 +30,8 @@ template <int R, int KS>
 __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     const int r0 = t.rt * R;
     t.rows = min(R, t.n * a.group - r0);
-    t.minpos = t.first + r0 / a.group;
-    t.maxpos = t.first + (r0 + t.rows - 1) / a.group;
+    t.minpos = t.first + a.per_group(r0);
+    t.maxpos = t.first + a.per_group(r0 + t.rows - 1);
     t.hi = max(0, t.maxpos + 1);
     int low = 0;
     if (a.window > 0) low = (int)max(0ll, (long long)t.minpos - a.window + 1);
@@ -40,79 +40,123 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     t.nblk = max(1, t.nsink + (t.hi + KS - 1) / KS - t.lo);
 }
 
-// Blocks of all tiles of sequence b (one head), and its rows.
-template <int R, int KS>
-__device__ __forceinline__ int seq_blocks(const AttnArgs &a, int b, Tile &t) {
+// Sequence b's rows into t; returns its tiles (of one head).
+template <int R>
+__device__ __forceinline__ int seq_rows(const AttnArgs &a, int b, Tile &t) {
     t.b = b;
     t.row0 = a.r.start(b);
     t.n = max(0, a.r.start(b + 1) - t.row0);
     t.first = max(a.r.lens[b], 0) - t.n;
-    int sum = 0;
-    const int nt = (t.n * a.group + R - 1) / R;
-    for (t.rt = 0; t.rt < nt; ++t.rt) {
-        tile_range<R, KS>(a, t);
-        sum += t.nblk;
-    }
-    return sum;
+    return (t.n * a.group + R - 1) / R;
 }
 
-// The blocks of all (sequence, row tile, head), in that order, form one
-// stream; block c of the launch takes the c-th of `parts` equal runs of it.
-// So ragged batches stay level without the host knowing a length, and a tile
-// may be cut over several blocks of the launch; attn_merge_kernel joins those.
+// The work of a launch is a stream: for every (sequence, row tile, head), in
+// that order, X units for the tile itself (its rows, its result) and one for
+// each key block.  Block c of the launch takes the c-th of `parts` equal runs
+// of it.  So ragged batches stay level without the host knowing a length, and
+// a tile may be cut over several blocks of the launch; attn_merge_kernel joins
+// those.
 struct Share {
-    long long total;  // blocks of the stream
+    long long total;  // units of the stream
     int parts;        // launch blocks that take part
     __device__ __forceinline__ long long begin(int c) const { return total * c / parts; }
     __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * parts + total - 1) / total) - 1; }
 };
 
-// Position in the stream: the tile, and the block in it.
+// A run's place in the stream: the tile, where the stream has its first unit,
+// and the key blocks [b0, b1) of it that are the run's (none: b0 == b1).
+template <int R, int KS, int X>
 struct Cursor {
     Tile t;
-    int blk;
-    long long tile_begin;  // stream position of the tile's block 0
+    long long at, end;  // the tile's first unit, the run's end
+    int b0, b1;
+    __device__ __forceinline__ void open(long long from) {
+        b0 = (int)max(0ll, from - at - X);
+        b1 = (int)max((long long)b0, min((long long)t.nblk, end - at - X));
+    }
+    // launch blocks that share the tile, if it begins here and goes on behind the run; else 0
+    __device__ __forceinline__ int shared(const Share &sh, int c) const {
+        return b0 == 0 && b1 > 0 && b1 < t.nblk ? sh.owner(at + X + t.nblk - 1) - c + 1 : 0;
+    }
+    // The next tile with key blocks of the run's; false: there is none.
+    __device__ __forceinline__ bool next(const AttnArgs &a) {
+        for (;;) {
+            at += X + t.nblk;
+            if (at + X >= end) return false;
+            if (++t.h >= a.c.kv_heads) {
+                t.h = 0;
+                if (++t.rt * (long long)R >= (long long)t.n * a.group) {
+                    t.rt = 0;
+                    int b = t.b, nt;
+                    do nt = seq_rows<R>(a, ++b, t);
+                    while (nt == 0);
+                }
+                tile_range<R, KS>(a, t);
+            }
+            open(at);
+            if (b1 > b0) return true;
+        }
+    }
 };
 
-// Finds the launch block's run; every thread of the block calls it (NTHR
-// threads, smem of at least NTHR / 32 + 6 long longs).  False: no work.
-template <int R, int KS, int NTHR>
-__device__ __forceinline__ bool find_share(const AttnArgs &a, int minb, long long *sm, Share &sh, Cursor &cur) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int NW = NTHR / 32;
+// Units of sequence b for one head.  A thread walks its tiles, or (WARP) a
+// warp's lanes share them; all lanes then hold the sum.
+template <int R, int KS, int X, bool WARP>
+__device__ __forceinline__ long long seq_units(const AttnArgs &a, int b) {
     Tile t;
-    long long carry = 0;
-    long long mine = 0;  // this thread's sequence of the first round
-    const int rounds = (a.r.n_seqs + NTHR - 1) / NTHR;
-    // total; with at most NTHR sequences one round finds everything
-    for (int k = 0; k < rounds; ++k) {
-        const int b = k * NTHR + tid;
-        const long long w = b < a.r.n_seqs ? (long long)seq_blocks<R, KS>(a, b, t) * a.c.kv_heads : 0;
-        if (k == 0) mine = w;
-        carry += w;
+    const int nt = seq_rows<R>(a, b, t);
+    long long sum = 0;
+    for (t.rt = WARP ? (threadIdx.x & 31) : 0; t.rt < nt; t.rt += WARP ? 32 : 1) {
+        tile_range<R, KS>(a, t);
+        sum += t.nblk + X;
     }
-    long long sum = carry;
+    if (WARP) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    return sum;
+}
+
+// Finds the launch block's run; every thread of the block calls it (NTHR
+// threads, sm of NTHR / 32 + 4 long longs).  False: no work.  WARP: a warp for
+// each sequence (few sequences of many tiles), else a thread.  minu: units a
+// run has at least.
+template <int R, int KS, int X, int NTHR, bool WARP>
+__device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long long *sm, Share &sh, Cursor<R, KS, X> &cur) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NW = NTHR / 32, PER = WARP ? NW : NTHR;  // sequences of a round
+    const int rounds = (a.r.n_seqs + PER - 1) / PER;
+    auto units = [&](int k) -> long long {  // of this warp's or thread's sequence of round k
+        const int b = k * PER + (WARP ? warp : tid);
+        return b < a.r.n_seqs ? seq_units<R, KS, X, WARP>(a, b) * a.c.kv_heads : 0;
+    };
+    const long long mine = units(0);
+    long long sum = mine;
+    for (int k = 1; k < rounds; ++k) sum += units(k);
+    if (!WARP) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
     if (lane == 0) sm[warp] = sum;
     __syncthreads();
     sh.total = 0;
     for (int w = 0; w < NW; ++w) sh.total += sm[w];
     __syncthreads();
     if (sh.total == 0) return false;
-    sh.parts = (int)min((long long)gridDim.x, max(1ll, sh.total / minb));
+    sh.parts = (int)min((long long)gridDim.x, max(1ll, sh.total / minu));
     if ((int)blockIdx.x >= sh.parts) return false;
     const long long s = sh.begin(blockIdx.x);
-    // the sequence that holds stream position s
+    // the sequence that holds unit s
     long long base = 0;
     for (int k = 0; k < rounds; ++k) {
-        const int b = k * NTHR + tid;
-        const long long w = k == 0 ? mine : (b < a.r.n_seqs ? (long long)seq_blocks<R, KS>(a, b, t) * a.c.kv_heads : 0);
+        const long long w = k == 0 ? mine : units(k);
         long long inc = w;
+        if (!WARP) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
         }
         if (lane == 31) sm[warp] = inc;
         __syncthreads();
@@ -122,54 +166,52 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minb, long lon
             base += sm[q];
         }
         before += inc - w;
-        if (w > 0 && before <= s && s < before + w) {
-            sm[NW] = b;
+        if (w > 0 && before <= s && s < before + w && (!WARP || lane == 0)) {
+            sm[NW] = k * PER + (WARP ? warp : tid);
             sm[NW + 1] = before;
         }
         __syncthreads();
         if (s < base) break;
     }
-    // its tile and head
-    Tile &ct = cur.t;
-    const int b = (int)sm[NW];
-    long long off = s - sm[NW + 1];
-    ct.b = b;
-    ct.row0 = a.r.start(b);
-    ct.n = max(0, a.r.start(b + 1) - ct.row0);
-    ct.first = max(a.r.lens[b], 0) - ct.n;
-    for (ct.rt = 0;; ++ct.rt) {
-        tile_range<R, KS>(a, ct);
-        const long long w = (long long)ct.nblk * a.c.kv_heads;
-        if (off < w) break;
-        off -= w;
-    }
-    ct.h = (int)(off / ct.nblk);
-    cur.blk = (int)(off % ct.nblk);
-    cur.tile_begin = s - cur.blk;
-    __syncthreads();
-    return true;
-}
-
-// The tile after cur's (there is one).
-template <int R, int KS>
-__device__ __forceinline__ void next_tile(const AttnArgs &a, Cursor &cur) {
+    // its tile: the first warp's lanes look at 32 tiles at a time
     Tile &t = cur.t;
-    cur.tile_begin += t.nblk;
-    cur.blk = 0;
-    if (++t.h < a.c.kv_heads) return;
-    t.h = 0;
-    if (++t.rt * (long long)R < (long long)t.n * a.group) {
-        tile_range<R, KS>(a, t);
-        return;
+    const int nt = seq_rows<R>(a, (int)sm[NW], t);
+    if (warp == 0) {
+        long long off = s - sm[NW + 1];
+        for (int r0 = 0;; r0 += 32) {
+            t.rt = r0 + lane;
+            long long w = 0;
+            if (t.rt < nt) {
+                tile_range<R, KS>(a, t);
+                w = (long long)(t.nblk + X) * a.c.kv_heads;
+            }
+            long long inc = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, off < inc);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    sm[NW + 2] = t.rt;
+                    sm[NW + 3] = off - (inc - w);
+                }
+                break;
+            }
+            off -= __shfl_sync(0xffffffffu, inc, 31);
+        }
     }
-    t.rt = 0;
-    do {
-        ++t.b;
-        t.row0 = a.r.start(t.b);
-        t.n = max(0, a.r.start(t.b + 1) - t.row0);
-    } while (t.n == 0);
-    t.first = max(a.r.lens[t.b], 0) - t.n;
+    __syncthreads();
+    t.rt = (int)sm[NW + 2];
     tile_range<R, KS>(a, t);
+    const long long off = sm[NW + 3];
+    t.h = (int)(off / (t.nblk + X));
+    cur.at = s - off % (t.nblk + X);
+    cur.end = sh.begin(blockIdx.x + 1);
+    cur.open(s);
+    __syncthreads();
+    return cur.b1 > cur.b0 || cur.next(a);
 }
 
 // Scratch: one record for each launch block (the cut tile that begins in its

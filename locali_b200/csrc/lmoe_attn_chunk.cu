@@ -50,9 +50,12 @@ static_assert(256 * kRegSoftmax + 256 * kRegLoad + 128 * kRegRest <= kCkThreads 
 constexpr int kLook = 4;  // key blocks looked up ahead
 constexpr int kSegs = 16;  // tiles in the ring: the look-up is at most 7 blocks ahead of the output
 constexpr int kCkMinBlocks = 2;  // key blocks a launch block takes at least
+constexpr int kCkTile = 4;       // what a tile costs besides its key blocks, in key blocks: its first block's extra
+                                 // pass, its result and the hand-over are about 12k cycles, a block 3k
 // Output staging of a warp: 32 rows of 64 bytes, 80 apart (no bank conflicts).  A lane holds a whole row, and rows
 // stored straight from lanes touch 32 lines an instruction (an epilogue took 10k cycles).
 constexpr int kStgRow = 80, kStgWarp = 32 * kStgRow;
+constexpr int kExpFma = 2;  // of 8 pairs of exponentials, on the FMA pipe
 constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
 
 template <int BITS, int D, int GS>
@@ -136,6 +139,13 @@ __device__ __forceinline__ uint32_t attn_idesc(int n, bool f16, bool b_mn) {
            ((uint32_t)(128 >> 4) << 24);
 }
 
+// true in one lane of the converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(e));
+    return e != 0;
+}
+
 // bits of [lo, hi) in the 32 positions from kb
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int kb) {
     const int l = min(max(lo - kb, 0), 32), h = min(max(hi - kb, 0), 32);
@@ -190,6 +200,27 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+// 2^x of a pair on the FMA pipe, for x up to 120 or so: x = n + f with n the
+// nearest integer, 2^f by a polynomial on [-1/2, 1/2] (the minimax one of
+// degree 4 with value 1 at 0, relative error 2.9e-6 in fp32), n added to the
+// exponent.  Below -127 the result is 0.  An SM has 16 exponentials a cycle,
+// half of what the tensor cores would have of a row's scores at a head of 128.
+__device__ __forceinline__ void exp2_fma(float &x, float &y) {
+    const uint64_t magic = pack_f2(12582912.0f, 12582912.0f), unmagic = pack_f2(-12582912.0f, -12582912.0f);
+    const uint64_t v = pack_f2(fmaxf(x, -127.0f), fmaxf(y, -127.0f));
+    const uint64_t t = add_f2(v, magic);  // n in the low bits
+    const uint64_t f = fma_f2(add_f2(t, unmagic), pack_f2(-1.0f, -1.0f), v);
+    uint64_t p = pack_f2(0.009582852944731712f, 0.009582852944731712f);
+    p = fma_f2(p, f, pack_f2(0.055906426161527634f, 0.055906426161527634f));
+    p = fma_f2(p, f, pack_f2(0.24024099111557007f, 0.24024099111557007f));
+    p = fma_f2(p, f, pack_f2(0.6931241750717163f, 0.6931241750717163f));
+    p = fma_f2(p, f, pack_f2(1.0f, 1.0f));
+    float p0, p1, t0, t1;
+    unpack_f2(p, p0, p1);
+    unpack_f2(t, t0, t1);
+    x = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    y = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 // largest of three, keeping a NaN
 __device__ __forceinline__ float max3_nan(float x, float y, float z) {
@@ -301,8 +332,12 @@ __device__ __forceinline__ float row_try(uint32_t ts, float sc, float m, bool &a
         for (int e = 0; e < 16; e += 2) {
             float p0, p1;
             unpack_f2(fma_f2(pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, mu2), p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
+            if (e / 2 % 8 < kExpFma) {
+                exp2_fma(p0, p1);
+            } else {
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+            }
             sum = add_f2(sum, pack_f2(p0, p1));
             pk[8 * c + e / 2] = Act<TA>::pack2(p0, p1);
         }
@@ -386,7 +421,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     constexpr int NG = G::NG;
     constexpr bool F16 = std::is_same<TA, __half>::value;
     extern __shared__ __align__(1024) uint8_t raw[];
-    __shared__ long long s_plan[kCkThreads / 32 + 6];
+    __shared__ long long s_plan[kCkThreads / 32 + 4];
     __shared__ uint32_t s_bad[8];  // block u & 7: its runs without a page
     __shared__ uint32_t s_poison[4][kPoison][4];  // tile & 3, its n-th block seen in part: rows taken out
     __shared__ int s_pblk[4][kPoison];
@@ -430,9 +465,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     MergeRec *rec = reinterpret_cast<MergeRec *>(a.scratch) + blockIdx.x;
     if (threadIdx.x == 0) rec->parts = 0;
     Share sh;
-    Cursor first;
-    if (!find_share<kCkRows, kCkKeys, kCkThreads>(a, kCkMinBlocks, s_plan, sh, first)) return;
-    const long long run = sh.begin(blockIdx.x + 1) - sh.begin(blockIdx.x);
+    Cursor<kCkRows, kCkKeys, kCkTile> cur;
+    const bool work =
+        a.r.n_seqs <= 2 * (kCkThreads / 32)
+            ? find_share<kCkRows, kCkKeys, kCkTile, kCkThreads, true>(a, kCkTile + kCkMinBlocks, s_plan, sh, cur)
+            : find_share<kCkRows, kCkKeys, kCkTile, kCkThreads, false>(a, kCkTile + kCkMinBlocks, s_plan, sh, cur);
+    if (!work) return;
     if (warp == kCkMmaWarp) {
         tmem_alloc(&s_tmem, 512);
         tmem_relinquish();
@@ -468,7 +506,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
         auto load_q = [&](const Tile &ti) {
             const int row = ti.rt * kCkRows + t * kCkSub + r;
             const bool in = row < ti.n * a.group;
-            const int tok = in ? row / a.group : 0;
+            const int tok = in ? a.per_group(row) : 0;
             const uint16_t *src = a.q + (int64_t)(ti.row0 + tok) * a.q_tok_stride +
                                   (int64_t)(ti.h * a.group + (in ? row - tok * a.group : 0)) * a.q_head_stride;
             // CH lanes a row, 32 / CH rows at a time
@@ -511,15 +549,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 if (lane == 0) mbar_arrive(&qfull[t]);
                 const int row = ti.rt * kCkRows + t * kCkSub + r;
                 const bool in = row < ti.n * a.group;
-                const int p = in ? ti.first + row / a.group : -1;
+                const int p = in ? ti.first + a.per_group(row) : -1;
                 const int see_hi = p + 1, see_lo = a.window ? (int)max(0ll, (long long)p - a.window + 1) : 0;
                 const int see_sink = min(a.sinks, see_hi);
                 // positions of the sub-tile's first and last row
                 const int lastrow = min(ti.rows, (t + 1) * kCkSub) - 1;
                 const int nsink = ti.nsink, lo = ti.lo - nsink;
                 const int tmin = ti.minpos, tmax = ti.maxpos;
-                const int smin = ti.first + (ti.rt * kCkRows + t * kCkSub) / a.group;
-                const int smax = ti.first + (ti.rt * kCkRows + lastrow) / a.group;
+                const int smin = ti.first + a.per_group(ti.rt * kCkRows + t * kCkSub);
+                const int smax = ti.first + a.per_group(ti.rt * kCkRows + lastrow);
                 float m = -INFINITY;
                 float l = 0.0f;
                 bool seen = false;
@@ -532,11 +570,6 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     if (r == 0) {  // the MMAs before S_t's end are done: the keys, and the values before
                         mbar_arrive(&kempty[u & 1]);
                         if (i > b0) mbar_arrive(&vempty[(u - 1) & 1]);
-                    }
-                    if (i == b1 - 1 && more) {  // Q_t is free
-                        ok = __all_sync(0xffffffffu, seg_ready(n + 1));
-                        if (!ok) break;
-                        load_q(seg(n + 1).t);
                     }
                     const uint32_t bad = s_bad[u & 7];
                     const bool full = !bad && block_full(a, k0, smin, smax);
@@ -584,6 +617,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     if (lane == 0) mbar_arrive(&pfull[t]);
                 }
                 if (!ok) break;
+                if (more) {  // Q_t is free
+                    ok = __all_sync(0xffffffffu, seg_ready(n + 1));
+                    if (!ok) break;
+                    load_q(seg(n + 1).t);
+                }
                 // ---- the tile's result
                 ok = __all_sync(0xffffffffu, wait(&ofull[t], active_segs & 1));
                 ++active_segs;
@@ -629,19 +667,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 }
                 // rows go out through the staging, 4 lanes a row of 64 bytes
                 const uint32_t stg = sb + G::OFF_STG + warp * kStgWarp;
-                const int tok = in ? row / a.group : 0;
-                uint8_t *mine = whole ? reinterpret_cast<uint8_t *>(
-                                            a.out + ((int64_t)(ti.row0 + tok) * a.q_heads + ti.h * a.group + row - tok * a.group) * D)
-                                      : reinterpret_cast<uint8_t *>(
-                                            part_ptr(a, gridDim.x, part_floats<kCkRows, D>(), blockIdx.x, b0 == 0 ? 1 : 0) +
-                                            (t * kCkSub + r) * D);
+                const int tok = in ? a.per_group(row) : 0;
+                uint8_t *to = whole ? reinterpret_cast<uint8_t *>(a.out + ((int64_t)ti.row0 * a.q_heads + ti.h * a.group) * D)
+                                    : reinterpret_cast<uint8_t *>(part_ptr(a, gridDim.x, part_floats<kCkRows, D>(),
+                                                                           blockIdx.x, b0 == 0 ? 1 : 0));
+                // the row's offset: 32 bytes at a time, so that it fits 32 bits
+                const uint32_t mine = whole ? (uint32_t)(((int64_t)tok * (a.q_heads - a.group) + row) * (D * 2 / 32))
+                                            : (uint32_t)((t * kCkSub + r) * (D * 4 / 32));
                 uint8_t *dst[4];
                 const uint32_t ins = __ballot_sync(0xffffffffu, in);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    dst[x] = reinterpret_cast<uint8_t *>(__shfl_sync(
-                                 0xffffffffu, reinterpret_cast<unsigned long long>(mine), 8 * x + (lane >> 2))) +
-                             (lane & 3) * 16;
+                    dst[x] = to + (int64_t)__shfl_sync(0xffffffffu, mine, 8 * x + (lane >> 2)) * 32 + (lane & 3) * 16;
                 const int cols = whole ? 32 : 16;  // columns of 64 bytes
 #pragma unroll 1
                 for (int c = 0; c < D; c += cols) {
@@ -889,71 +926,87 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegRest));
     }
-    if (warp >= kCkMmaWarp && warp < kCkMmaWarp + 2 && lane == 0) {
+    if (warp >= kCkMmaWarp && warp < kCkMmaWarp + 2) {
         // ---------------------------------------------------- MMAs of sub-tile t
-        const int t = warp - kCkMmaWarp;
+        // The whole warp walks along and one elected lane issues: with the
+        // control flow uniform, the descriptors stay in uniform registers.
+        // (Issued from a lane's own branch, every MMA first moved its operands
+        // there, and the issue took longer than the MMAs.)
+        const int t = __shfl_sync(0xffffffffu, warp - kCkMmaWarp, 0);
         const uint32_t id_s = attn_idesc(kCkKeys, F16, false), id_o = attn_idesc(D, F16, true);
-        const uint64_t qd = sw128_desc(sb + G::OFF_Q + t * G::TILE);
+        const uint32_t sbu = __shfl_sync(0xffffffffu, sb, 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t ds = tm + (uint32_t)(t * 128), dd = tm + (uint32_t)(256 + t * D);
+        const uint64_t qd = sw128_desc(sbu + G::OFF_Q + t * G::TILE);
+        auto all = [&](bool x) -> bool { return __all_sync(0xffffffffu, x); };
         auto scores = [&](int u) {
-            const uint64_t kd = sw128_desc(sb + G::OFF_K + (u & 1) * G::TILE);
+            const uint64_t kd = sw128_desc(sbu + G::OFF_K + (u & 1) * G::TILE);
+            if (elect_one()) {
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s) {
-                const uint64_t o = (uint64_t)((s >> 2) * (16384 >> 4) + (s & 3) * 2);
-                umma_f16(tm_s(t), qd + o, kd + o, id_s, s ? 1u : 0u);
+                for (int s = 0; s < D / 16; ++s) {
+                    const uint64_t o = (uint64_t)((s >> 2) * (16384 >> 4) + (s & 3) * 2);
+                    umma_f16(ds, qd + o, kd + o, id_s, s ? 1u : 0u);
+                }
             }
+            __syncwarp();
+        };
+        auto commit = [&](uint64_t *bar) {
+            if (elect_one()) umma_commit(bar);
+            __syncwarp();
         };
         int u = 0, act = 0, active_segs = 0;
         bool ok = true;
         for (int n = 0; !s_abort; ++n) {
-            if (!seg_ready(n)) break;
-            const int nb = seg(n).b1 - seg(n).b0, rows = seg(n).t.rows, more = seg(n).more;
-            seg_done(n);
+            if (!all(seg_ready(n))) break;
+            const int nb = __shfl_sync(0xffffffffu, seg(n).b1 - seg(n).b0, 0);
+            const int rows = __shfl_sync(0xffffffffu, seg(n).t.rows, 0), more = __shfl_sync(0xffffffffu, seg(n).more, 0);
+            if (lane == 0) seg_done(n);
+            __syncwarp();
             if (t == 1 && rows <= kCkSub) {
                 for (int j = 0; j < nb && ok; ++j, ++u) {  // only pass the turn on
-                    ok = wait(&turn[1], u & 1);
-                    if (ok) mbar_arrive(&turn[0]);
+                    ok = all(wait(&turn[1], u & 1));
+                    if (ok && lane == 0) mbar_arrive(&turn[0]);
+                    __syncwarp();
                 }
             } else {
-                ok = wait(&qfull[t], active_segs & 1) && wait(&kfull[u & 1], u >> 1 & 1);
+                ok = all(wait(&qfull[t], active_segs & 1) && wait(&kfull[u & 1], u >> 1 & 1));
                 ++active_segs;
                 if (!ok) break;
                 tc_fence_after();
                 scores(u);
-                umma_commit(&sfull[t]);
+                commit(&sfull[t]);
                 for (int j = 0; j < nb; ++j, ++u, ++act) {
                     const bool last = j + 1 == nb;
-                    ok = wait(&vfull[u & 1], u >> 1 & 1) && (last || wait(&kfull[(u + 1) & 1], (u + 1) >> 1 & 1)) &&
-                         wait(&pfull[t], act & 1) && wait(&turn[t], t ? u & 1 : (u & 1) ^ 1);
+                    ok = all(wait(&vfull[u & 1], u >> 1 & 1) && (last || wait(&kfull[(u + 1) & 1], (u + 1) >> 1 & 1)) &&
+                             wait(&pfull[t], act & 1) && wait(&turn[t], t ? u & 1 : (u & 1) ^ 1));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t vd = mn128_desc(sb + G::OFF_V + (u & 1) * G::TILE);
+                    const uint64_t vd = mn128_desc(sbu + G::OFF_V + (u & 1) * G::TILE);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int s = 0; s < kCkKeys / 16; ++s)
-                        umma_f16_ts(tm_o(t), tm_s(t) + 8 * s, vd + (uint64_t)(s * (2048 >> 4)), id_o, j || s ? 1u : 0u);
+                        for (int s = 0; s < kCkKeys / 16; ++s)
+                            umma_f16_ts(dd, ds + 8 * s, vd + (uint64_t)(s * (2048 >> 4)), id_o, s ? 1u : (uint32_t)(j != 0));
+                    }
+                    __syncwarp();
                     if (!last) scores(u + 1);
-                    mbar_arrive(&turn[t ^ 1]);
-                    umma_commit(last ? &ofull[t] : &sfull[t]);
+                    if (lane == 0) mbar_arrive(&turn[t ^ 1]);
+                    commit(last ? &ofull[t] : &sfull[t]);
                 }
             }
             if (!ok || !more) break;
         }
     } else if (warp == kCkWalkWarp && lane == 0) {
         // ---------------------------------------------------- the walk
-        long long left = run;
-        for (int n = 0; !s_abort; ++n) {
+        bool more = true;
+        for (int n = 0; more && !s_abort; ++n) {
             if (n >= kSegs && !wait(&gempty[n % kSegs], (n / kSegs - 1) & 1)) break;
             Seg &sg = s_seg[n % kSegs];
-            sg.t = first.t;
-            sg.b0 = first.blk;
-            sg.b1 = (int)min((long long)first.t.nblk, first.blk + left);
-            left -= sg.b1 - sg.b0;
-            sg.more = left > 0;
-            sg.parts = sg.b0 == 0 && sg.b1 < first.t.nblk
-                           ? sh.owner(first.tile_begin + first.t.nblk - 1) - (int)blockIdx.x + 1
-                           : 0;
+            sg.t = cur.t;
+            sg.b0 = cur.b0;
+            sg.b1 = cur.b1;
+            sg.parts = cur.shared(sh, blockIdx.x);
+            more = cur.next(a);
+            sg.more = more;
             mbar_arrive(&gfull[n % kSegs]);
-            if (left <= 0) break;
-            next_tile<kCkRows, kCkKeys>(a, first);
         }
     } else if (warp == kCkLookWarp) {
         // ---------------------------------------------------- the pages of the key blocks
@@ -1057,7 +1110,7 @@ cudaError_t launch_chunk_t(const AttnArgs &a, cudaStream_t st) {
     const int grid = attn_num_sms();
     e = launch_pdl(kern, dim3((unsigned)grid), dim3(kCkThreads), G::SMEM, st, a);
     if (e != cudaSuccess) return e;
-    return launch_attn_merge(std::is_same<TA, __half>::value, kCkRows, D, grid, 8, a, st);
+    return launch_attn_merge(std::is_same<TA, __half>::value, kCkRows, D, grid, kCkRows / 8, a, st);
 }
 
 template <typename TA>

@@ -393,6 +393,8 @@ int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, i
     a.out = static_cast<uint16_t *>(out);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
+    while ((1 << a.group_shift) < a.group) ++a.group_shift;
+    a.group_mul = (((uint64_t)1 << (31 + a.group_shift)) + a.group - 1) / a.group;
     // a scale of zero (all terms equal) as one that no score makes visible: 0 times a hidden score's -inf is no number
     a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 2e-38f);
     a.window = window > 0 ? window : 0;

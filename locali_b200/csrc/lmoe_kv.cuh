@@ -96,9 +96,13 @@ struct AttnArgs {
     uint16_t *out;
     int32_t q_heads;
     int32_t group;  // query heads of one key/value head
+    uint64_t group_mul;  // ceil(2^(31 + group_shift) / group), 2^group_shift >= group
+    int32_t group_shift;
     float scale_log2;  // scale * log2(e)
     int32_t window, sinks;
     uint8_t *scratch;
+    // x / group for 0 <= x < 2^31: the multiplier is off by less than group, so the quotient by less than 1 / group
+    __device__ __forceinline__ int per_group(int x) const { return (int)((uint64_t)x * group_mul >> (31 + group_shift)); }
 };
 
 cudaError_t launch_attention(int act_f16, int head_dim, int bits, int group_size, const AttnArgs &a, cudaStream_t st);
