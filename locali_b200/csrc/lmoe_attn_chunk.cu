@@ -63,7 +63,7 @@ struct ChunkGeo {
     static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
     static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
-    static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * 4;  // (scale, bias) pairs of the loader warps' rows
+    static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * (int)sizeof(uint2);  // scales and biases of the loader warps' rows
     static constexpr int OFF_STG = OFF_X + SCALES;                   // output staging of the softmax warps
     static constexpr int SMEM = 1024 + OFF_STG + 8 * kStgWarp;
 };

@@ -19,7 +19,8 @@ namespace lmoe {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvMaxRows = 16;  // rows of one block
+constexpr int kKvMaxRows = 32;  // rows of one block
+constexpr int kKvBatch = 4;     // 16-byte pieces of a thread whose loads are in flight together
 
 template <typename TA>
 struct Fin;
@@ -49,13 +50,14 @@ __device__ __forceinline__ uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_
     return d;
 }
 
-// Scale and bias of a group from its finite extremes, as 16-bit values.
+// Scale and bias of a group from its extremes, as 16-bit values; false (both
+// NaN) where the group holds an infinity or a NaN.
 template <typename TA, int BITS>
-__device__ __forceinline__ void group_scale(float lo, float hi, bool bad, uint16_t *s16, uint16_t *b16) {
+__device__ __forceinline__ bool group_scale(float lo, float hi, uint16_t *s16, uint16_t *b16) {
     constexpr float n = (float)((1 << BITS) - 1);
-    if (bad) {
+    if (!(fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f)) {
         *s16 = *b16 = Fin<TA>::kNan;
-        return;
+        return false;
     }
     // the fp32 quotient is the rounded exact one whenever hi - lo is exact in
     // fp32 (both extremes then reproduce each other); fp64 holds the rest
@@ -70,19 +72,95 @@ __device__ __forceinline__ void group_scale(float lo, float hi, bool bad, uint16
         sb = (uint16_t)(sb - 1);
     *s16 = sb;
     *b16 = Act<TA>::from_f(lo);
+    return true;
 }
 
-// clamp(rint((x - b) / s), 0, n) as if computed exactly.  The fp32 quotient
-// is within 5e-5 of the true one up to 255; only next to a half is the exact
-// side needed, from fp64.
+// Pairwise maximum of two packed 16-bit pairs, keeping a NaN.
+template <typename TA>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t x, uint32_t y);
+template <>
+__device__ __forceinline__ uint32_t max2_nan<__nv_bfloat16>(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t max2_nan<__half>(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+
+// Extremes of a group of GS elements, 8 to a lane: the maximum and the
+// negated minimum travel as one packed pair.
+template <typename TA, int GS>
+__device__ __forceinline__ void group_extremes(const uint32_t (&w)[4], float &lo, float &hi) {
+    constexpr uint32_t kNeg = 0x80008000u;
+    const uint32_t h = max2_nan<TA>(max2_nan<TA>(w[0], w[1]), max2_nan<TA>(w[2], w[3]));
+    const uint32_t l = max2_nan<TA>(max2_nan<TA>(w[0] ^ kNeg, w[1] ^ kNeg), max2_nan<TA>(w[2] ^ kNeg, w[3] ^ kNeg));
+    uint32_t m = max2_nan<TA>(__byte_perm(h, l, 0x5410), __byte_perm(h, l, 0x7632));
+#pragma unroll
+    for (int o = 1; o < GS / 8; o <<= 1) m = max2_nan<TA>(m, __shfl_xor_sync(0xffffffffu, m, o));
+    hi = Act<TA>::to_f((uint16_t)(m & 0xFFFFu));
+    lo = -Act<TA>::to_f((uint16_t)(m >> 16));
+}
+
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float &x, float &y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+
+// Codes clamp(rint((x - b) / s), 0, n) of 8 elements (x >= b), as if computed
+// exactly, in the low bytes of q.  (x - b) * (1 / s) in fp32 is within 7e-5
+// of the quotient up to 256 (2^-24 of the difference, 2^-23 of the approximate
+// reciprocal, 2^-24 of the product); only next to a half is the exact side
+// needed, from fp64.  Rounding to an integer is the addition of 1.5 * 2^23,
+// whose sum has the code in its low byte.
 template <int BITS>
-__device__ __forceinline__ uint32_t group_code(float x, float b, float s, float inv) {
-    constexpr float n = (float)((1 << BITS) - 1);
-    const float q = (x - b) * inv;
-    float r = rintf(q);
-    if (!(fabsf(q - r) < 0.4999f && q < 1024.0f))
-        r = s > 0.0f ? (float)rint(((double)x - (double)b) / (double)s) : 0.0f;
-    return (uint32_t)fminf(fmaxf(r, 0.0f), n);
+__device__ __forceinline__ void group_codes(const float (&x)[8], float b, float s, uint32_t (&q)[8]) {
+    constexpr float n = (float)((1 << BITS) - 1), kMagic = 12582912.0f;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const uint64_t nb = f2(-b, -b), i2 = f2(inv, inv), mg = f2(kMagic, kMagic), um = f2(-kMagic, -kMagic);
+    const uint64_t neg = f2(-1.0f, -1.0f);
+    float off = 0.0f, t[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const uint64_t v = mul2(add2(f2(x[e], x[e + 1]), nb), i2);
+        const uint64_t r = add2(v, mg);
+        unf2(r, t[e], t[e + 1]);
+        float d0, d1;
+        unf2(add2(v, mul2(add2(r, um), neg)), d0, d1);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d0)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d1)));
+    }
+    if (!(off < 0.4999f)) {  // the NaN of a subnormal or zero scale too
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+            float y = x[0];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) y = e == k ? x[k] : y;
+            y = kMagic + (s > 0.0f ? (float)rint(((double)y - (double)b) / (double)s) : 0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = e == k ? y : t[k];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(fminf(t[e], kMagic + n));
 }
 
 // where the rows of a block live: page (-1: no place) and slot
@@ -112,9 +190,26 @@ __device__ __forceinline__ void place_rows(const KvCopyArgs &a, int r0, RowPlace
     __syncthreads();
 }
 
-template <typename TA, int BITS, int D>
+// The pieces of a block's rows in turn: piece i = thread + 256 k is piece
+// `u` of row `row` (a row has `units`: keys, then values, by head, 8 elements
+// each), walked without a division.
+struct Piece {
+    int row, u;
+    __device__ __forceinline__ Piece(int units) : row(threadIdx.x / units), u(threadIdx.x % units) {}
+    __device__ __forceinline__ void step(int units, int dr, int du) {
+        row += dr;
+        u += du;
+        if (u >= units) {
+            u -= units;
+            ++row;
+        }
+    }
+};
+
+template <typename TA, int BITS, int D, int GS>
 __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs a) {
     constexpr int LPR = D / 8;  // lanes of a head row
+    constexpr int NG = D / GS;
     __shared__ RowPlace pl[kKvMaxRows];
     __shared__ bool own[kKvMaxRows];
     pdl_wait();
@@ -122,74 +217,74 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs 
     const int r0 = blockIdx.x * a.rows_per_block;
     place_rows(a, r0, pl, own);
     const int units = 2 * a.c.kv_heads * LPR;  // per row
-    const int total = a.rows_per_block * units;
-    for (int i0 = 0; i0 < total; i0 += kKvThreads) {
-        const int i = i0 + threadIdx.x;
-        // whole head rows are in or out, so the lanes of a group agree
-        const int rl = i < total ? i / units : 0;
-        const RowPlace p = pl[rl];
-        const bool in = i < total && p.page >= 0;
-        const int u = i - rl * units;
-        const int hv = u / LPR, c = u % LPR;
-        const int which = hv >= a.c.kv_heads, head = which ? hv - a.c.kv_heads : hv;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (in)
-            x = *reinterpret_cast<const uint4 *>(a.src[which] + (int64_t)(r0 + rl) * a.tok_stride[which] +
-                                                 (int64_t)head * a.head_stride[which] + c * 8);
-        const int64_t row = in ? a.c.row(p.page, head, p.slot) : 0;
-        if constexpr (BITS == 16) {
-            if (in) *reinterpret_cast<uint4 *>(a.c.kv[which] + row * (2 * D) + c * 16) = x;
-        } else {
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            float f[8];
+    const int dr = kKvThreads / units, du = kKvThreads % units;
+    Piece p(units);
+    const int rounds = (a.rows_per_block * units + kKvThreads - 1) / kKvThreads;
+    for (int k = 0; k < rounds; k += kKvBatch) {
+        uint4 x[kKvBatch];
+        Piece at = p;
+        auto where = [&](const Piece &q, int &which, int &head, int &c) -> bool {
+            const int hv = q.u / LPR;
+            c = q.u % LPR;
+            which = hv >= a.c.kv_heads;
+            head = which ? hv - a.c.kv_heads : hv;
+            return q.row < a.rows_per_block && pl[q.row].page >= 0;
+        };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = Act<TA>::to_f((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
-            float lo = f[0], hi = f[0];
-            bool bad = false;
+        for (int b = 0; b < kKvBatch; ++b) {
+            int which, head, c;
+            x[b] = make_uint4(0u, 0u, 0u, 0u);
+            if (where(p, which, head, c))
+                x[b] = *reinterpret_cast<const uint4 *>(a.src[which] + (int64_t)(r0 + p.row) * a.tok_stride[which] +
+                                                        (int64_t)head * a.head_stride[which] + c * 8);
+            p.step(units, dr, du);
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                lo = fminf(lo, f[e]);
-                hi = fmaxf(hi, f[e]);
-                bad |= !(fabsf(f[e]) <= 3.402823466e38f);
-            }
-            uint32_t ibad = bad;
-            for (int o = 1; o < a.c.group_size / 8; o <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                ibad |= __shfl_xor_sync(0xffffffffu, ibad, o);
-            }
-            uint16_t s16, b16;
-            group_scale<TA, BITS>(lo, hi, ibad != 0, &s16, &b16);
-            const float s = Act<TA>::to_f(s16), b = lo;
-            uint32_t q[8];
-            const float inv = 1.0f / s;
+        for (int b = 0; b < kKvBatch; ++b) {
+            int which, head, c;
+            // whole head rows are in or out, so the lanes of a group agree
+            const bool in = where(at, which, head, c);
+            const int64_t row = in ? a.c.row(pl[at.row].page, head, pl[at.row].slot) : 0;
+            at.step(units, dr, du);
+            if constexpr (BITS == 16) {
+                if (in) *reinterpret_cast<uint4 *>(a.c.kv[which] + row * (2 * D) + c * 16) = x[b];
+            } else {
+                const uint32_t w[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+                float f[8], lo, hi;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[e] = ibad ? 0u : group_code<BITS>(f[e], b, s, inv);
-            if (in) {
-                if constexpr (BITS == 8) {
-                    uint2 o;
-                    o.x = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-                    o.y = q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24;
-                    *reinterpret_cast<uint2 *>(a.c.kv[which] + row * D + c * 8) = o;
-                } else {
-                    uint32_t o = 0;
+                for (int e = 0; e < 8; ++e) f[e] = Act<TA>::to_f((uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu));
+                group_extremes<TA, GS>(w, lo, hi);
+                uint16_t s16, b16;
+                const bool fine = group_scale<TA, BITS>(lo, hi, &s16, &b16);
+                uint32_t q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (fine) group_codes<BITS>(f, lo, Act<TA>::to_f(s16), q);
+                if (in) {
+                    if constexpr (BITS == 8) {
+                        uint2 o;
+                        o.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                        o.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+                        *reinterpret_cast<uint2 *>(a.c.kv[which] + row * D + c * 8) = o;
+                    } else {
+                        uint32_t o = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o |= q[e] << (4 * e);
-                    *reinterpret_cast<uint32_t *>(a.c.kv[which] + row * (D / 2) + c * 4) = o;
-                }
-                if (c % (a.c.group_size / 8) == 0) {
-                    const int64_t gi = row * a.c.groups + c / (a.c.group_size / 8);
-                    a.c.scale[which][gi] = s16;
-                    a.c.bias[which][gi] = b16;
+                        for (int e = 0; e < 8; ++e) o |= (q[e] & 15u) << (4 * e);
+                        *reinterpret_cast<uint32_t *>(a.c.kv[which] + row * (D / 2) + c * 4) = o;
+                    }
+                    if (c % (GS / 8) == 0) {
+                        const int64_t gi = row * NG + c / (GS / 8);
+                        a.c.scale[which][gi] = s16;
+                        a.c.bias[which][gi] = b16;
+                    }
                 }
             }
         }
     }
 }
 
-template <typename TA, int BITS, int D>
+template <typename TA, int BITS, int D, int GS>
 __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvCopyArgs a) {
     constexpr int LPR = D / 8;
+    constexpr int NG = D / GS;
     __shared__ RowPlace pl[kKvMaxRows];
     __shared__ bool own[kKvMaxRows];
     pdl_wait();
@@ -197,65 +292,89 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvCopyArgs a)
     const int r0 = blockIdx.x * a.rows_per_block;
     place_rows(a, r0, pl, own);
     const int units = 2 * a.c.kv_heads * LPR;
-    const int total = a.rows_per_block * units;
-    for (int i = threadIdx.x; i < total; i += kKvThreads) {
-        const int rl = i / units;
-        if (!own[rl]) continue;  // no sequence's row: left as it was
-        const RowPlace p = pl[rl];
-        const int u = i - rl * units;
-        const int hv = u / LPR, c = u % LPR;
-        const int which = hv >= a.c.kv_heads, head = which ? hv - a.c.kv_heads : hv;
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (p.page >= 0) {
-            const int64_t row = a.c.row(p.page, head, p.slot);
-            if constexpr (BITS == 16) {
-                o = *reinterpret_cast<const uint4 *>(a.c.kv[which] + row * (2 * D) + c * 16);
-            } else {
-                const int64_t gi = row * a.c.groups + c / (a.c.group_size / 8);
-                const uint32_t s2 = a.c.scale[which][gi] * 0x10001u, b2 = a.c.bias[which][gi] * 0x10001u;
-                uint32_t r[4];
-                if constexpr (BITS == 8) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(a.c.kv[which] + row * D + c * 8);
-                    const uint32_t ww[2] = {w.x, w.y};
+    const int dr = kKvThreads / units, du = kKvThreads % units;
+    Piece p(units);
+    const int rounds = (a.rows_per_block * units + kKvThreads - 1) / kKvThreads;
+    for (int k = 0; k < rounds; k += kKvBatch) {
+        uint4 o[kKvBatch];  // 16 bits: the row's; else the codes, then scale and bias
+        Piece at = p;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t v = ww[e >> 1] >> (16 * (e & 1));
-                        r[e] = fma2<TA>(Act<TA>::pack2((float)(v & 255u), (float)(v >> 8 & 255u)), s2, b2);
-                    }
+        for (int b = 0; b < kKvBatch; ++b) {
+            o[b] = make_uint4(0u, 0u, 0u, 0u);
+            const int hv = p.u / LPR, c = p.u % LPR;
+            const int which = hv >= a.c.kv_heads, head = which ? hv - a.c.kv_heads : hv;
+            if (p.row < a.rows_per_block && pl[p.row].page >= 0) {
+                const int64_t row = a.c.row(pl[p.row].page, head, pl[p.row].slot);
+                if constexpr (BITS == 16) {
+                    o[b] = *reinterpret_cast<const uint4 *>(a.c.kv[which] + row * (2 * D) + c * 16);
                 } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t *>(a.c.kv[which] + row * (D / 2) + c * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t v = w >> (8 * e);
-                        r[e] = fma2<TA>(Act<TA>::pack2((float)(v & 15u), (float)(v >> 4 & 15u)), s2, b2);
+                    const int64_t gi = row * NG + c / (GS / 8);
+                    if constexpr (BITS == 8) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(a.c.kv[which] + row * D + c * 8);
+                        o[b].x = w.x;
+                        o[b].y = w.y;
+                    } else {
+                        o[b].x = *reinterpret_cast<const uint32_t *>(a.c.kv[which] + row * (D / 2) + c * 4);
                     }
+                    o[b].z = a.c.scale[which][gi];
+                    o[b].w = a.c.bias[which][gi];
                 }
-                o = make_uint4(r[0], r[1], r[2], r[3]);
             }
+            p.step(units, dr, du);
         }
-        *reinterpret_cast<uint4 *>(a.dst[which] + ((int64_t)(r0 + rl) * a.c.kv_heads + head) * D + c * 8) = o;
+#pragma unroll
+        for (int b = 0; b < kKvBatch; ++b) {
+            const int hv = at.u / LPR, c = at.u % LPR;
+            const int which = hv >= a.c.kv_heads, head = which ? hv - a.c.kv_heads : hv;
+            const int row = at.row;
+            at.step(units, dr, du);
+            if (row >= a.rows_per_block || !own[row]) continue;  // no sequence's row: left as it was
+            uint4 v = o[b];
+            if constexpr (BITS != 16) {
+                // a row without a place: codes, scale and bias 0
+                const uint32_t s2 = v.z * 0x10001u, b2 = v.w * 0x10001u;
+                uint32_t r[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = BITS == 8 ? (e < 2 ? v.x : v.y) >> (16 * (e & 1)) : v.x >> (8 * e);
+                    const uint32_t c0 = w & (BITS == 8 ? 255u : 15u), c1 = w >> BITS & (BITS == 8 ? 255u : 15u);
+                    r[e] = fma2<TA>(Act<TA>::pack2((float)c0, (float)c1), s2, b2);
+                }
+                v = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+            *reinterpret_cast<uint4 *>(a.dst[which] + ((int64_t)(r0 + row) * a.c.kv_heads + head) * D + c * 8) = v;
+        }
     }
 }
 
-template <typename TA, int BITS, int D>
+template <typename TA, int BITS, int D, int GS>
 cudaError_t launch_kv_t(bool append, KvCopyArgs a, cudaStream_t st) {
-    // few rows: one block each, for latency; many: 8 rows a block
-    a.rows_per_block = a.r.n_rows <= 2048 ? 1 : 8;
+    // few rows: one block each, for latency; many: a block takes several, whose look-up (a search, a length and a page
+    // id, one behind the other) they share
+    a.rows_per_block = a.r.n_rows <= 1024 ? 1 : a.r.n_rows <= 8192 ? 8 : kKvMaxRows;
     const dim3 grid((unsigned)((a.r.n_rows + a.rows_per_block - 1) / a.rows_per_block));
-    return append ? launch_pdl(kv_append_kernel<TA, BITS, D>, grid, dim3(kKvThreads), 0, st, a)
-                  : launch_pdl(kv_read_kernel<TA, BITS, D>, grid, dim3(kKvThreads), 0, st, a);
+    return append ? launch_pdl(kv_append_kernel<TA, BITS, D, GS>, grid, dim3(kKvThreads), 0, st, a)
+                  : launch_pdl(kv_read_kernel<TA, BITS, D, GS>, grid, dim3(kKvThreads), 0, st, a);
 }
 
 template <typename TA>
-cudaError_t launch_kv(bool append, int bits, int D, const KvCopyArgs &a, cudaStream_t st) {
-    if (D == 64) {
-        if (bits == 16) return launch_kv_t<TA, 16, 64>(append, a, st);
-        if (bits == 8) return launch_kv_t<TA, 8, 64>(append, a, st);
-        return launch_kv_t<TA, 4, 64>(append, a, st);
-    }
-    if (bits == 16) return launch_kv_t<TA, 16, 128>(append, a, st);
-    if (bits == 8) return launch_kv_t<TA, 8, 128>(append, a, st);
-    return launch_kv_t<TA, 4, 128>(append, a, st);
+cudaError_t launch_kv(bool append, int bits, int D, int gs, const KvCopyArgs &a, cudaStream_t st) {
+#define LMOE_KV_CASE(B, DD, GG) \
+    if (bits == B && D == DD && (B == 16 || gs == GG)) return launch_kv_t<TA, B, DD, GG>(append, a, st);
+    LMOE_KV_CASE(16, 64, 64)
+    LMOE_KV_CASE(16, 128, 64)
+    LMOE_KV_CASE(8, 64, 32)
+    LMOE_KV_CASE(8, 64, 64)
+    LMOE_KV_CASE(8, 128, 32)
+    LMOE_KV_CASE(8, 128, 64)
+    LMOE_KV_CASE(8, 128, 128)
+    LMOE_KV_CASE(4, 64, 32)
+    LMOE_KV_CASE(4, 64, 64)
+    LMOE_KV_CASE(4, 128, 32)
+    LMOE_KV_CASE(4, 128, 64)
+    LMOE_KV_CASE(4, 128, 128)
+#undef LMOE_KV_CASE
+    return cudaErrorInvalidValue;
 }
 
 bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -340,8 +459,8 @@ int lmoe_kv_append(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, const v
     a.head_stride[0] = k_head_stride;
     a.head_stride[1] = v_head_stride;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return kv_rc(cache->dtype == LMOE_F16 ? launch_kv<__half>(true, cache->bits, cache->head_dim, a, st)
-                                          : launch_kv<__nv_bfloat16>(true, cache->bits, cache->head_dim, a, st));
+    return kv_rc(cache->dtype == LMOE_F16 ? launch_kv<__half>(true, cache->bits, cache->head_dim, cache->group_size, a, st)
+                                          : launch_kv<__nv_bfloat16>(true, cache->bits, cache->head_dim, cache->group_size, a, st));
 }
 
 int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, void *v, void *workspace,
@@ -355,8 +474,8 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
     a.dst[0] = static_cast<uint16_t *>(k);
     a.dst[1] = static_cast<uint16_t *>(v);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return kv_rc(cache->dtype == LMOE_F16 ? launch_kv<__half>(false, cache->bits, cache->head_dim, a, st)
-                                          : launch_kv<__nv_bfloat16>(false, cache->bits, cache->head_dim, a, st));
+    return kv_rc(cache->dtype == LMOE_F16 ? launch_kv<__half>(false, cache->bits, cache->head_dim, cache->group_size, a, st)
+                                          : launch_kv<__nv_bfloat16>(false, cache->bits, cache->head_dim, cache->group_size, a, st));
 }
 
 size_t lmoe_paged_attention_scratch(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, int32_t q_heads) {

@@ -22,6 +22,7 @@ backbone, dsv4_engine.py:22-42).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -32,9 +33,12 @@ from ._lib import check, lmoe
 from .ops import _ACT, Workspace, _need_cuda, _ptr
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Context that makes ``device`` current (the C calls launch there)."""
-    return torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 class PagedKVCache:

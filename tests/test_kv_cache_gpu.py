@@ -506,6 +506,28 @@ def test_refusals(built):
     c.check()
 
 
+@pytest.mark.parametrize("bits,gs", [(16, 32), (8, 32), (4, 64)])
+def test_many_short_chunks(built, bits, gs):
+    """More tiles than launch blocks, so one tile's results leave while the next one's keys and values arrive: every
+    sequence's rows equal those of a call of its own."""
+    rng = np.random.default_rng(4)
+    rows = rng.integers(20, 60, 150).tolist()
+    lens = [int(r + rng.integers(0, 150)) for r in rows]
+    case = Case(lens, rows, bits=bits, gs=gs, d=128, hk=3, page=16)
+    c, q = case.cache, case.q(12)
+    first = c.attend(q, case.table, case.lens, case.start)
+    for _ in range(5):
+        assert torch.equal(first, c.attend(q, case.table, case.lens, case.start))
+    for b in range(0, 150, 7):
+        a, e = case.start_l[b], case.start_l[b + 1]
+        st = torch.tensor([0, e - a], dtype=torch.int32, device="cuda")
+        one = c.attend(q[a:e], case.table[b:b + 1], case.lens[b:b + 1], st)
+        # the same arithmetic unless the tile was cut over two launch blocks: then two sums of terms rounded once
+        assert float((one.float() - first[a:e].float()).abs().max()) <= 4 * 2.0**-8 * float(c.v.abs().max() if bits == 16
+                                                                                           else 6.0)
+    c.check()
+
+
 @pytest.mark.parametrize("rows", [1, 50])
 def test_repeatable_and_on_a_side_stream(built, rows):
     case = Case([3000, 500, 40 + rows], [rows] * 3, bits=8, gs=64, d=128, hk=2, page=64)
