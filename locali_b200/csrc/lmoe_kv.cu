@@ -19,8 +19,8 @@ namespace lmoe {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvMaxRows = 32;  // rows of one block
-constexpr int kKvBatch = 4;     // 16-byte pieces of a thread whose loads are in flight together
+constexpr int kKvMaxRows = 8;  // rows of one block
+constexpr int kKvBatch = 2;     // 16-byte pieces of a thread whose loads are in flight together
 
 template <typename TA>
 struct Fin;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void unf2(uint64_t v, float &x, float &y) {
 // exactly, in the low bytes of q.  (x - b) * (1 / s) in fp32 is within 7e-5
 // of the quotient up to 256 (2^-24 of the difference, 2^-23 of the approximate
 // reciprocal, 2^-24 of the product); only next to a half is the exact side
-// needed, from fp64.  Rounding to an integer is the addition of 1.5 * 2^23,
+// needed (0.02 % of elements, but 15 % of warps).  Rounding to an integer is the addition of 1.5 * 2^23,
 // whose sum has the code in its low byte.
 template <int BITS>
 __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float s, uint32_t (&q)[8]) {
@@ -148,15 +148,30 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float 
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d0)));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d1)));
     }
-    if (!(off < 0.4999f)) {  // the NaN of a subnormal or zero scale too
+    if (!(off < 0.4999f)) {
+        if (off <= 0.5f) {
+            // The side of the half h: the sign of (x - b) - s h.  x - b is d
+            // plus its rounding error, both in fp32; s h (at most 20 bits) and
+            // its difference from the near d are exact.
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = x[e] - b, v = d * inv, r = t[e] - kMagic, f = v - r;
+                const float bp = d - x[e], err = (x[e] - (d - bp)) + (-b - bp);
+                const float low = f > 0.0f ? r : r - 1.0f;
+                const float z = fmaf(-s, low + 0.5f, d) + err;
+                const float tie = low + ((int)low & 1 ? 1.0f : 0.0f);
+                if (!(fabsf(f) < 0.4999f)) t[e] = kMagic + (z == 0.0f ? tie : z > 0.0f ? low + 1.0f : low);
+            }
+        } else {  // a subnormal or zero scale has no reciprocal
 #pragma unroll 1
-        for (int e = 0; e < 8; ++e) {
-            float y = x[0];
+            for (int e = 0; e < 8; ++e) {
+                float y = x[0];
 #pragma unroll
-            for (int k = 1; k < 8; ++k) y = e == k ? x[k] : y;
-            y = kMagic + (s > 0.0f ? (float)rint(((double)y - (double)b) / (double)s) : 0.0f);
+                for (int k = 1; k < 8; ++k) y = e == k ? x[k] : y;
+                y = kMagic + (s > 0.0f ? (float)rint(((double)y - (double)b) / (double)s) : 0.0f);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = e == k ? y : t[k];
+                for (int k = 0; k < 8; ++k) t[k] = e == k ? y : t[k];
+            }
         }
     }
 #pragma unroll
@@ -168,24 +183,38 @@ struct RowPlace {
     int32_t page, slot;
 };
 
+// The first warp finds them: the sequence of the block's first row by
+// counting the row starts up to it, 32 at a time (loads that do not wait for
+// one another, unlike a binary search's), the other rows from there on.
 __device__ __forceinline__ void place_rows(const KvCopyArgs &a, int r0, RowPlace *pl, bool *own) {
-    const int i = threadIdx.x;
-    if (blockIdx.x == 0) a.r.validate(i, kKvThreads);
-    if (i < a.rows_per_block) {
-        RowPlace p{-1, 0};
-        bool mine = false;
-        const int r = r0 + i;
-        if (r < a.r.n_rows) {
-            int pos = 0;
-            const int b = a.r.find(r, &pos);
-            mine = b >= 0 || pos < 0;  // a row of a sequence, with or without a place
-            if (b >= 0) {
-                p.page = a.r.page(a.c, b, pos);
-                p.slot = pos % a.c.page_size;
-            }
+    if (blockIdx.x == 0) a.r.validate(threadIdx.x, kKvThreads);
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, r = r0 + lane;
+        int b = r;
+        if (a.r.row_start) {
+            int n = 0;  // row starts at or in front of r0
+            for (int b0 = 0; b0 <= a.r.n_seqs; b0 += 32)
+                n += __popc(__ballot_sync(0xffffffffu, b0 + lane <= a.r.n_seqs && a.r.start(b0 + lane) <= r0));
+            b = n - 1;
         }
-        pl[i] = p;
-        own[i] = mine;
+        if (lane < a.rows_per_block) {
+            RowPlace p{-1, 0};
+            bool mine = false;
+            if (r < a.r.n_rows && b >= 0) {
+                if (a.r.row_start)
+                    while (b < a.r.n_seqs && a.r.start(b + 1) <= r) ++b;
+                mine = b < a.r.n_seqs;  // a row of a sequence, with or without a place
+                if (mine) {
+                    const int pos = a.r.lens[b] - (a.r.start(b + 1) - r);
+                    if (pos >= 0) {
+                        p.page = a.r.page(a.c, b, pos);
+                        p.slot = pos % a.c.page_size;
+                    }
+                }
+            }
+            pl[lane] = p;
+            own[lane] = mine;
+        }
     }
     __syncthreads();
 }
@@ -207,7 +236,7 @@ struct Piece {
 };
 
 template <typename TA, int BITS, int D, int GS>
-__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs a) {
+__global__ void __launch_bounds__(kKvThreads, 5) kv_append_kernel(const KvCopyArgs a) {
     constexpr int LPR = D / 8;  // lanes of a head row
     constexpr int NG = D / GS;
     __shared__ RowPlace pl[kKvMaxRows];
@@ -215,7 +244,6 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs 
     pdl_wait();
     pdl_trigger();
     const int r0 = blockIdx.x * a.rows_per_block;
-    place_rows(a, r0, pl, own);
     const int units = 2 * a.c.kv_heads * LPR;  // per row
     const int dr = kKvThreads / units, du = kKvThreads % units;
     Piece p(units);
@@ -228,7 +256,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs 
             c = q.u % LPR;
             which = hv >= a.c.kv_heads;
             head = which ? hv - a.c.kv_heads : hv;
-            return q.row < a.rows_per_block && pl[q.row].page >= 0;
+            return q.row < a.rows_per_block && r0 + q.row < a.r.n_rows;
         };
 #pragma unroll
         for (int b = 0; b < kKvBatch; ++b) {
@@ -239,11 +267,12 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs 
                                                         (int64_t)head * a.head_stride[which] + c * 8);
             p.step(units, dr, du);
         }
+        if (k == 0) place_rows(a, r0, pl, own);  // behind the first loads, which do not need it
 #pragma unroll
         for (int b = 0; b < kKvBatch; ++b) {
             int which, head, c;
             // whole head rows are in or out, so the lanes of a group agree
-            const bool in = where(at, which, head, c);
+            const bool in = where(at, which, head, c) && pl[at.row].page >= 0;
             const int64_t row = in ? a.c.row(pl[at.row].page, head, pl[at.row].slot) : 0;
             at.step(units, dr, du);
             if constexpr (BITS == 16) {
@@ -282,7 +311,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvCopyArgs 
 }
 
 template <typename TA, int BITS, int D, int GS>
-__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvCopyArgs a) {
+__global__ void __launch_bounds__(kKvThreads, 6) kv_read_kernel(const KvCopyArgs a) {
     constexpr int LPR = D / 8;
     constexpr int NG = D / GS;
     __shared__ RowPlace pl[kKvMaxRows];
@@ -351,7 +380,7 @@ template <typename TA, int BITS, int D, int GS>
 cudaError_t launch_kv_t(bool append, KvCopyArgs a, cudaStream_t st) {
     // few rows: one block each, for latency; many: a block takes several, whose look-up (a search, a length and a page
     // id, one behind the other) they share
-    a.rows_per_block = a.r.n_rows <= 1024 ? 1 : a.r.n_rows <= 8192 ? 8 : kKvMaxRows;
+    a.rows_per_block = a.r.n_rows <= 1024 ? 1 : kKvMaxRows;
     const dim3 grid((unsigned)((a.r.n_rows + a.rows_per_block - 1) / a.rows_per_block));
     return append ? launch_pdl(kv_append_kernel<TA, BITS, D, GS>, grid, dim3(kKvThreads), 0, st, a)
                   : launch_pdl(kv_read_kernel<TA, BITS, D, GS>, grid, dim3(kKvThreads), 0, st, a);
