@@ -56,11 +56,26 @@ __device__ __forceinline__ int seq_rows(const AttnArgs &a, int b, Tile &t) {
 // of it.  So ragged batches stay level without the host knowing a length, and
 // a tile may be cut over several blocks of the launch; attn_merge_kernel joins
 // those.
+// quotient of values that mostly fit 32 bits
+__device__ __forceinline__ long long div_small(long long x, long long y) {
+    return ((x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
+}
 struct Share {
     long long total;  // units of the stream
+    long long each;   // a run's units; the first `more` runs have one more
     int parts;        // launch blocks that take part
-    __device__ __forceinline__ long long begin(int c) const { return total * c / parts; }
-    __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * parts + total - 1) / total) - 1; }
+    int more;
+    __device__ __forceinline__ void split(long long units, int n) {
+        total = units;
+        parts = n;
+        each = div_small(units, n);
+        more = (int)(units - each * n);
+    }
+    __device__ __forceinline__ long long begin(int c) const { return each * c + min(c, more); }
+    __device__ __forceinline__ int owner(long long x) const {
+        const long long big = (each + 1) * more;
+        return x < big ? (int)div_small(x, each + 1) : more + (int)div_small(x - big, each);
+    }
 };
 
 // A run's place in the stream: the tile, where the stream has its first unit,
@@ -139,11 +154,11 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long lon
     }
     if (lane == 0) sm[warp] = sum;
     __syncthreads();
-    sh.total = 0;
-    for (int w = 0; w < NW; ++w) sh.total += sm[w];
+    long long total = 0;
+    for (int w = 0; w < NW; ++w) total += sm[w];
     __syncthreads();
-    if (sh.total == 0) return false;
-    sh.parts = (int)min((long long)gridDim.x, max(1ll, sh.total / minu));
+    if (total == 0) return false;
+    sh.split(total, (int)min((long long)gridDim.x, max(1ll, div_small(total, minu))));
     if ((int)blockIdx.x >= sh.parts) return false;
     const long long s = sh.begin(blockIdx.x);
     // the sequence that holds unit s
@@ -206,8 +221,8 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long lon
     t.rt = (int)sm[NW + 2];
     tile_range<R, KS>(a, t);
     const long long off = sm[NW + 3];
-    t.h = (int)(off / (t.nblk + X));
-    cur.at = s - off % (t.nblk + X);
+    t.h = (int)div_small(off, t.nblk + X);
+    cur.at = s - (off - (long long)t.h * (t.nblk + X));
     cur.end = sh.begin(blockIdx.x + 1);
     cur.open(s);
     __syncthreads();

@@ -126,13 +126,14 @@ __device__ __forceinline__ void unf2(uint64_t v, float &x, float &y) {
 
 // Codes clamp(rint((x - b) / s), 0, n) of 8 elements (x >= b), as if computed
 // exactly, in the low bytes of q.  (x - b) * (1 / s) in fp32 is within 7e-5
-// of the quotient up to 256 (2^-24 of the difference, 2^-23 of the approximate
+// of the quotient up to 256, 5e-6 up to 16 (2^-24 of the difference, 2^-23 of the approximate
 // reciprocal, 2^-24 of the product); only next to a half is the exact side
 // needed (0.02 % of elements, but 15 % of warps).  Rounding to an integer is the addition of 1.5 * 2^23,
 // whose sum has the code in its low byte.
 template <int BITS>
 __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float s, uint32_t (&q)[8]) {
     constexpr float n = (float)((1 << BITS) - 1), kMagic = 12582912.0f;
+    constexpr float kSure = BITS == 8 ? 0.4999f : 0.49999f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     const uint64_t nb = f2(-b, -b), i2 = f2(inv, inv), mg = f2(kMagic, kMagic), um = f2(-kMagic, -kMagic);
@@ -148,7 +149,7 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float 
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d0)));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d1)));
     }
-    if (!(off < 0.4999f)) {
+    if (!(off < kSure)) {
         if (off <= 0.5f) {
             // The side of the half h: the sign of (x - b) - s h.  x - b is d
             // plus its rounding error, both in fp32; s h (at most 20 bits) and
@@ -160,7 +161,7 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float 
                 const float low = f > 0.0f ? r : r - 1.0f;
                 const float z = fmaf(-s, low + 0.5f, d) + err;
                 const float tie = low + ((int)low & 1 ? 1.0f : 0.0f);
-                if (!(fabsf(f) < 0.4999f)) t[e] = kMagic + (z == 0.0f ? tie : z > 0.0f ? low + 1.0f : low);
+                if (!(fabsf(f) < kSure)) t[e] = kMagic + (z == 0.0f ? tie : z > 0.0f ? low + 1.0f : low);
             }
         } else {  // a subnormal or zero scale has no reciprocal
 #pragma unroll 1
@@ -175,7 +176,7 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float 
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(fminf(t[e], kMagic + n));
+    for (int e = 0; e < 8; ++e) q[e] = __float_as_uint(fminf(t[e], kMagic + n));  // x >= b: no code below 0
 }
 
 // where the rows of a block live: page (-1: no place) and slot
@@ -273,6 +274,10 @@ __global__ void __launch_bounds__(kKvThreads, 5) kv_append_kernel(const KvCopyAr
             int which, head, c;
             // whole head rows are in or out, so the lanes of a group agree
             const bool in = where(at, which, head, c) && pl[at.row].page >= 0;
+            if (!__any_sync(0xffffffffu, in)) {  // the rounds' end, rows without a place
+                at.step(units, dr, du);
+                continue;
+            }
             const int64_t row = in ? a.c.row(pl[at.row].page, head, pl[at.row].slot) : 0;
             at.step(units, dr, du);
             if constexpr (BITS == 16) {
@@ -294,9 +299,10 @@ __global__ void __launch_bounds__(kKvThreads, 5) kv_append_kernel(const KvCopyAr
                         o.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
                         *reinterpret_cast<uint2 *>(a.c.kv[which] + row * D + c * 8) = o;
                     } else {
-                        uint32_t o = 0;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) o |= (q[e] & 15u) << (4 * e);
+                        // even codes in the low, odd ones in the high nibbles of the bytes
+                        const uint32_t ev = __byte_perm(__byte_perm(q[0], q[2], 0x0040), __byte_perm(q[4], q[6], 0x0040), 0x5410);
+                        const uint32_t od = __byte_perm(__byte_perm(q[1], q[3], 0x0040), __byte_perm(q[5], q[7], 0x0040), 0x5410);
+                        const uint32_t o = ev | od << 4;
                         *reinterpret_cast<uint32_t *>(a.c.kv[which] + row * (D / 2) + c * 4) = o;
                     }
                     if (c % (GS / 8) == 0) {
