@@ -100,14 +100,21 @@ __device__ __forceinline__ void sts_u16(uint32_t a, uint16_t v) {
 // row's parity (rows g with 4 neighbouring chunks), V codes by the row pair
 // (lane t reads rows 2t and 2t + 1).
 template <int BITS, int D, int WHICH>
-__device__ __forceinline__ int unit_off(int row, int o) {
+__host__ __device__ constexpr int unit_swizzle(int row) {
     constexpr int RB = D * BITS / 8;
-    const int lin = row * RB + o;
-    int h = 0;
-    if constexpr (BITS == 16) h = row & 7;
-    else if constexpr (WHICH == 0) h = RB == 128 ? (row & 1) << 2 : 0;
-    else h = RB == 32 ? ((row >> 2) & 1) << 1 : ((row >> 1) & 3) << 1;
-    return lin ^ (h << 4);
+    if (BITS == 16) return (row & 7) << 4;
+    if (WHICH == 0) return RB == 128 ? (row & 1) << 6 : 0;
+    return RB == 32 ? (row & 4) << 3 : (row & 6) << 4;
+}
+template <int BITS, int D, int WHICH>
+__device__ __forceinline__ int unit_off(int row, int o) {
+    return (row * (D * BITS / 8) + o) ^ unit_swizzle<BITS, D, WHICH>(row);
+}
+// The same for row base + r, where `base` is known at compile time and has no
+// bit of r, and base rows are whole 128-byte lines: `part` is unit_off(r, o).
+template <int BITS, int D, int WHICH>
+__device__ __forceinline__ uint32_t unit_at(int base, uint32_t part) {
+    return base * (D * BITS / 8) + (part ^ unit_swizzle<BITS, D, WHICH>(base));
 }
 
 template <typename TA, int BITS, int D, int GS, int NT>
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const int p = t.block(b0 + warp + i * kRowWarps) * KS + lane * 16;
                 if (p < t.hi) {
                     const int32_t pg = a.r.page(a.c, t.b, p);
-                    r = pg < 0 ? -1 : a.c.row(pg, t.h, p % a.c.page_size);
+                    r = pg < 0 ? -1 : a.c.row(pg, t.h, a.c.slot_of(p));
                 }
             }
             return r;
@@ -219,19 +226,27 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
                 const uint32_t u = ring + slot * G::UB;
                 const int r0 = lane / (RB / 16), c0 = lane % (RB / 16);
+                const uint32_t part = unit_off<BITS, D, W>(r0, c0 * 16);
                 const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, runs == -1);
+                const uint8_t *const kv = a.c.kv[W] + lane * 16;
+                if (all) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const long long run = __shfl_sync(0xffffffffu, runs, kt);
-                    const uint8_t *src = a.c.kv[W] + (run < 0 ? 0 : run * RB + lane * 16);
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const uint8_t *src = kv + __shfl_sync(0xffffffffu, runs, kt) * RB;
 #pragma unroll
-                    for (int it = 0; it < 16 / RPI; ++it) {
-                        const int row = kt * 16 + it * RPI + r0;
-                        const uint32_t dst = u + unit_off<BITS, D, W>(row, c0 * 16);
-                        if (all) cp16(dst, src + it * 512);
-                        else {
+                        for (int it = 0; it < 16 / RPI; ++it)
+                            cp16(u + unit_at<BITS, D, W>(kt * 16 + it * RPI, part), src + it * 512);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const long long run = __shfl_sync(0xffffffffu, runs, kt);
+#pragma unroll 1
+                        for (int it = 0; it < 16 / RPI; ++it) {
+                            const int row = kt * 16 + it * RPI + r0;
                             const bool in = run >= 0 && k0 + row < t.hi;
-                            cp16z(dst, in ? src + it * 512 : a.c.kv[W], in ? 16 : 0);
+                            cp16z(u + unit_off<BITS, D, W>(row, c0 * 16), in ? kv + run * RB + it * 512 : a.c.kv[W],
+                                  in ? 16 : 0);
                         }
                     }
                 }
@@ -278,11 +293,11 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.0f;
                 if constexpr (BITS == 16) {
-                    const int r = kt * 16 + (lane & 15), ch = lane >> 4;
+                    const uint32_t part = unit_off<16, D, 0>(lane & 15, (lane >> 4) * 16);
 #pragma unroll
                     for (int x = 0; x < QS; ++x) {
                         uint32_t f[4];
-                        ldsm4(ku + unit_off<16, D, 0>(r, (2 * x + ch) * 16), f);
+                        ldsm4(ku + kt * 16 * RB + (part ^ (x * 32)), f);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             Act<TA>::mma(s[kt][n], f[0], f[1], f[2], f[3], qf[n][x][0], qf[n][x][1]);
@@ -294,11 +309,12 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                     for (int nc = 0; nc < NC; ++nc) {
                         uint32_t w[2][WC], s2[2], b2[2];
                         const int dim0 = BITS == 8 ? 64 * nc + 16 * t4 : (D / 4) * t4;
+                        const uint32_t part = unit_off<BITS, D, 0>(g, dim0 * BITS / 8);
+                        const uint32_t spart = ku + G::CB + (g * NG + dim0 / GS) * 2;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const int r = kt * 16 + 8 * h + g;
-                            lds_words<WC>(ku + unit_off<BITS, D, 0>(r, dim0 * BITS / 8), w[h]);
-                            const uint32_t so = ku + G::CB + (r * NG + dim0 / GS) * 2;
+                            lds_words<WC>(ku + unit_at<BITS, D, 0>(kt * 16 + 8 * h, part), w[h]);
+                            const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2;
                             s2[h] = Pair<TA>::template scale<BITS>(lds_u16(so) * 0x10001u);
                             b2[h] = lds_u16(so + G::SB) * 0x10001u;
                         }
@@ -339,16 +355,21 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[kt][n][e] *= sc;
-                        if (!full) {
+                    for (int e = 0; e < 4; ++e) s[kt][n][e] *= sc;
+            if (!full) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
                             const int j = k0 + kt * 16 + g + 8 * (e >> 1), p = pos[n][e & 1];
                             const bool see = j <= p && !(bad >> kt & 1u) &&
                                              (a.window == 0 || p - j < a.window || j < a.sinks);
                             seen[n][e & 1] |= see;
                             if (!see) s[kt][n][e] = -INFINITY;
                         }
-                    }
+            }
             bool moved = false;
             float mu[NT][2], f[NT][2];
 #pragma unroll
@@ -472,11 +493,11 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 if constexpr (BITS == 16) {
-                    const int r = kt * 16 + (lane & 7) + (lane >> 4) * 8, ch = lane >> 3 & 1;
+                    const uint32_t part = unit_off<16, D, 1>((lane & 7) + (lane >> 4) * 8, (lane >> 3 & 1) * 16);
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
                         uint32_t f4[4];
-                        ldsm4t(vu + unit_off<16, D, 1>(r, (2 * x + ch) * 16), f4);
+                        ldsm4t(vu + kt * 16 * RB + (part ^ (x * 32)), f4);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             Act<TA>::mma(o[n][x], f4[0], f4[1], f4[2], f4[3], pf[kt][n][0], pf[kt][n][1]);
@@ -487,18 +508,20 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                     // is dim (D / 8) g + x, row g + 8 is D / 16 further
                     constexpr int WL = RB / 8 / 4;  // words of the lane's dims
                     uint32_t u[2][WL][2], s2[2], b2[2];
+                    const uint32_t part0 = unit_off<BITS, D, 1>(2 * t4, g * (RB / 8));
+                    const uint32_t part1 = unit_off<BITS, D, 1>(2 * t4 + 1, g * (RB / 8));
+                    const uint32_t spart = vu + G::CB + (2 * t4 * NG + (D / 8) * g / GS) * 2;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int r = kt * 16 + 8 * h + 2 * t4;
                         uint32_t w0[WL], w1[WL];
-                        lds_words<WL>(vu + unit_off<BITS, D, 1>(r, g * (RB / 8)), w0);
-                        lds_words<WL>(vu + unit_off<BITS, D, 1>(r + 1, g * (RB / 8)), w1);
+                        lds_words<WL>(vu + unit_at<BITS, D, 1>(kt * 16 + 8 * h, part0), w0);
+                        lds_words<WL>(vu + unit_at<BITS, D, 1>(kt * 16 + 8 * h, part1), w1);
 #pragma unroll
                         for (int x = 0; x < WL; ++x) {
                             u[h][x][0] = __byte_perm(w0[x], w1[x], 0x5410);
                             u[h][x][1] = __byte_perm(w0[x], w1[x], 0x7632);
                         }
-                        const uint32_t so = vu + G::CB + (r * NG + (D / 8) * g / GS) * 2;
+                        const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2;
                         s2[h] = Pair<TA>::template scale<BITS>(lds_u16(so) | lds_u16(so + NG * 2) << 16);
                         b2[h] = lds_u16(so + G::SB) | lds_u16(so + G::SB + NG * 2) << 16;
                     }

@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         const bool sees = j < see_hi && (j >= see_lo || j < see_sink);
                         const int32_t pg = a.r.page(a.c, ti.b, j);
                         if (pg < 0) continue;
-                        const int64_t kr = a.c.row(pg, ti.h, j % a.c.page_size);
+                        const int64_t kr = a.c.row(pg, ti.h, a.c.slot_of(j));
 #pragma unroll 1
                         for (int d = 0; d < D; ++d) {
                             float y;
@@ -1056,7 +1056,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 int32_t pg = -1;
                 int sl = -1;
                 if (lane < kCkKeys / 16 && p < ti.hi) {
-                    const int en = p / a.c.page_size;
+                    const int en = a.c.page_of(p);
                     sl = p - en * a.c.page_size;
                     if (en < a.r.table_width) pg = a.r.table[(int64_t)ti.b * a.r.table_stride + en];
                 }

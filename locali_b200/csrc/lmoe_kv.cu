@@ -209,7 +209,7 @@ __device__ __forceinline__ void place_rows(const KvCopyArgs &a, int r0, RowPlace
                     const int pos = a.r.lens[b] - (a.r.start(b + 1) - r);
                     if (pos >= 0) {
                         p.page = a.r.page(a.c, b, pos);
-                        p.slot = pos % a.c.page_size;
+                        p.slot = a.c.slot_of(pos);
                     }
                 }
             }
@@ -441,6 +441,8 @@ int check_cache(const lmoe_kv_cache *c, KvView *v) {
     }
     v->n_pages = c->n_pages;
     v->page_size = c->page_size;
+    while (((int64_t)1 << v->page_shift) < c->page_size) ++v->page_shift;
+    v->page_mul = (((uint64_t)1 << (31 + v->page_shift)) + c->page_size - 1) / c->page_size;
     v->kv_heads = c->kv_heads;
     v->row_bytes = c->head_dim * c->bits / 8;
     return LMOE_OK;

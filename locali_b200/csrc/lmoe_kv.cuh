@@ -20,6 +20,12 @@ struct KvView {
     int32_t row_bytes;  // bytes of one head row: head_dim * bits / 8
     int32_t groups;     // groups of one head row
     int32_t group_size;
+    uint64_t page_mul;  // ceil(2^(31 + page_shift) / page_size), 2^page_shift >= page_size
+    int32_t page_shift;
+    // p / page_size for 0 <= p < 2^31: the multiplier is off by less than
+    // page_size, so the quotient by less than 1 / page_size
+    __device__ __forceinline__ int page_of(int p) const { return (int)((uint64_t)p * page_mul >> (31 + page_shift)); }
+    __device__ __forceinline__ int slot_of(int p) const { return p - page_of(p) * page_size; }
     // row index (of head rows) of a slot in a page
     __device__ __forceinline__ int64_t row(int32_t page, int32_t head, int32_t slot) const {
         return ((int64_t)page * kv_heads + head) * page_size + slot;
@@ -50,7 +56,7 @@ struct KvRows {
     }
     // the page that holds position p of sequence b, -1 when it has none
     __device__ __forceinline__ int32_t page(const KvView &c, int b, int p) const {
-        const int e = p / c.page_size;
+        const int e = c.page_of(p);
         int32_t pg = -1;
         if (e < table_width) pg = table[(int64_t)b * table_stride + e];
         if (pg < 0 || pg >= c.n_pages) {
@@ -58,24 +64,6 @@ struct KvRows {
             pg = -1;
         }
         return pg;
-    }
-    // The sequence that row r belongs to (the last b with start(b) <= r), its
-    // position in *pos; -1 when it belongs to none or has no place.
-    __device__ __forceinline__ int find(int r, int *pos) const {
-        int b = r;
-        if (row_start) {
-            int lo = 0, hi = n_seqs + 1;
-            while (lo < hi) {  // first b in [0, n_seqs] with start(b) > r, else n_seqs + 1
-                const int m = (lo + hi) >> 1;
-                if (start(m) > r) hi = m;
-                else lo = m + 1;
-            }
-            b = lo - 1;
-        }
-        if (b < 0 || b >= n_seqs) return -1;
-        const int p = lens[b] - (start(b + 1) - r);
-        *pos = p;
-        return p < 0 ? -1 : b;
     }
 };
 
