@@ -19,6 +19,15 @@
 // operands that come from memory can be assembled in registers straight from
 // codes: the contraction order of K (the head dimension) and the row order of
 // V^T are free, so a lane takes whole words of codes where they lie.
+//
+// Quantised keys are contracted as codes, one group of the head dimension
+// after the other; scale and bias meet the group's fp32 sum, s (q . c) + b
+// sum(q), so a key is never rounded (rounded to bf16 first, the keys were the
+// largest part of a result's error, 2.9e-3 of 3.9e-3) and a code costs two
+// instructions instead of four.  A constant added to the codes by the cheapest
+// way to make them numbers (128 or 1024) is taken off with the bias.  Values
+// are dequantised to the 16-bit type: there a scale belongs to a position of
+// the contraction.
 #include "lmoe_attn.cuh"
 
 namespace lmoe {
@@ -96,25 +105,28 @@ __device__ __forceinline__ void sts_u16(uint32_t a, uint16_t v) {
 
 // Byte offset in a unit's codes of byte `o` of position `row`.  16-byte chunks
 // are XOR-swizzled inside 128-byte lines so that a warp's reads fall in
-// distinct banks: 16-bit rows by the row (ldmatrix of 8 rows), K codes by the
-// row's parity (rows g with 4 neighbouring chunks), V codes by the row pair
-// (lane t reads rows 2t and 2t + 1).
-template <int BITS, int D, int WHICH>
+// distinct banks: 16-bit rows by the row (ldmatrix of 8 rows); K codes, of
+// which lane t of rows g = 0..7 reads the t-th quarter of a group (SEG bytes),
+// so that the segments of as many rows as are read at once lie apart; V codes
+// by the row pair (lane t reads rows 2t and 2t + 1).
+template <int BITS, int D, int GS, int WHICH>
 __host__ __device__ constexpr int unit_swizzle(int row) {
-    constexpr int RB = D * BITS / 8;
+    constexpr int RB = D * BITS / 8, SEG = GS * BITS / 8;
     if (BITS == 16) return (row & 7) << 4;
-    if (WHICH == 0) return RB == 128 ? (row & 1) << 6 : 0;
-    return RB == 32 ? (row & 4) << 3 : (row & 6) << 4;
+    if (WHICH == 1) return RB == 32 ? (row & 4) << 3 : (row & 6) << 4;
+    if (RB == 128) return SEG == 128 ? (row & 1) << 4 : SEG == 64 ? (row & 1) << 6 : (row & 3) << 5;
+    if (RB == 64) return SEG == 64 ? 0 : SEG == 32 ? (row & 2) << 4 : (row & 6) << 3;
+    return SEG == 32 ? 0 : (row & 4) << 2;
 }
-template <int BITS, int D, int WHICH>
+template <int BITS, int D, int GS, int WHICH>
 __device__ __forceinline__ int unit_off(int row, int o) {
-    return (row * (D * BITS / 8) + o) ^ unit_swizzle<BITS, D, WHICH>(row);
+    return (row * (D * BITS / 8) + o) ^ unit_swizzle<BITS, D, GS, WHICH>(row);
 }
 // The same for row base + r, where `base` is known at compile time and has no
 // bit of r, and base rows are whole 128-byte lines: `part` is unit_off(r, o).
-template <int BITS, int D, int WHICH>
+template <int BITS, int D, int GS, int WHICH>
 __device__ __forceinline__ uint32_t unit_at(int base, uint32_t part) {
-    return base * (D * BITS / 8) + (part ^ unit_swizzle<BITS, D, WHICH>(base));
+    return base * (D * BITS / 8) + (part ^ unit_swizzle<BITS, D, GS, WHICH>(base));
 }
 
 template <typename TA, int BITS, int D, int GS, int NT>
@@ -162,22 +174,19 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         x0 = *reinterpret_cast<const uint32_t *>(q + 16 * s + 2 * t4);
                         x1 = *reinterpret_cast<const uint32_t *>(q + 16 * s + 8 + 2 * t4);
                     }
-                } else if constexpr (BITS == 8) {
-                    // codes (c0, c2), (c1, c3) of word s of the lane's chunk
+                } else {
+                    // step s: word (or half of a word's code pairs) s % SPG of
+                    // the lane's quarter of group s / SPG
+                    constexpr int SPG = GS / 16;
+                    const int d0 = (s / SPG) * GS + t4 * (GS / 4) + (BITS == 8 ? 4 * (s % SPG) : 8 * (s % SPG >> 1) + 2 * (s & 1));
                     uint2 v = make_uint2(0u, 0u);
-                    if (in) v = *reinterpret_cast<const uint2 *>(q + 64 * (s >> 2) + 16 * t4 + 4 * (s & 3));
+                    if (in) {
+                        v.x = *reinterpret_cast<const uint32_t *>(q + d0);
+                        v.y = *reinterpret_cast<const uint32_t *>(q + d0 + (BITS == 8 ? 2 : 4));
+                    }
+                    // 8 bits: codes (c0, c2), (c1, c3); 4 bits: (c0, c4), (c1, c5), then (c2, c6), (c3, c7)
                     x0 = __byte_perm(v.x, v.y, 0x5410);
                     x1 = __byte_perm(v.x, v.y, 0x7632);
-                } else {
-                    // codes (c0, c4), (c1, c5) of word s / 2, then (c2, c6), (c3, c7)
-                    uint2 lo = make_uint2(0u, 0u);
-                    if (in) {
-                        const uint16_t *p = q + t4 * (D / 4) + 8 * (s >> 1) + 2 * (s & 1);
-                        lo.x = *reinterpret_cast<const uint32_t *>(p);
-                        lo.y = *reinterpret_cast<const uint32_t *>(p + 4);
-                    }
-                    x0 = __byte_perm(lo.x, lo.y, 0x5410);
-                    x1 = __byte_perm(lo.x, lo.y, 0x7632);
                 }
                 qf[n][s][0] = x0;
                 qf[n][s][1] = x1;
@@ -187,6 +196,25 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const int rc = t.rt * R + n * 8 + 2 * t4 + c;
                 pos[n][c] = rc < t.n * a.group ? t.first + a.per_group(rc) : -1;
             }
+        }
+        // sums of the columns' rows over the groups
+        float qs[NT][2][NG ? NG : 1];
+        if constexpr (Q) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int gi = 0; gi < NG; ++gi) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int s = gi * (GS / 16); s < (gi + 1) * (GS / 16); ++s)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            x += Act<TA>::to_f((uint16_t)(qf[n][s][h] & 0xFFFFu)) + Act<TA>::to_f((uint16_t)(qf[n][s][h] >> 16));
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) qs[n][c][gi] = __shfl_sync(0xffffffffu, x, (2 * t4 + c) * 4);
+                }
         }
         float o[NT][MT][4], m[NT][2], l[NT][2];
         bool seen[NT][2];
@@ -226,7 +254,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
                 const uint32_t u = ring + slot * G::UB;
                 const int r0 = lane / (RB / 16), c0 = lane % (RB / 16);
-                const uint32_t part = unit_off<BITS, D, W>(r0, c0 * 16);
+                const uint32_t part = unit_off<BITS, D, GS, W>(r0, c0 * 16);
                 const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, runs == -1);
                 const uint8_t *const kv = a.c.kv[W] + lane * 16;
                 if (all) {
@@ -235,7 +263,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         const uint8_t *src = kv + __shfl_sync(0xffffffffu, runs, kt) * RB;
 #pragma unroll
                         for (int it = 0; it < 16 / RPI; ++it)
-                            cp16(u + unit_at<BITS, D, W>(kt * 16 + it * RPI, part), src + it * 512);
+                            cp16(u + unit_at<BITS, D, GS, W>(kt * 16 + it * RPI, part), src + it * 512);
                     }
                 } else {
 #pragma unroll 1
@@ -245,7 +273,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         for (int it = 0; it < 16 / RPI; ++it) {
                             const int row = kt * 16 + it * RPI + r0;
                             const bool in = run >= 0 && k0 + row < t.hi;
-                            cp16z(u + unit_off<BITS, D, W>(row, c0 * 16), in ? kv + run * RB + it * 512 : a.c.kv[W],
+                            cp16z(u + unit_off<BITS, D, GS, W>(row, c0 * 16), in ? kv + run * RB + it * 512 : a.c.kv[W],
                                   in ? 16 : 0);
                         }
                     }
@@ -293,7 +321,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.0f;
                 if constexpr (BITS == 16) {
-                    const uint32_t part = unit_off<16, D, 0>(lane & 15, (lane >> 4) * 16);
+                    const uint32_t part = unit_off<16, D, GS, 0>(lane & 15, (lane >> 4) * 16);
 #pragma unroll
                     for (int x = 0; x < QS; ++x) {
                         uint32_t f[4];
@@ -303,46 +331,50 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             Act<TA>::mma(s[kt][n], f[0], f[1], f[2], f[3], qf[n][x][0], qf[n][x][1]);
                     }
                 } else {
-                    constexpr int NC = BITS == 8 && D == 128 ? 2 : 1;  // word chunks of a lane's row part
-                    constexpr int WC = RB / 4 / 4 / NC;                // words of a chunk
+                    constexpr int SEG = GS * BITS / 8, WPG = SEG / 16;  // bytes of a group, words of a lane's quarter
+                    constexpr int WV = WPG < 4 ? WPG : 4;               // read at once
+                    using RC = RawCode<TA, BITS>;
+                    const uint32_t part = unit_off<BITS, D, GS, 0>(g, t4 * (SEG / 4));
+                    const uint32_t spart = ku + G::CB + g * NG * 2;
 #pragma unroll
-                    for (int nc = 0; nc < NC; ++nc) {
-                        uint32_t w[2][WC], s2[2], b2[2];
-                        const int dim0 = BITS == 8 ? 64 * nc + 16 * t4 : (D / 4) * t4;
-                        const uint32_t part = unit_off<BITS, D, 0>(g, dim0 * BITS / 8);
-                        const uint32_t spart = ku + G::CB + (g * NG + dim0 / GS) * 2;
+                    for (int gi = 0; gi < NG; ++gi) {
+                        float sf[2], bf[2], acc[NT][4];
+                        uint32_t w[2][WPG];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            lds_words<WC>(ku + unit_at<BITS, D, 0>(kt * 16 + 8 * h, part), w[h]);
-                            const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2;
-                            s2[h] = Pair<TA>::template scale<BITS>(lds_u16(so) * 0x10001u);
-                            b2[h] = lds_u16(so + G::SB) * 0x10001u;
+#pragma unroll
+                            for (int x = 0; x < WPG; x += WV) {
+                                uint32_t y[WV];
+                                lds_words<WV>(ku + (kt * 16 + 8 * h) * RB + (part ^ (gi * SEG + x * 4)), y);
+#pragma unroll
+                                for (int e = 0; e < WV; ++e) w[h][x + e] = y[e];
+                            }
+                            const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2 + gi * 2;
+                            const float sv = Act<TA>::to_f((uint16_t)lds_u16(so)), bv = Act<TA>::to_f((uint16_t)lds_u16(so + G::SB));
+                            // a scale or bias that is no number (0 times it is none either) makes the key's score none
+                            bf[h] = fmaf(-RC::kOffset, sv, bv) + ((sv - sv) + (bv - bv));
+                            sf[h] = sv * RC::kScale;
                         }
 #pragma unroll
-                        for (int x = 0; x < WC; ++x) {
-                            if constexpr (BITS == 8) {
-                                const int st = nc * WC + x;
-                                const uint32_t a0 = code_pair<TA, 8>(w[0][x], 0, s2[0], b2[0]);
-                                const uint32_t a1 = code_pair<TA, 8>(w[1][x], 0, s2[1], b2[1]);
-                                const uint32_t a2 = code_pair<TA, 8>(w[0][x], 1, s2[0], b2[0]);
-                                const uint32_t a3 = code_pair<TA, 8>(w[1][x], 1, s2[1], b2[1]);
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < WPG; ++x)
+#pragma unroll
+                            for (int hf = 0; hf < (BITS == 4 ? 2 : 1); ++hf) {
+                                const int st = gi * (GS / 16) + (BITS == 4 ? 2 * x + hf : x);
+                                const uint32_t a0 = RC::pair(w[0][x], 2 * hf), a1 = RC::pair(w[1][x], 2 * hf);
+                                const uint32_t a2 = RC::pair(w[0][x], 2 * hf + 1), a3 = RC::pair(w[1][x], 2 * hf + 1);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
-                                    Act<TA>::mma(s[kt][n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
-                            } else {
-#pragma unroll
-                                for (int hf = 0; hf < 2; ++hf) {
-                                    const int st = 2 * x + hf;
-                                    const uint32_t a0 = code_pair<TA, 4>(w[0][x], 2 * hf, s2[0], b2[0]);
-                                    const uint32_t a1 = code_pair<TA, 4>(w[1][x], 2 * hf, s2[1], b2[1]);
-                                    const uint32_t a2 = code_pair<TA, 4>(w[0][x], 2 * hf + 1, s2[0], b2[0]);
-                                    const uint32_t a3 = code_pair<TA, 4>(w[1][x], 2 * hf + 1, s2[1], b2[1]);
-#pragma unroll
-                                    for (int n = 0; n < NT; ++n)
-                                        Act<TA>::mma(s[kt][n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
-                                }
+                                    Act<TA>::mma(acc[n], a0, a1, a2, a3, qf[n][st][0], qf[n][st][1]);
                             }
-                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                s[kt][n][e] = fmaf(sf[e >> 1], acc[n][e], fmaf(bf[e >> 1], qs[n][e & 1][gi], s[kt][n][e]));
                     }
                 }
             }
@@ -452,13 +484,13 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                                 if constexpr (Q) {
                                     const int byte = dim * BITS / 8;
                                     uint32_t w[1];
-                                    lds_words<1>(vu + unit_off<BITS, D, 1>(k, byte & ~3), w);
+                                    lds_words<1>(vu + unit_off<BITS, D, GS, 1>(k, byte & ~3), w);
                                     const uint32_t code = w[0] >> (dim * BITS % 32) & ((1u << BITS) - 1u);
                                     const uint32_t so = vu + G::CB + (k * SW + dim / GS) * 2;
                                     v = fmaf(Act<TA>::to_f((uint16_t)lds_u16(so)), (float)code,
                                              Act<TA>::to_f((uint16_t)lds_u16(so + G::SB)));
                                 } else {
-                                    v = Act<TA>::to_f((uint16_t)lds_u16(vu + unit_off<16, D, 1>(k, dim * 2)));
+                                    v = Act<TA>::to_f((uint16_t)lds_u16(vu + unit_off<16, D, GS, 1>(k, dim * 2)));
                                 }
                                 if (!(fabsf(v) <= 3.402823466e38f)) {
 #pragma unroll
@@ -493,7 +525,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 if constexpr (BITS == 16) {
-                    const uint32_t part = unit_off<16, D, 1>((lane & 7) + (lane >> 4) * 8, (lane >> 3 & 1) * 16);
+                    const uint32_t part = unit_off<16, D, GS, 1>((lane & 7) + (lane >> 4) * 8, (lane >> 3 & 1) * 16);
 #pragma unroll
                     for (int x = 0; x < MT; ++x) {
                         uint32_t f4[4];
@@ -508,14 +540,14 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                     // is dim (D / 8) g + x, row g + 8 is D / 16 further
                     constexpr int WL = RB / 8 / 4;  // words of the lane's dims
                     uint32_t u[2][WL][2], s2[2], b2[2];
-                    const uint32_t part0 = unit_off<BITS, D, 1>(2 * t4, g * (RB / 8));
-                    const uint32_t part1 = unit_off<BITS, D, 1>(2 * t4 + 1, g * (RB / 8));
+                    const uint32_t part0 = unit_off<BITS, D, GS, 1>(2 * t4, g * (RB / 8));
+                    const uint32_t part1 = unit_off<BITS, D, GS, 1>(2 * t4 + 1, g * (RB / 8));
                     const uint32_t spart = vu + G::CB + (2 * t4 * NG + (D / 8) * g / GS) * 2;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t w0[WL], w1[WL];
-                        lds_words<WL>(vu + unit_at<BITS, D, 1>(kt * 16 + 8 * h, part0), w0);
-                        lds_words<WL>(vu + unit_at<BITS, D, 1>(kt * 16 + 8 * h, part1), w1);
+                        lds_words<WL>(vu + unit_at<BITS, D, GS, 1>(kt * 16 + 8 * h, part0), w0);
+                        lds_words<WL>(vu + unit_at<BITS, D, GS, 1>(kt * 16 + 8 * h, part1), w1);
 #pragma unroll
                         for (int x = 0; x < WL; ++x) {
                             u[h][x][0] = __byte_perm(w0[x], w1[x], 0x5410);

@@ -311,6 +311,21 @@ struct Pair<__half> {
     static constexpr uint32_t kExpMask = 0x7C00u;
 };
 
+// Pair j of a word's two halves as an operand without scale and bias: 4-bit
+// codes j = 0..3 and f16 8-bit codes carry kRawOffset, bf16 8-bit codes are
+// multiplied by 1 / kRawScale.
+template <typename TA, int BITS>
+struct RawCode {
+    static constexpr bool kBf = std::is_same<TA, __nv_bfloat16>::value;
+    static constexpr float kOffset = kBf ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f;
+    static constexpr float kScale = kBf && BITS == 8 ? 64.0f : 1.0f;
+    __device__ __forceinline__ static uint32_t pair(uint32_t u, int j) {
+        if constexpr (BITS == 4) return and_or(u >> (4 * j), 0x000F000Fu, Act<TA>::kMagic);
+        else if constexpr (kBf) return Pair<TA>::mul(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, 0x7F007F00u);
+        else return j ? __byte_perm(u, 0x64646464u, 0x4341) : and_or(u, 0x00FF00FFu, 0x64006400u);
+    }
+};
+
 // Value pair j of a word's two halves: 4-bit codes j = 0..3, 8-bit codes j = 0..1.
 template <typename TA, int BITS>
 __device__ __forceinline__ uint32_t code_pair(uint32_t u, int j, uint32_t s2, uint32_t b2) {
