@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
     constexpr bool Q = BITS != 16;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long s_plan[kRowWarps + 4];
+    __shared__ float s_qs[kRowWarps][NG ? NG : 1][R];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(sm) + warp * (G::NU * G::UB);
     float *s_o = reinterpret_cast<float *>(sm);
@@ -197,8 +198,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 pos[n][c] = rc < t.n * a.group ? t.first + a.per_group(rc) : -1;
             }
         }
-        // sums of the columns' rows over the groups
-        float qs[NT][2][NG ? NG : 1];
+        // sums of the tile's rows over the groups, in shared memory: registers are short
         if constexpr (Q) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             x += Act<TA>::to_f((uint16_t)(qf[n][s][h] & 0xFFFFu)) + Act<TA>::to_f((uint16_t)(qf[n][s][h] >> 16));
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) qs[n][c][gi] = __shfl_sync(0xffffffffu, x, (2 * t4 + c) * 4);
+                    __syncwarp();
+                    if (t4 == 0) s_qs[warp][gi][n * 8 + g] = x;
                 }
+            __syncwarp();
         }
         float o[NT][MT][4], m[NT][2], l[NT][2];
         bool seen[NT][2];
@@ -315,12 +316,14 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
             float s[KT][NT][4];
             const uint32_t ku = ring + ks * G::UB;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.0f;
-                if constexpr (BITS == 16) {
+            if constexpr (BITS == 16) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
                     const uint32_t part = unit_off<16, D, GS, 0>(lane & 15, (lane >> 4) * 16);
 #pragma unroll
                     for (int x = 0; x < QS; ++x) {
@@ -330,14 +333,20 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         for (int n = 0; n < NT; ++n)
                             Act<TA>::mma(s[kt][n], f[0], f[1], f[2], f[3], qf[n][x][0], qf[n][x][1]);
                     }
-                } else {
-                    constexpr int SEG = GS * BITS / 8, WPG = SEG / 16;  // bytes of a group, words of a lane's quarter
-                    constexpr int WV = WPG < 4 ? WPG : 4;               // read at once
-                    using RC = RawCode<TA, BITS>;
-                    const uint32_t part = unit_off<BITS, D, GS, 0>(g, t4 * (SEG / 4));
-                    const uint32_t spart = ku + G::CB + g * NG * 2;
+                }
+            } else {
+                constexpr int SEG = GS * BITS / 8, WPG = SEG / 16;  // bytes of a group, words of a lane's quarter
+                constexpr int WV = WPG < 4 ? WPG : 4;               // read at once
+                using RC = RawCode<TA, BITS>;
+                const uint32_t part = unit_off<BITS, D, GS, 0>(g, t4 * (SEG / 4));
+                const uint32_t spart = ku + G::CB + g * NG * 2;
 #pragma unroll
-                    for (int gi = 0; gi < NG; ++gi) {
+                for (int gi = 0; gi < NG; ++gi) {
+                    float2 qs[NT];  // of the lane's two columns
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) qs[n] = *reinterpret_cast<const float2 *>(&s_qs[warp][gi][n * 8 + 2 * t4]);
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
                         float sf[2], bf[2], acc[NT][4];
                         uint32_t w[2][WPG];
 #pragma unroll
@@ -374,7 +383,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                s[kt][n][e] = fmaf(sf[e >> 1], acc[n][e], fmaf(bf[e >> 1], qs[n][e & 1][gi], s[kt][n][e]));
+                                s[kt][n][e] = fmaf(sf[e >> 1], acc[n][e], fmaf(bf[e >> 1], e & 1 ? qs[n].y : qs[n].x, s[kt][n][e]));
                     }
                 }
             }
