@@ -444,8 +444,8 @@ typedef struct lmoe_kv_cache {
  * All arrays are on the device and are read by the kernels only; entries of
  * page_table behind a sequence's last page are not read.  A sequence's rows
  * with a negative position (lens[b] < n_b) have no place.  Where a page id is
- * outside [0, n_pages), a position needs an entry at or behind table_width,
- * lens[b] is negative or row_start is not a non-decreasing run inside [0,
+ * outside [0, n_pages), a length needs more entries than table_width, lens[b]
+ * is negative or row_start is not a non-decreasing run inside [0,
  * n_rows], the kernels latch LMOE_EINDEX in the workspace's status word and
  * take that part as absent. */
 typedef struct lmoe_kv_rows {
@@ -483,8 +483,11 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
  * zero for a row that sees nothing.  What a row does not see does not touch
  * its result, infinities and NaN included.  Softmax statistics and sums are in
- * fp32; q, the softmax terms and quantised keys and values enter the products
- * in dtype.  scratch: lmoe_paged_attention_scratch() bytes, 16-byte aligned,
+ * fp32; the softmax terms and quantised values enter the products in dtype, and
+ * so do quantised keys where the sequences have more than 16 rows (tokens x
+ * query heads of a key/value head) on average; for fewer the keys' codes are
+ * contracted exactly.  A scale or bias that is not finite makes its key's
+ * score, or its values, no number.  scratch: lmoe_paged_attention_scratch() bytes, 16-byte aligned,
  * with no need of initialisation, in use until the call's kernels end. */
 size_t lmoe_paged_attention_scratch(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, int32_t q_heads);
 int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, int32_t q_heads, const void *q,

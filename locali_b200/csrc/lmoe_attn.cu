@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
             const int k0 = t.block(b0 + warp + i * kRowWarps) * KS;
             const uint32_t bad = __ballot_sync(0xffffffffu, pg_cur == -1);  // runs without a page
             // every row of the tile sees every position of the block
-            const bool full = !bad && k0 + KS - 1 <= t.minpos &&
+            const bool full = !bad && k0 + KS - 1 <= t.minpos && k0 + KS <= t.hi &&
                               (a.window == 0 || k0 > (long long)t.maxpos - a.window || k0 + KS <= a.sinks);
 
             // ---- S^T = K Q^T
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int j = k0 + kt * 16 + g + 8 * (e >> 1), p = pos[n][e & 1];
-                            const bool see = j <= p && !(bad >> kt & 1u) &&
+                            const bool see = j <= p && j < t.hi && !(bad >> kt & 1u) &&
                                              (a.window == 0 || p - j < a.window || j < a.sinks);
                             seen[n][e & 1] |= see;
                             if (!see) s[kt][n][e] = -INFINITY;

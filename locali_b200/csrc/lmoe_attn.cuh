@@ -20,7 +20,7 @@ struct Tile {
     int first;          // position of its token row 0 (may be negative)
     int rows;           // rows of the tile, 1..R
     int minpos, maxpos; // positions of the tile's first and last row
-    int hi;             // keys [0, hi) are looked at
+    int hi;             // keys [0, hi) are looked at: those the table has room for
     int nsink, lo;      // sink blocks, first block of the rest
     int nblk;           // blocks; at least 1, so a tile that sees nothing is written
     __device__ __forceinline__ int block(int i) const { return i < nsink ? i : lo + i - nsink; }
@@ -32,12 +32,12 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     t.rows = min(R, t.n * a.group - r0);
     t.minpos = t.first + a.per_group(r0);
     t.maxpos = t.first + a.per_group(r0 + t.rows - 1);
-    t.hi = max(0, t.maxpos + 1);
+    t.hi = min(max(0, t.maxpos + 1), a.r.max_pos);
     int low = 0;
     if (a.window > 0) low = (int)max(0ll, (long long)t.minpos - a.window + 1);
     t.lo = low / KS;
     t.nsink = t.lo > 0 ? min((min(a.sinks, t.hi) + KS - 1) / KS, t.lo) : 0;
-    t.nblk = max(1, t.nsink + (t.hi + KS - 1) / KS - t.lo);
+    t.nblk = max(1, t.nsink + max(0, (t.hi + KS - 1) / KS - t.lo));
 }
 
 // Sequence b's rows into t; returns its tiles (of one head).

@@ -550,13 +550,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const int row = ti.rt * kCkRows + t * kCkSub + r;
                 const bool in = row < ti.n * a.group;
                 const int p = in ? ti.first + a.per_group(row) : -1;
-                const int see_hi = p + 1, see_lo = a.window ? (int)max(0ll, (long long)p - a.window + 1) : 0;
+                const int see_hi = min(p + 1, ti.hi), see_lo = a.window ? (int)max(0ll, (long long)p - a.window + 1) : 0;
                 const int see_sink = min(a.sinks, see_hi);
                 // positions of the sub-tile's first and last row
                 const int lastrow = min(ti.rows, (t + 1) * kCkSub) - 1;
                 const int nsink = ti.nsink, lo = ti.lo - nsink;
-                const int tmin = ti.minpos, tmax = ti.maxpos;
-                const int smin = ti.first + a.per_group(ti.rt * kCkRows + t * kCkSub);
+                const int tmin = min(ti.minpos, ti.hi - 1), tmax = ti.maxpos;
+                const int smin = min(ti.first + a.per_group(ti.rt * kCkRows + t * kCkSub), ti.hi - 1);
                 const int smax = ti.first + a.per_group(ti.rt * kCkRows + lastrow);
                 float m = -INFINITY;
                 float l = 0.0f;
@@ -1068,7 +1068,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 e.left = ti.hi - blk * kCkKeys;
                 e.blk = blk;
                 e.seg = n;
-                e.part = block_full(a, blk * kCkKeys, ti.minpos, ti.maxpos) ? -1 : parts++;
+                e.part = block_full(a, blk * kCkKeys, min(ti.minpos, ti.hi - 1), ti.maxpos) ? -1 : parts++;
             }
         }
         if (ok && asked) ok = give();

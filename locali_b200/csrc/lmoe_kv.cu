@@ -449,7 +449,7 @@ int check_cache(const lmoe_kv_cache *c, KvView *v) {
 }
 
 // LMOE_OK with out->n_rows = 0: nothing to do
-int check_rows(const lmoe_kv_rows *r, void *workspace, KvRows *out) {
+int check_rows(const lmoe_kv_rows *r, int page_size, void *workspace, KvRows *out) {
     if (!r || r->n_seqs < 0 || r->n_rows < 0 || r->table_width < 0 || r->table_stride < r->table_width)
         return LMOE_EINVAL;
     std::memset(out, 0, sizeof(*out));
@@ -463,6 +463,8 @@ int check_rows(const lmoe_kv_rows *r, void *workspace, KvRows *out) {
     out->lens = r->lens;
     out->row_start = r->row_start;
     out->n_rows = r->n_rows;
+    const int64_t room = (int64_t)r->table_width * page_size;
+    out->max_pos = room < 0x7FFFFFFF ? (int32_t)room : 0x7FFFFFFF;
     out->err = static_cast<int32_t *>(workspace);
     return LMOE_OK;
 }
@@ -485,7 +487,7 @@ int lmoe_kv_append(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, const v
     KvCopyArgs a;
     std::memset(&a, 0, sizeof(a));
     int rc = check_cache(cache, &a.c);
-    if (!rc) rc = check_rows(rows, workspace, &a.r);
+    if (!rc) rc = check_rows(rows, cache->page_size, workspace, &a.r);
     if (rc || a.r.n_rows == 0) return rc;
     if (!strided_ok(k, k_token_stride, k_head_stride) || !strided_ok(v, v_token_stride, v_head_stride))
         return LMOE_EINVAL;
@@ -505,7 +507,7 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
     KvCopyArgs a;
     std::memset(&a, 0, sizeof(a));
     int rc = check_cache(cache, &a.c);
-    if (!rc) rc = check_rows(rows, workspace, &a.r);
+    if (!rc) rc = check_rows(rows, cache->page_size, workspace, &a.r);
     if (rc || a.r.n_rows == 0) return rc;
     if (!k || !v || !al16(k) || !al16(v)) return LMOE_EINVAL;
     a.dst[0] = static_cast<uint16_t *>(k);
@@ -535,7 +537,7 @@ int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, i
     if (rc) return rc;
     if (q_heads < 1 || q_heads % cache->kv_heads != 0 || sinks < 0) return LMOE_EINVAL;
     if (!(scale >= 0.0f) || scale > 1e30f) return LMOE_EINVAL;
-    rc = check_rows(rows, workspace, &a.r);
+    rc = check_rows(rows, cache->page_size, workspace, &a.r);
     if (rc || a.r.n_rows == 0) return rc;
     if (!strided_ok(q, q_token_stride, q_head_stride) || !out || !al16(out) || !al16(scratch)) return LMOE_EINVAL;
     // row numbers of the tiles (rows x heads of a group) are 32-bit

@@ -40,6 +40,7 @@ struct KvRows {
     const int32_t *lens;
     const int32_t *row_start;  // nullptr: row b is sequence b's
     int32_t n_rows;
+    int32_t max_pos;  // positions a table has room for
     int32_t *err;
     // first row of sequence b, held inside [0, n_rows]
     __device__ __forceinline__ int start(int b) const {
@@ -49,7 +50,7 @@ struct KvRows {
     // out of range (one block of a launch does).
     __device__ __forceinline__ void validate(int i, int n) const {
         for (int b = i; b < n_seqs; b += n) {
-            bool bad = lens[b] < 0;
+            bool bad = lens[b] < 0 || lens[b] > max_pos;
             if (row_start) bad |= row_start[b] < 0 || row_start[b + 1] < row_start[b] || row_start[b + 1] > n_rows;
             if (bad) set_error(err, kErrIndex);
         }

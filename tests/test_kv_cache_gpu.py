@@ -455,6 +455,34 @@ def test_bad_pages_are_reported(built, rows):
         assert (k == 0).all()
 
 
+@pytest.mark.parametrize("rows", [1, 4, 60])
+def test_lengths_past_the_table_are_reported(built, rows):
+    """A length the table has no room for, up to the largest: the positions behind the table are absent (and not
+    walked), the others are seen."""
+    case = Case([128, 90 + rows], [rows, rows], bits=8, gs=32, d=64, hk=1, page=16, width=12)
+    c, q = case.cache, case.q(2)
+    for length in (200, 128 + 10**6, 2**31 - 1):
+        lens = torch.tensor([length, 90 + rows], dtype=torch.int32, device="cuda")
+        tab = case.table[:, :8].contiguous()  # room for 128 positions
+        got = c.attend(q, tab, lens, case.start)
+        with pytest.raises(_lib.LmoeError):
+            c.check()
+        kn, vn, qn = case.held("k"), case.held("v"), np64(q)
+        for h in range(2):
+            pos = np.arange(length - rows, length)
+            see = K.visible(np.minimum(pos, 10**6), 128, 0, 0)
+            o, A, B, N = K.attention(qn[:rows, h], case.seq(kn, 0, 0), case.seq(vn, 0, 0), see, 0.125)
+            assert (np.abs(np64(got)[:rows, h] - o) <= K.tolerance(o, A, B, N, "bf16", True, 128)).all()
+        # a window that lies wholly behind the table sees nothing
+        if length > 10**5:
+            assert (c.attend(q, tab, lens, case.start, window=50)[:rows] == 0).all()
+            with pytest.raises(_lib.LmoeError):
+                c.check()
+        k, v = c.read(tab, lens, case.start, rows=case.n)
+        with pytest.raises(_lib.LmoeError):
+            c.check()
+
+
 def test_bad_row_starts_are_reported(built):
     case = Case([50, 60], [5, 6], bits=16, d=64, hk=1)
     c = case.cache
