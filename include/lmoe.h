@@ -485,7 +485,8 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
  * its result, infinities and NaN included.  Softmax statistics and sums are in
  * fp32; the softmax terms and quantised values enter the products in dtype, and
  * so do quantised keys where the sequences have more than 16 rows (tokens x
- * query heads of a key/value head) on average; for fewer the keys' codes are
+ * query heads of a key/value head) on average (as two numbers, their sum exact
+ * to 16 bits, for bf16 and heads of 64); for fewer the keys' codes are
  * contracted exactly.  A scale or bias that is not finite makes its key's
  * score, or its values, no number.  scratch: lmoe_paged_attention_scratch() bytes, 16-byte aligned,
  * with no need of initialisation, in use until the call's kernels end. */

@@ -64,11 +64,17 @@ constexpr int kStgRow = 80, kStgWarp = 32 * kStgRow;
 constexpr int kExpFma = 2;  // of 8 pairs of exponentials, on the FMA pipe
 constexpr int kPoison = 12;      // key blocks of a tile that some of its rows see in part: at most 8
 
-template <int BITS, int D, int GS>
+// Keys of 64 elements dequantised to bf16 bring a second operand tile with
+// what the rounding took off: rounded, they were most of a result's error (4.9e-3
+// of its norm; the result's own rounding is 1.7e-3), and at 64 the tensor pipe
+// and shared memory have room for it.  (At 128 they have not; f16 has three more
+// bits.)
+template <typename TA, int BITS, int D, int GS>
 struct ChunkGeo {
+    static constexpr bool LO = BITS != 16 && D == 64 && std::is_same<TA, __nv_bfloat16>::value;
     static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
-    static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_X = 6 * TILE;
+    static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_L = 6 * TILE, OFF_X = (LO ? 8 : 6) * TILE;
     static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * (int)sizeof(uint2);  // scales and biases of the loader warps' rows
     static constexpr int OFF_STG = OFF_X + SCALES;                   // output staging of the softmax warps
     static constexpr int SMEM = 1024 + OFF_STG + 8 * kStgWarp;
@@ -418,9 +424,28 @@ __device__ __forceinline__ float row_terms(uint32_t ts, F &&mask, float sc, floa
     return s0 + s1;
 }
 
+// What rounding scale * code + bias to the 8 bf16 values v took off them
+// (s2 as dequant8 takes it).
+template <int BITS>
+__device__ __forceinline__ uint4 dequant8_rest(uint32_t w0, uint32_t w1, uint32_t s2, uint32_t b2, const uint4 &v) {
+    const float s = __uint_as_float(s2 << 16) * (BITS == 8 ? 1.0f / 64.0f : 1.0f), b = __uint_as_float(b2 << 16);
+    const uint32_t hi[4] = {v.x, v.y, v.z, v.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = BITS == 8 ? (i < 2 ? w0 : w1) >> (16 * (i & 1)) : w0 >> (8 * i);
+        const uint32_t c0 = w & (BITS == 8 ? 255u : 15u), c1 = w >> BITS & (BITS == 8 ? 255u : 15u);
+        // 2^23 + code as a number
+        const float f0 = __uint_as_float(0x4B000000u | c0) - 8388608.0f, f1 = __uint_as_float(0x4B000000u | c1) - 8388608.0f;
+        r[i] = Act<__nv_bfloat16>::pack2(fmaf(s, f0, b) - __uint_as_float(hi[i] << 16),
+                                         fmaf(s, f1, b) - __uint_as_float(hi[i] & 0xFFFF0000u));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 template <typename TA, int BITS, int D, int GS>
 __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArgs a) {
-    using G = ChunkGeo<BITS, D, GS>;
+    using G = ChunkGeo<TA, BITS, D, GS>;
     constexpr int CH = D / 8;   // 16-byte chunks of an operand row
     constexpr int RB = D * BITS / 8;
     constexpr bool Q = BITS != 16;
@@ -848,6 +873,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         sts128v(dst + op_off(lw * 32 + (x0 + x) * RPI + rr, cc), v[x].x, v[x].y, v[x].z, v[x].w);
+                    if (G::LO && !which) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint4 y = dequant8_rest<BITS>(code[x0 + x][0], code[x0 + x][WPC - 1], sv[x].x, sv[x].y, v[x]);
+                            sts128v(dst - G::OFF_K + G::OFF_L + op_off(lw * 32 + (x0 + x) * RPI + rr, cc), y.x, y.y, y.z, y.w);
+                        }
+                    }
                 }
                 done(n, u, taken);
             };
@@ -951,6 +983,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 for (int s = 0; s < D / 16; ++s) {
                     const uint64_t o = (uint64_t)((s >> 2) * (16384 >> 4) + (s & 3) * 2);
                     umma_f16(ds, qd + o, kd + o, id_s, s ? 1u : 0u);
+                }
+                if constexpr (G::LO) {
+                    const uint64_t ld = sw128_desc(sbu + G::OFF_L + (u & 1) * G::TILE);
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s) umma_f16(ds, qd + s * 2, ld + s * 2, id_s, 1u);
                 }
             }
             __syncwarp();
@@ -1102,7 +1139,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
 
 template <typename TA, int BITS, int D, int GS>
 cudaError_t launch_chunk_t(const AttnArgs &a, cudaStream_t st) {
-    using G = ChunkGeo<BITS, D, GS>;
+    using G = ChunkGeo<TA, BITS, D, GS>;
     auto kern = attn_chunk_kernel<TA, BITS, D, GS>;
     static bool configured[64];
     int dev = 0;
