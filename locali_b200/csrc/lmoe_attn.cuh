@@ -21,7 +21,7 @@ struct Tile {
     int rows;           // rows of the tile, 1..R
     int minpos, maxpos; // positions of the tile's first and last row
     int hi;             // keys [0, hi) are looked at: those the table has room for
-    int nsink, lo;      // sink blocks, first block of the rest
+    int nsink, lo;      // sink blocks, first block of the rest (held at the first one behind hi)
     int nblk;           // blocks; at least 1, so a tile that sees nothing is written
     __device__ __forceinline__ int block(int i) const { return i < nsink ? i : lo + i - nsink; }
 };
@@ -35,7 +35,10 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     t.hi = min(max(0, t.maxpos + 1), a.r.max_pos);
     int low = 0;
     if (a.window > 0) low = (int)max(0ll, (long long)t.minpos - a.window + 1);
-    t.lo = low / KS;
+    // Held at the first block behind hi: the window of a length far past its
+    // table may begin in the last block that 32 bits can count, whose end they
+    // cannot.
+    t.lo = min(low / KS, (t.hi + KS - 1) / KS);
     t.nsink = t.lo > 0 ? min((min(a.sinks, t.hi) + KS - 1) / KS, t.lo) : 0;
     t.nblk = max(1, t.nsink + max(0, (t.hi + KS - 1) / KS - t.lo));
 }

@@ -208,7 +208,7 @@ __device__ __forceinline__ void place_rows(const KvCopyArgs &a, int r0, RowPlace
                     while (b < a.r.n_seqs && a.r.start(b + 1) <= r) ++b;
                 mine = b < a.r.n_seqs;  // a row of a sequence, with or without a place
                 if (mine) {
-                    const int pos = a.r.lens[b] - (a.r.start(b + 1) - r);
+                    const int pos = max(a.r.lens[b], 0) - (a.r.start(b + 1) - r);
                     if (pos >= 0) {
                         p.page = a.r.page(a.c, b, pos);
                         p.slot = a.c.slot_of(pos);
@@ -466,7 +466,7 @@ int check_rows(const lmoe_kv_rows *r, int page_size, void *workspace, KvRows *ou
     out->row_start = r->row_start;
     out->n_rows = r->n_rows;
     const int64_t room = (int64_t)r->table_width * page_size;
-    out->max_pos = room < 0x7FFFFFFF ? (int32_t)room : 0x7FFFFFFF;
+    out->max_pos = room < kMaxPos ? (int32_t)room : kMaxPos;
     out->err = static_cast<int32_t *>(workspace);
     return LMOE_OK;
 }

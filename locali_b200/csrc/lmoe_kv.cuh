@@ -32,6 +32,10 @@ struct KvView {
     }
 };
 
+// Positions of a sequence, at most: the end of the key block behind them still
+// fits 32 bits (blocks are 128 positions at most).
+constexpr int32_t kMaxPos = 0x7FFFFFFF - 255;
+
 struct KvRows {
     const int32_t *table;
     int64_t table_stride;
@@ -40,7 +44,7 @@ struct KvRows {
     const int32_t *lens;
     const int32_t *row_start;  // nullptr: row b is sequence b's
     int32_t n_rows;
-    int32_t max_pos;  // positions a table has room for
+    int32_t max_pos;  // positions a table has room for, kMaxPos at most
     int32_t *err;
     // first row of sequence b, held inside [0, n_rows]
     __device__ __forceinline__ int start(int b) const {
@@ -59,7 +63,7 @@ struct KvRows {
     __device__ __forceinline__ int32_t page(const KvView &c, int b, int p) const {
         const int e = c.page_of(p);
         int32_t pg = -1;
-        if (e < table_width) pg = table[(int64_t)b * table_stride + e];
+        if (p < max_pos) pg = table[(int64_t)b * table_stride + e];
         if (pg < 0 || pg >= c.n_pages) {
             set_error(err, kErrIndex);
             pg = -1;

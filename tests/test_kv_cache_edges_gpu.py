@@ -1,0 +1,85 @@
+"""The paged key/value cache at its edges: lengths and offsets at the ends of
+32 bits, sequences across the look-up's blocks, pages that a window has left
+behind, extreme values, and how near to 64 bits each path comes."""
+
+import numpy as np
+import pytest
+import torch
+
+from locali_b200 import _lib
+from locali_b200.kv_cache import PagedKVCache
+from oracle import kv_oracle as K
+from tests.test_kv_cache_gpu import T, Case, attend_and_check, np64
+
+pytestmark = pytest.mark.gpu
+
+I32 = dict(dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ lengths
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 60])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (50, 0), (50, 3), (70, 200)])
+def test_windows_of_lengths_far_past_the_table(built, bits, rows, window, sinks):
+    """The window of the largest length lies in the last key block that 32 bits can count: nothing of it is there,
+    only the first tokens are seen."""
+    case = Case([128, 90 + rows], [rows, rows], bits=bits, gs=32, d=64, hk=1, page=16, width=8 + (90 + rows) // 16)
+    c, q = case.cache, case.q(2)
+    tab = case.table[:, :8].contiguous()  # room for 128 positions
+    kn, vn, qn = case.held("k"), case.held("v"), np64(q)
+    for length in (2**31 - 1, 2**31 - 40, 2**31 - 128, 2**31 - 256, 2**31 - 300):
+        got = c.attend(q, tab, torch.tensor([length, rows], **I32), case.start, window=window, sinks=sinks)
+        with pytest.raises(_lib.LmoeError):
+            c.check()
+        see = np.zeros((rows, 128), bool)
+        see[:, :sinks] = True
+        for h in range(2):
+            o, A, B, N = K.attention(qn[:rows, h], case.seq(kn, 0, 0), case.seq(vn, 0, 0), see, 0.125)
+            assert (np.abs(np64(got)[:rows, h] - o) <= K.tolerance(o, A, B, N, "bf16", bits < 16, 128)).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 60])
+def test_positions_up_to_the_largest(built, rows):
+    """A table that names the same page over and over and has room for every position: windowed attention, append and
+    read at the last positions there are; a length behind them is reported."""
+    page, d = 1 << 20, 64
+    c = PagedKVCache(2, page, 1, d, bits=4, group_size=64)
+    tab = torch.zeros(1, 2048, **I32)
+    tab[0, -1] = 1  # the last page alone is its own
+    start = torch.tensor([0, rows], **I32)
+    last = 2**31 - 256
+    g = torch.Generator("cuda").manual_seed(0)
+    fill = 300
+    x, y = (torch.randn(fill, 1, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    c.append(x, y, tab, torch.tensor([last], **I32), torch.tensor([0, fill], **I32))
+    c.check()
+    lens = torch.tensor([last], **I32)
+    k, v = c.read(tab, lens, torch.tensor([0, fill], **I32), rows=fill)
+    c.check()
+    for t, z in ((x, k), (y, v)):
+        codes, s, b = K.quantise(np64(t), 4, 64, "bf16")
+        assert np.array_equal(np64(z), K.round_to(K.dequantise(codes, s, b, 64), "bf16"))
+    q = torch.randn(rows, 2, d, generator=g, device="cuda").to(torch.bfloat16)
+    kn, vn = (np64(t).reshape(fill, d) for t in (k, v))
+    for W in (1, 50, 200):
+        got = c.attend(q, tab, lens, start, window=W)
+        c.check()
+        see = K.visible(np.arange(fill - rows, fill), fill, W, 0)
+        for h in range(2):
+            o, A, B, N = K.attention(np64(q)[:, h], kn, vn, see, 0.125)
+            # kn, vn are rounded already: once more the same rounding
+            assert (np.abs(np64(got)[:, h] - o) <= 2 * K.tolerance(o, A, B, N, "bf16", True, fill)).all()
+    before = c.k.clone()
+    for length in (last + 1, 2**31 - 1):
+        over = torch.tensor([length], **I32)
+        assert torch.isfinite(c.attend(q, tab, over, start, window=3)).all()
+        with pytest.raises(_lib.LmoeError):
+            c.check()
+        c.append(x[:1], y[:1], tab, over)
+        with pytest.raises(_lib.LmoeError):
+            c.check()
+    neg = torch.tensor([-2**31], **I32)
+    c.append(x[:1], y[:1], tab, neg)
+    with pytest.raises(_lib.LmoeError):
+        c.check()
+    assert torch.equal(before, c.k)
