@@ -440,7 +440,8 @@ typedef struct lmoe_kv_cache {
  * its n_b rows has position lens[b] - n_b + i.  row_start NULL: one row for
  * each sequence (n_rows == n_seqs).  Position p of sequence b lives in slot
  * p % page_size of page page_table[b * table_stride + p / page_size].  Rows
- * at and behind row_start[n_seqs] belong to no sequence and are left alone.
+ * in front of row_start[0] and from row_start[n_seqs] on belong to no sequence
+ * and are left alone.
  * All arrays are on the device and are read by the kernels only; entries of
  * page_table behind a sequence's last page are not read.  A sequence's rows
  * with a negative position (lens[b] < n_b) have no place.  Where a page id is

@@ -198,15 +198,15 @@ __device__ __forceinline__ void place_rows(const KvCopyArgs &a, int r0, RowPlace
             int n = 0;  // row starts at or in front of r0
             for (int b0 = 0; b0 <= a.r.n_seqs; b0 += 32)
                 n += __popc(__ballot_sync(0xffffffffu, b0 + lane <= a.r.n_seqs && a.r.start(b0 + lane) <= r0));
-            b = n - 1;
+            b = max(n - 1, 0);  // none: the first sequence may begin inside the block
         }
         if (lane < a.rows_per_block) {
             RowPlace p{-1, 0};
             bool mine = false;
-            if (r < a.r.n_rows && b >= 0) {
+            if (r < a.r.n_rows) {
                 if (a.r.row_start)
                     while (b < a.r.n_seqs && a.r.start(b + 1) <= r) ++b;
-                mine = b < a.r.n_seqs;  // a row of a sequence, with or without a place
+                mine = b < a.r.n_seqs && r >= a.r.start(b);  // a row of a sequence, with or without a place
                 if (mine) {
                     const int pos = max(a.r.lens[b], 0) - (a.r.start(b + 1) - r);
                     if (pos >= 0) {

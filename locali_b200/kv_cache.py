@@ -61,8 +61,9 @@ class PagedKVCache:
     sequences' lengths with the rows of the call, and ``row_start`` int32
     [n_seqs + 1]: rows ``row_start[b]`` to ``row_start[b + 1] - 1`` are
     sequence b's last positions.  Without ``row_start`` each sequence has one
-    row.  Rows from ``row_start[n_seqs]`` on (padding of a captured batch)
-    belong to no sequence: they are read by nothing and left as they were.
+    row.  Rows in front of ``row_start[0]`` and from ``row_start[n_seqs]`` on
+    (padding of a captured batch) belong to no sequence: they are left as they
+    were.
     The three arrays are device arrays, so a captured call replays with the
     values they hold then.
     """

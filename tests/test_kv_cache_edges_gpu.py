@@ -83,3 +83,50 @@ def test_positions_up_to_the_largest(built, rows):
     with pytest.raises(_lib.LmoeError):
         c.check()
     assert torch.equal(before, c.k)
+
+
+# ------------------------------------------------------------------ rows of many sequences
+@pytest.mark.parametrize("first", [0, 3, 11])
+@pytest.mark.parametrize("bits,dtype", [(16, "bf16"), (8, "bf16"), (4, "f16")])
+def test_many_rows_across_sequences(built, first, bits, dtype):
+    """More rows than get a launch block each, of sequences whose borders lie anywhere, some without rows and some
+    shorter than theirs, rows in front of the first sequence and behind the last: every row in its place, the others
+    as they were."""
+    rng = np.random.default_rng(7)
+    B, page, hk, d, gs = 140, 16, 2, 64, 32
+    rows = rng.choice([0, 0, 1, 3, 17, 40], B)
+    lens = np.where(rng.random(B) < 0.1, rows // 2, rows + rng.integers(0, 50, B))
+    start = first + np.concatenate([[0], np.cumsum(rows)])
+    n = int(start[-1]) + 13
+    assert n > 1024
+    need = -(-lens // page)
+    tab = np.full((B, max(need)), -7, np.int32)
+    perm, at = rng.permutation(int(need.sum()) + 2), 0
+    for b in range(B):
+        tab[b, :need[b]] = perm[at:at + need[b]]
+        at += need[b]
+    c = PagedKVCache(len(perm), page, hk, d, bits=bits, group_size=gs, dtype=T[dtype])
+    g = torch.Generator("cuda").manual_seed(0)
+    x, y = (torch.randn(n, hk, d, generator=g, device="cuda").to(T[dtype]) for _ in range(2))
+    args = [torch.from_numpy(np.ascontiguousarray(a)).to(**I32) for a in (tab, lens, start)]
+    c.append(x, y, *args)
+    out = tuple(torch.full((n, hk, d), 7.0, dtype=T[dtype], device="cuda") for _ in range(2))
+    c.read(*args, out=out)
+    c.check()
+    for t, got, held in ((x, out[0], c.k), (y, out[1], c.v)):
+        want = np64(t)
+        words = want
+        if bits < 16:
+            codes, s, b = K.quantise(want, bits, gs, dtype)
+            want, words = K.round_to(K.dequantise(codes, s, b, gs), dtype), K.pack(codes, bits)
+        cells = np.zeros((len(perm), page, hk, words.shape[-1]))
+        expect = np.full((n, hk, d), 7.0)
+        for b in range(B):
+            for r in range(start[b], start[b + 1]):
+                p = lens[b] - (start[b + 1] - r)
+                expect[r] = want[r] if p >= 0 else 0.0
+                if p >= 0:
+                    cells[tab[b, p // page], p % page] = words[r]
+        assert np.array_equal(np64(got), expect)
+        held = np64(held) if bits == 16 else held.cpu().numpy().view(np.uint32)
+        assert np.array_equal(held.transpose(0, 2, 1, 3), cells)
