@@ -443,11 +443,13 @@ typedef struct lmoe_kv_cache {
  * in front of row_start[0] and from row_start[n_seqs] on belong to no sequence
  * and are left alone.
  * All arrays are on the device and are read by the kernels only; entries of
- * page_table behind a sequence's last page are not read.  A sequence's rows
- * with a negative position (lens[b] < n_b) have no place.  Where a page id is
- * outside [0, n_pages), a length needs more entries than table_width or
- * passes 2^31 - 256, lens[b] is negative or row_start is not a non-decreasing
- * run inside [0, n_rows], the kernels latch LMOE_EINDEX in the workspace's status word and
+ * page_table behind a sequence's last page, and (attention with a window)
+ * those of pages that none of the sequence's rows sees a position of, are not
+ * looked at and may hold anything.  A sequence's rows with a negative position
+ * (lens[b] < n_b) have no place.  Where another page id is outside [0,
+ * n_pages), a length needs more entries than table_width or passes 2^31 - 256,
+ * lens[b] is negative or row_start is not a non-decreasing run inside [0,
+ * n_rows], the kernels latch LMOE_EINDEX in the workspace's status word and
  * take that part as absent. */
 typedef struct lmoe_kv_rows {
     const int32_t *page_table;

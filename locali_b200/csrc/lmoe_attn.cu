@@ -241,12 +241,13 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
         // ---- this warp's blocks of [b0, b1), as units K, V, K, V, ...
         const int nb = b0 + warp < b1 ? (b1 - b0 - warp + kRowWarps - 1) / kRowWarps : 0;
         // Head row (of all pages') where 16-position run `lane` of block i of
-        // the warp's begins; -2: no such positions, -1: no page.
+        // the warp's begins; -2: no such positions, or none
+        // that a row sees; -1: no page.
         auto runs_of = [&](int i) -> long long {
             long long r = -2;
             if (lane < KT && i < nb) {
                 const int p = t.block(b0 + warp + i * kRowWarps) * KS + lane * 16;
-                if (p < t.hi) {
+                if (p < t.hi && run_seen(a, t, p)) {
                     const int32_t pg = a.r.page(a.c, t.b, p);
                     r = pg < 0 ? -1 : a.c.row(pg, t.h, a.c.slot_of(p));
                 }
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const uint32_t u = ring + slot * G::UB;
                 const int r0 = lane / (RB / 16), c0 = lane % (RB / 16);
                 const uint32_t part = unit_off<BITS, D, GS, W>(r0, c0 * 16);
-                const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, runs == -1);
+                const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, lane < KT && runs < 0);
                 const uint8_t *const kv = a.c.kv[W] + lane * 16;
                 if (all) {
 #pragma unroll

@@ -21,6 +21,7 @@ struct Tile {
     int rows;           // rows of the tile, 1..R
     int minpos, maxpos; // positions of the tile's first and last row
     int hi;             // keys [0, hi) are looked at: those the table has room for
+    int low;            // no row sees keys in front of this, but for the first tokens that stay visible
     int nsink, lo;      // sink blocks, first block of the rest (held at the first one behind hi)
     int nblk;           // blocks; at least 1, so a tile that sees nothing is written
     __device__ __forceinline__ int block(int i) const { return i < nsink ? i : lo + i - nsink; }
@@ -38,9 +39,17 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     // Held at the first block behind hi: the window of a length far past its
     // table may begin in the last block that 32 bits can count, whose end they
     // cannot.
+    t.low = low;
     t.lo = min(low / KS, (t.hi + KS - 1) / KS);
     t.nsink = t.lo > 0 ? min((min(a.sinks, t.hi) + KS - 1) / KS, t.lo) : 0;
     t.nblk = max(1, t.nsink + max(0, (t.hi + KS - 1) / KS - t.lo));
+}
+
+// Does a row of the tile see one of the 16 positions from p < hi?  Blocks
+// reach past the first tokens and the window's lower edge, and what lies
+// between those may have no page any more.
+__device__ __forceinline__ bool run_seen(const AttnArgs &a, const Tile &t, int p) {
+    return p < a.sinks || p + 16 > t.low;
 }
 
 // Sequence b's rows into t; returns its tiles (of one head).

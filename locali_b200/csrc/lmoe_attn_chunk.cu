@@ -89,7 +89,7 @@ struct Seg {
 };
 
 // A key block as the loaders need it: the head row where each 16-position run
-// begins (-2: none, -1: no page).
+// begins (-2: none, or none that a row sees, -1: no page).
 struct Look {
     long long run[kCkKeys / 16];
     int left;  // positions in front of the end
@@ -1098,7 +1098,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const int blk = ti.block(i), p = blk * kCkKeys + lane * 16;
                 int32_t pg = -1;
                 int sl = -1;
-                if (lane < kCkKeys / 16 && p < ti.hi) {
+                if (lane < kCkKeys / 16 && p < ti.hi && run_seen(a, ti, p)) {
                     const int en = a.c.page_of(p);
                     sl = p - en * a.c.page_size;
                     if (en < a.r.table_width) pg = a.r.table[(int64_t)ti.b * a.r.table_stride + en];

@@ -251,7 +251,8 @@ class PagedKVCache:
         to and with each row's own position (append the rows first).  heads is
         a multiple of kv_heads; ``scale`` is head_dim ** -0.5 by default.  With
         ``window`` > 0 a row sees its own and the ``window - 1`` positions
-        before it, and the sequence's first ``sinks`` positions.  A row that
+        before it, and the sequence's first ``sinks`` positions; table entries
+        of pages that no row sees a position of may hold anything.  A row that
         sees nothing is zero.  ``out`` must not share memory with q."""
         _need_cuda(q)
         q = self._heads(q, "q", None)

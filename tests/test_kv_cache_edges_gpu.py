@@ -130,3 +130,34 @@ def test_many_rows_across_sequences(built, first, bits, dtype):
         assert np.array_equal(np64(got), expect)
         held = np64(held) if bits == 16 else held.cpu().numpy().view(np.uint32)
         assert np.array_equal(held.transpose(0, 2, 1, 3), cells)
+
+
+# ------------------------------------------------------------------ pages that a window has left behind
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("page", [16, 48])
+@pytest.mark.parametrize("rows", [1, 7, 150])
+@pytest.mark.parametrize("window,sinks", [(40, 4), (100, 0), (129, 20)])
+def test_pages_no_row_sees_may_be_gone(built, bits, page, rows, window, sinks):
+    """Pages between the first tokens and the window of a sequence's first row are looked up by nothing: a table that
+    has them at -1 gives the same bits, and nothing is reported."""
+    lens = [rows + 600, rows + 333, rows]
+    case = Case(lens, [rows] * 3, bits=bits, gs=32, d=64, hk=2, page=page)
+    c, q = case.cache, case.q(4)
+    want = c.attend(q, case.table, case.lens, case.start, window=window, sinks=sinks)
+    tab, gone = case.table.clone(), 0
+    for b, L in enumerate(lens):
+        for e in range(-(-L // page)):
+            if e * page >= sinks and (e + 1) * page <= L - rows - window + 1:
+                tab[b, e] = -1
+                gone += 1
+    assert gone > 10
+    c.check()
+    got = c.attend(q, tab, case.lens, case.start, window=window, sinks=sinks)
+    c.check()
+    assert torch.equal(got, want)
+    attend_and_check(case, 4, window=window, sinks=sinks, q=q, got=got)
+    # one page further is seen
+    tab[0, (lens[0] - rows - window + 1) // page] = -1
+    c.attend(q, tab, case.lens, case.start, window=window, sinks=sinks)
+    with pytest.raises(_lib.LmoeError):
+        c.check()
