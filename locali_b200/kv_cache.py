@@ -188,6 +188,7 @@ class PagedKVCache:
             x = x.contiguous()
             if x.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
                 x = x.clone()
+            x = x.view(-1).view(x.shape)  # a dimension of size one may have kept any stride
         return x
 
     def _out(self, out: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:

@@ -161,3 +161,27 @@ def test_pages_no_row_sees_may_be_gone(built, bits, page, rows, window, sinks):
     c.attend(q, tab, case.lens, case.start, window=window, sinks=sinks)
     with pytest.raises(_lib.LmoeError):
         c.check()
+
+
+# ------------------------------------------------------------------ strides and arguments
+def test_strides_of_dimensions_of_one(built):
+    """A dimension of size one may have any stride: nothing is ever one step along it."""
+    i32 = I32
+    c = PagedKVCache(2, 16, 4, 64)
+    base = torch.randn(5, 257, device="cuda").to(torch.bfloat16)
+    one = torch.as_strided(base, (1, 4, 64), (257, 64, 1))  # a token stride of 257
+    assert one.is_contiguous()
+    tab, lens = torch.tensor([[1]], **i32), torch.tensor([3], **i32)
+    c.append(one, one, tab, lens)
+    k, v = c.read(tab, lens)
+    assert torch.equal(k, one) and torch.equal(v, one)
+    assert torch.equal(c.attend(one, tab, lens), c.attend(one.clone(memory_format=torch.contiguous_format), tab, lens))
+    c1 = PagedKVCache(2, 16, 1, 64)
+    x = torch.as_strided(base.view(-1), (2, 1, 64), (64, 37, 1))  # a head stride of 37
+    tab, lens = torch.tensor([[1], [0]], **i32), torch.tensor([3, 9], **i32)
+    c1.append(x, x, tab, lens)
+    k, v = c1.read(tab, lens)
+    assert torch.equal(k, x) and torch.equal(v, x)
+    want = c1.attend(base.view(-1)[:128].view(2, 1, 64), tab, lens)
+    assert torch.equal(c1.attend(x, tab, lens), want)
+    c1.check()
