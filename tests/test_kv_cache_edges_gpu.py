@@ -185,3 +185,13 @@ def test_strides_of_dimensions_of_one(built):
     want = c1.attend(base.view(-1)[:128].view(2, 1, 64), tab, lens)
     assert torch.equal(c1.attend(x, tab, lens), want)
     c1.check()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_windows_of_zero_and_less_are_none(built, rows):
+    case = Case([90 + rows], [rows], d=64, hk=1)
+    q = case.q(2)
+    want = case.cache.attend(q, case.table, case.lens, case.start)
+    for window in (0, -1, -2**31, -2**32 + 5, -2**40):
+        got = case.cache.attend(q, case.table, case.lens, case.start, window=window, sinks=1)
+        assert torch.equal(got, want), window
