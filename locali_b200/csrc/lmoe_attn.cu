@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
     const bool work = find_share<R, KS, kRowTile, kRowThreads, false>(a, kRowTile + kRowWarps, s_plan, sh, cur);
     if (tid == 0) rec->parts = 0;
     if (!work) return;
-    const float sc = a.scale_log2;
+    const float sc = a.scale_log2 / RawCode<TA, BITS>::kDown;
 
     for (;;) {
         const Tile &t = cur.t;
@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2 + gi * 2;
                             const float sv = Act<TA>::to_f((uint16_t)lds_u16(so)), bv = Act<TA>::to_f((uint16_t)lds_u16(so + G::SB));
                             // a scale or bias that is no number (0 times it is none either) makes the key's score none
-                            bf[h] = fmaf(-RC::kOffset, sv, bv) + ((sv - sv) + (bv - bv));
-                            sf[h] = sv * RC::kScale;
+                            bf[h] = fmaf(-RC::kOffset * RC::kDown, sv, bv * RC::kDown) + ((sv - sv) + (bv - bv));
+                            sf[h] = sv * (RC::kScale * RC::kDown);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n)

@@ -324,13 +324,16 @@ struct Pair<__half> {
 };
 
 // Pair j of a word's two halves as an operand without scale and bias: 4-bit
-// codes j = 0..3 and f16 8-bit codes carry kRawOffset, bf16 8-bit codes are
-// multiplied by 1 / kRawScale.
+// codes j = 0..3 and f16 8-bit codes carry kOffset, bf16 8-bit codes are
+// multiplied by 1 / kScale.  Scores are summed times kDown: a bf16 scale of
+// 4-bit codes may be 2^125, and 128 of those are no fp32 (8 bits down they
+// are, and the smallest scale and bias stay exact).
 template <typename TA, int BITS>
 struct RawCode {
     static constexpr bool kBf = std::is_same<TA, __nv_bfloat16>::value;
     static constexpr float kOffset = kBf ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f;
     static constexpr float kScale = kBf && BITS == 8 ? 64.0f : 1.0f;
+    static constexpr float kDown = kBf && BITS == 4 ? 1.0f / 256.0f : 1.0f;
     __device__ __forceinline__ static uint32_t pair(uint32_t u, int j) {
         if constexpr (BITS == 4) return and_or(u >> (4 * j), 0x000F000Fu, Act<TA>::kMagic);
         else if constexpr (kBf) return Pair<TA>::mul(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, 0x7F007F00u);

@@ -288,6 +288,7 @@ class PagedKVCache:
             scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
             check(lib.lmoe_paged_attention(self._desc_ref, ctypes.byref(r), heads, q.data_ptr(), q.stride(0),
                                            q.stride(1), scale, min(max(int(window), 0), 2**31 - 1),
-                                           min(int(sinks), 2**31 - 1), out.data_ptr(), _ptr(scratch), need, self.ws.ptr(), self._stream()),
+                                           min(int(sinks), 2**31 - 1), out.data_ptr(), _ptr(scratch), need,
+                                           self.ws.ptr(), self._stream()),
                   "lmoe_paged_attention")
         return out

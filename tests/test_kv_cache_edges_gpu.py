@@ -195,3 +195,17 @@ def test_windows_of_zero_and_less_are_none(built, rows):
     for window in (0, -1, -2**31, -2**32 + 5, -2**40):
         got = case.cache.attend(q, case.table, case.lens, case.start, window=window, sinks=1)
         assert torch.equal(got, want), window
+
+
+# ------------------------------------------------------------------ extreme values
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 60])
+def test_keys_near_the_largest_value(built, bits, rows):
+    """bf16 keys up to 1e38 and queries so small that the scores are ordinary."""
+    case = Case([200 + rows, 70], [rows, min(rows, 50)], bits=bits, gs=32, d=64, hk=1, page=16)
+    c, cells = case.cache, case.n_pages * 16
+    k = (torch.randn(cells, 1, 64, device="cuda") * 1.5e38).clamp(-3.3e38, 3.3e38).to(torch.bfloat16)
+    v = torch.randn(cells, 1, 64, device="cuda").to(torch.bfloat16)
+    c.append(k, v, torch.arange(case.n_pages, **I32)[None], torch.tensor([cells], **I32), torch.tensor([0, cells], **I32))
+    assert bits == 16 or float(c.k_scales.max()) > 4e38 / 2**bits
+    attend_and_check(case, 2, q=case.q(2, amp=2.0**-122), scale=0.02)
