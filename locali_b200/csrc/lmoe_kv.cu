@@ -555,8 +555,9 @@ int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, i
     a.group = q_heads / cache->kv_heads;
     while ((1 << a.group_shift) < a.group) ++a.group_shift;
     a.group_mul = (((uint64_t)1 << (31 + a.group_shift)) + a.group - 1) / a.group;
-    // a scale of zero (all terms equal) as one that no score makes visible: 0 times a hidden score's -inf is no number
-    a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 2e-38f);
+    // a scale of zero (all terms equal) as the smallest fp32, which no finite score makes visible (2^-149 2^128): 0 times
+    // a hidden score's -inf is no number
+    a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 1.401298464324817e-45f);
     a.window = window > 0 ? window : 0;
     a.sinks = window > 0 ? sinks : 0;
     a.scratch = static_cast<uint8_t *>(scratch);

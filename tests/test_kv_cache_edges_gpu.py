@@ -209,3 +209,16 @@ def test_keys_near_the_largest_value(built, bits, rows):
     c.append(k, v, torch.arange(case.n_pages, **I32)[None], torch.tensor([cells], **I32), torch.tensor([0, cells], **I32))
     assert bits == 16 or float(c.k_scales.max()) > 4e38 / 2**bits
     attend_and_check(case, 2, q=case.q(2, amp=2.0**-122), scale=0.02)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 60])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 3e-39])
+def test_smallest_scales(built, rows, scale):
+    """A scale of zero makes all terms equal, whatever the scores; a tiny one is taken as it is."""
+    case = Case([200 + rows], [rows], d=64, hk=1)
+    c = case.cache
+    c.k.zero_()
+    c.k[..., 0] = (torch.rand(c.k.shape[:3], device="cuda") * 1.5e19).to(torch.bfloat16)
+    q = torch.zeros(case.n, 2, 64, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1e19
+    attend_and_check(case, 2, q=q, scale=scale)
