@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
         // the warp's begins; -2: no such positions, or none
         // that a row sees; -1: no page.
         auto runs_of = [&](int i) -> long long {
-            long long r = -2;
+            long long r = lane < KT ? -2 : 0;
             if (lane < KT && i < nb) {
                 const int p = t.block(b0 + warp + i * kRowWarps) * KS + lane * 16;
                 if (p < t.hi && run_seen(a, t, p)) {
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 const uint32_t u = ring + slot * G::UB;
                 const int r0 = lane / (RB / 16), c0 = lane % (RB / 16);
                 const uint32_t part = unit_off<BITS, D, GS, W>(r0, c0 * 16);
-                const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, lane < KT && runs < 0);
+                const bool all = k0 + KS <= t.hi && !__any_sync(0xffffffffu, runs < 0);
                 const uint8_t *const kv = a.c.kv[W] + lane * 16;
                 if (all) {
 #pragma unroll
