@@ -2,8 +2,8 @@
 // key/value cache, and the join of tiles cut over several blocks.
 //
 // out = sum_j softmax_j(scale q . k_j) v_j in one pass over the keys with the
-// running maximum and sum of the softmax.  A tile's keys and values are read
-// once.  On a B200 a 16-bit cache is bound by HBM (128 windowed sequences, 272
+// running reference (the maximum, shifted: Term in lmoe_attn.cuh) and sum of
+// the softmax.  A tile's keys and values are read once.  On a B200 a 16-bit cache is bound by HBM (128 windowed sequences, 272
 // MB: 55 us, 4.9 of 6.5 TB/s); codes by the instructions that make numbers of
 // them (64 sequences of 4500 on average, 8 bits, 626 MB: 132 us, 4.7 TB/s, two
 // thirds of the issue slots busy; 4 bits, 482 MB: 137 us, 3.5 TB/s).
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                     for (int kt = 1; kt < KT; ++kt) x = max_nan(x, max_nan(s[kt][n][c], s[kt][n][c + 2]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    x = max_nan(m[n][c], x);
+                    x = max_nan(m[n][c], x - Term<TA, false>::kSet);
                     if (full) seen[n][c] = true;
                     mu[n][c] = x == -INFINITY ? 0.0f : x;
                     f[n][c] = ex2(m[n][c] - mu[n][c]);

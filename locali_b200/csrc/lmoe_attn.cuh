@@ -259,6 +259,22 @@ __device__ __forceinline__ float *part_ptr(const AttnArgs &a, int grid, size_t f
     return reinterpret_cast<float *>(a.scratch + (size_t)grid * sizeof(MergeRec)) + ((size_t)2 * c + slot) * floats;
 }
 
+// A row's terms are exp2(score - m), m its reference: any value may serve, as
+// the result is a quotient.  m is set so that the largest score's term is
+// 2^kSet.  The few-row kernel sets it at every larger score.  The chunk kernel,
+// whose sums lie in tensor memory, waits until a term would pass 2^kTop (2^8
+// above; 2^4 for f16, set 2^11 high, cost windowed chunks 15 %).
+//   f16: the terms of many keys far below the largest still count together,
+//   and f16 has no normal value under 2^-14: the largest term is put near the
+//   largest f16, so terms of 2^-29 of it (chunks: 2^-21) and more keep all
+//   their bits.
+template <typename TA, bool CHUNK>
+struct Term {
+    static constexpr bool kF16 = std::is_same<TA, __half>::value;
+    static constexpr float kSet = kF16 ? (CHUNK ? 7.0f : 15.0f) : 0.0f;
+    static constexpr float kTop = kF16 ? 15.0f : 8.0f;
+};
+
 // maximum that keeps a NaN
 __device__ __forceinline__ float max_nan(float x, float y) {
     float r;

@@ -24,9 +24,9 @@
 // MMAs.  Issued as they came, the MMAs of both interleaved and ended together,
 // and the two softmaxes then shared the exponential unit while the tensor pipe
 // waited.  The
-// running maximum of a row moves only when a score passes it by 2^8: until
-// then terms may exceed 1, which costs nothing in fp32 and leaves the sums in
-// tensor memory untouched (a row's result is the quotient either way).
+// reference of a row (Term in lmoe_attn.cuh) moves only when a score passes it
+// by some powers of two: until then terms grow, which costs nothing in fp32
+// and leaves the sums in tensor memory untouched.
 //
 // V is the MN-major B operand (head dimension contiguous), so keys and values
 // share one layout: [D / 64][128 positions][128 bytes], 16-byte chunk c of
@@ -324,9 +324,9 @@ __device__ __forceinline__ float row_terms(uint32_t ts, F &&mask, float sc, floa
     return s0 + s1;
 }
 
-// Terms over an S seen in full with the running maximum m as it is, in one
-// read; nothing is written (again = true) when a score of a row of the warp
-// passes its maximum by more than 2^8 or is no number.
+// Terms over an S seen in full with the reference m as it is, in one read;
+// nothing is written (again = true) when a term of a row of the warp passes
+// the largest there may be or a score is no number.
 template <typename TA>
 __device__ __forceinline__ float row_try(uint32_t ts, float sc, float m, bool &again) {
     const float mu = m == -INFINITY ? 0.0f : m;
@@ -367,7 +367,7 @@ __device__ __forceinline__ float row_try(uint32_t ts, float sc, float m, bool &a
         if (c < 6) tmem_wait_ld(v);
     }
     const float x = max_nan(x0, x1) * sc;
-    again = __any_sync(0xffffffffu, !(x <= m + 8.0f) && !(x == -INFINITY));
+    again = __any_sync(0xffffffffu, !(x <= m + Term<TA, true>::kTop) && !(x == -INFINITY));
     if (!again) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         if (bad >> (2 * c) & 2u) x &= 0x0000FFFFu;
                         return x;
                     };
-                    // with the maximum as it is, unless a score of the block passes it
+                    // with the reference as it is, unless a score of the block passes it
                     const uint32_t ts = tm_s(t) + lanes;
                     bool again = true;
                     if (full && i > b0) {
@@ -623,10 +623,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     }
                     if (again) {
                         const float x = row_max(ts, mask, seen) * sc;
-                        const bool move = !(x <= m + 8.0f) && !(x == -INFINITY);
+                        const bool move = !(x <= m + Term<TA, true>::kTop) && !(x == -INFINITY);
                         if (__any_sync(0xffffffffu, move)) {
-                            const float f = move ? ex2(m - x) : 1.0f;
-                            if (move) m = x;
+                            const float to = x - Term<TA, true>::kSet, f = move ? ex2(m - to) : 1.0f;
+                            if (move) m = to;
                             l *= f;
                             if (i > b0) {  // the sums so far
 #pragma unroll 1

@@ -222,3 +222,38 @@ def test_smallest_scales(built, rows, scale):
     q = torch.zeros(case.n, 2, 64, dtype=torch.bfloat16, device="cuda")
     q[..., 0] = 1e19
     attend_and_check(case, 2, q=q, scale=scale)
+
+
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("rows,seqs", [(1, 1200), (5, 1200), (60, 300)])
+@pytest.mark.parametrize("drop", [8.0, 12.0, 17.1])
+def test_f16_terms_far_below_the_first_token(built, bits, rows, seqs, drop):
+    """One first token far above thousands of others, whose terms together still count: at exp(-17.1) each would be
+    near half the smallest f16.  The terms are held 2^7 and more above that.  Many sequences (of the same pages), so
+    that a row's keys are not cut over launch blocks, each with a largest term of its own."""
+    L, d = 12000, 64
+    case = Case([L], [rows], dtype="f16", bits=bits, gs=32, d=d, hk=1, page=16)
+    c, g = case.cache, case.gen
+    k = torch.randn(L, 1, d, generator=g, device="cuda") * 0.1
+    k[:, :, 0] = 0.0
+    k[0, 0, :] = 0.0
+    k[0, 0, 0] = 4.0
+    v = 100.0 + torch.randn(L, 1, d, generator=g, device="cuda")
+    v[0] = 0.0
+    c.append(k.half(), v.half(), case.table, case.lens, torch.tensor([0, L], **I32))
+    q = torch.randn(seqs * rows, 2, d, generator=g, device="cuda")
+    q[..., 0] = drop * 8.0 / 4.0
+    q = q.half()
+    start = torch.arange(seqs + 1, **I32) * rows
+    got, qn = np64(c.attend(q, case.table.repeat(seqs, 1), case.lens.repeat(seqs), start)), np64(q)
+    hk, hv = case.seq(case.held("k"), 0, 0), case.seq(case.held("v"), 0, 0)
+    see = K.visible(np.arange(L - rows, L), L, 0, 0)
+    for b in (0, 7, seqs // 2, seqs - 1):
+        at = slice(b * rows, (b + 1) * rows)
+        for h in range(2):
+            o, A, B, N = K.attention(qn[at, h], hk, hv, see, 0.125)
+            tol = K.tolerance(o, A, B, N * 2.0**-7, "f16", bits < 16, L)
+            err = np.abs(got[at, h] - o)
+            assert (err <= tol).all(), ((err / tol).max(), (err / np.abs(o)).max())
