@@ -486,7 +486,8 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
  * zero for a row that sees nothing.  What a row does not see does not touch
  * its result, infinities and NaN included.  Softmax statistics and sums are in
- * fp32; the softmax terms and quantised values enter the products in dtype, and
+ * fp32 (with bf16 values of 3e38 the sums of 2^16 keys fit, and values under
+ * 2^-100 lose bits); the softmax terms and quantised values enter the products in dtype, and
  * so do quantised keys where the sequences have more than 16 rows (tokens x
  * query heads of a key/value head) on average (as two numbers, their sum exact
  * to 16 bits, for bf16 and heads of 64); for fewer the keys' codes are

@@ -268,11 +268,14 @@ __device__ __forceinline__ float *part_ptr(const AttnArgs &a, int grid, size_t f
 //   and f16 has no normal value under 2^-14: the largest term is put near the
 //   largest f16, so terms of 2^-29 of it (chunks: 2^-21) and more keep all
 //   their bits.
+//   bf16: a value may be near 2^128, where the fp32 sums end too: with terms of
+//   2^-24 (2^-16) the sums of 2^16 keys and more stay below it.  The price is
+//   at the other end, where values under 2^-100 lose bits.
 template <typename TA, bool CHUNK>
 struct Term {
     static constexpr bool kF16 = std::is_same<TA, __half>::value;
-    static constexpr float kSet = kF16 ? (CHUNK ? 7.0f : 15.0f) : 0.0f;
-    static constexpr float kTop = kF16 ? 15.0f : 8.0f;
+    static constexpr float kSet = kF16 ? (CHUNK ? 7.0f : 15.0f) : -24.0f;
+    static constexpr float kTop = kF16 ? 15.0f : -16.0f;
 };
 
 // maximum that keeps a NaN

@@ -257,3 +257,20 @@ def test_f16_terms_far_below_the_first_token(built, bits, rows, seqs, drop):
             tol = K.tolerance(o, A, B, N * 2.0**-7, "f16", bits < 16, L)
             err = np.abs(got[at, h] - o)
             assert (err <= tol).all(), ((err / tol).max(), (err / np.abs(o)).max())
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("rows", [1, 5, 60])
+@pytest.mark.parametrize("size", [3e38, 2.0**-96])
+def test_values_of_the_largest_and_small_sizes(built, bits, rows, size):
+    """bf16 values of one sign near the largest one, thousands of them with nearly equal terms: their sum before the
+    division is far past the type.  And small ones, which the terms' scaling must not lose."""
+    L = 6000 + rows
+    case = Case([L, 300], [rows, rows], bits=bits, gs=32, d=64, hk=1, page=64)
+    c, cells = case.cache, case.n_pages * 64
+    k = torch.randn(cells, 1, 64, device="cuda").to(torch.bfloat16)
+    v = (size * (0.9 + 0.1 * torch.rand(cells, 1, 64, device="cuda"))).to(torch.bfloat16)
+    c.append(k, v, torch.arange(case.n_pages, **I32)[None], torch.tensor([cells], **I32), torch.tensor([0, cells], **I32))
+    got = attend_and_check(case, 2, q=case.q(2, amp=0.3))
+    assert (np64(got) > 0.85 * size).all()
+    attend_and_check(case, 2, q=case.q(2, amp=0.3), window=500, sinks=3)
