@@ -417,7 +417,10 @@ int lmoe_ep_combine(const float *back, int32_t tokens, int32_t world,
  *           + bias would exceed the largest finite T,
  *   code  = clamp(rint((x - bias) / scale), 0, n), 0 where scale is 0,
  * the quotients as if computed exactly, and stands for T(scale * code +
- * bias).  A group with an infinity or a NaN holds scale = bias = NaN. */
+ * bias).  A group with an infinity or a NaN holds scale = bias = NaN.  Arrays
+ * that another program wrote may hold scales and biases whose values pass the
+ * type: those are infinities (bf16 with 8 bits: no numbers at a scale of 2^122
+ * and more), and reach the rows that see them only. */
 typedef struct lmoe_kv_cache {
     void *k; /* bits 16: dtype [n_pages, kv_heads, page_size, head_dim];
               * bits 8, 4: uint32 [n_pages, kv_heads, page_size, head_dim * bits / 32] */

@@ -367,6 +367,26 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t u, int j, uint32_t s2, ui
     else return Pair<TA>::value8(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, s2, b2);
 }
 
+// The value of one code, as the pairs above give it, in 16 bits.
+template <typename TA, int BITS>
+__device__ __forceinline__ uint32_t code_value(uint32_t code, uint32_t s16, uint32_t b16) {
+    const uint32_t s2 = Pair<TA>::template scale<BITS>(s16 * 0x10001u), b2 = b16 * 0x10001u;
+    return (BITS == 4 ? Pair<TA>::value4(code, 0, s2, b2) : Pair<TA>::value8(code, s2, b2)) & 0xFFFFu;
+}
+template <typename TA>
+__device__ __forceinline__ bool nonfinite16(uint32_t x) {
+    return (x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
+}
+// Is a value of the group no number, or rounded past the type's largest?  The
+// values lie between the bias (code 0) and the last code's, and where the bias
+// is no number the last is none either.
+template <typename TA, int BITS>
+__device__ __forceinline__ bool group_nonfinite(uint32_t s16, uint32_t b16) {
+    // from here on values round past the largest
+    constexpr float lim = std::is_same<TA, __half>::value ? 65520.0f : 3.39617752923046e38f;
+    return !(fabsf(fmaf(Act<TA>::to_f((uint16_t)s16), (float)((1 << BITS) - 1), Act<TA>::to_f((uint16_t)b16))) < lim);
+}
+
 int attn_num_sms();
 // lmoe_attn.cu: joins the cut tiles of R rows of a launch of `grid` blocks; y: merge blocks for each
 cudaError_t launch_attn_merge(int act_f16, int R, int D, int grid, int y, const AttnArgs &a, cudaStream_t st);

@@ -175,7 +175,14 @@ __device__ __forceinline__ void cpa16(uint32_t dst, const void *src, int bytes) 
 
 template <typename TA>
 __device__ __forceinline__ bool nonfinite2(uint32_t x) {
-    return (x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask || (x >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
+    return nonfinite16<TA>(x) || nonfinite16<TA>(x >> 16);
+}
+// the pair with what is no number as zero
+template <typename TA>
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+    if (nonfinite16<TA>(x)) x &= 0xFFFF0000u;
+    if (nonfinite16<TA>(x >> 16)) x &= 0xFFFFu;
+    return x;
 }
 
 // 8 codes -> 8 values as 16-bit pairs in order
@@ -685,8 +692,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                             if constexpr (Q) {
                                 const uint32_t by = a.c.kv[1][kr * RB + d * BITS / 8];
                                 const uint32_t code = BITS == 8 ? by : by >> (4 * (d & 1)) & 15u;
-                                y = fmaf(Act<TA>::to_f(a.c.scale[1][kr * NG + d / GS]), (float)code,
-                                         Act<TA>::to_f(a.c.bias[1][kr * NG + d / GS]));
+                                y = Act<TA>::to_f((uint16_t)code_value<TA, BITS>(code, a.c.scale[1][kr * NG + d / GS],
+                                                                                 a.c.bias[1][kr * NG + d / GS]));
                             } else {
                                 y = Act<TA>::to_f(reinterpret_cast<const uint16_t *>(a.c.kv[1])[kr * D + d]);
                             }
@@ -848,12 +855,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 bool no = false;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    uint32_t x = in_lane ? __byte_perm(sc[g / 2], bi[g / 2], g & 1 ? 0x7632 : 0x5410) : 0u;
+                    const uint32_t x = in_lane ? __byte_perm(sc[g / 2], bi[g / 2], g & 1 ? 0x7632 : 0x5410) : 0u;
                     // in a block that only some rows see, values that are no numbers are taken out
-                    if (which && n.part >= 0 && nonfinite2<TA>(x)) {
-                        no = true;
-                        x = 0;
-                    }
+                    if (which && n.part >= 0) no |= group_nonfinite<TA, BITS>(x & 0xFFFFu, x >> 16);
                     spair[lane * NG + g] = make_uint2(Pair<TA>::template scale<BITS>(__byte_perm(x, 0u, 0x1010)),
                                                       __byte_perm(x, 0u, 0x3232));
                 }
@@ -879,6 +883,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                             const uint4 y = dequant8_rest<BITS>(code[x0 + x][0], code[x0 + x][WPC - 1], sv[x].x, sv[x].y, v[x]);
                             sts128v(dst - G::OFF_K + G::OFF_L + op_off(lw * 32 + (x0 + x) * RPI + rr, cc), y.x, y.y, y.z, y.w);
                         }
+                    }
+                }
+                if (taken) {  // the lane's own stores
+#pragma unroll 1
+                    for (int x = 0; x < IT; ++x) {
+                        const uint32_t at = dst + op_off(lw * 32 + x * RPI + rr, cc);
+                        const uint4 v = lds128(at);
+                        sts128v(at, finite2<TA>(v.x), finite2<TA>(v.y), finite2<TA>(v.z), finite2<TA>(v.w));
                     }
                 }
                 done(n, u, taken);
@@ -920,14 +932,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                         const bool no = nonfinite2<TA>(v.x) || nonfinite2<TA>(v.y) || nonfinite2<TA>(v.z) || nonfinite2<TA>(v.w);
                         const uint32_t bl = __ballot_sync(0xffffffffu, no);
                         if (bl == 0) continue;
-                        if (no) {
-                            auto out = [](uint32_t y) {
-                                if ((y & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) y &= 0xFFFF0000u;
-                                if ((y >> 16 & Pair<TA>::kExpMask) == Pair<TA>::kExpMask) y &= 0xFFFFu;
-                                return y;
-                            };
-                            sts128v(at, out(v.x), out(v.y), out(v.z), out(v.w));
-                        }
+                        if (no) sts128v(at, finite2<TA>(v.x), finite2<TA>(v.y), finite2<TA>(v.z), finite2<TA>(v.w));
 #pragma unroll
                         for (int y = 0; y < RPI; ++y)
                             if (bl >> (y * LPR) & ((1u << LPR) - 1u)) taken |= 1u << (x * RPI + y);

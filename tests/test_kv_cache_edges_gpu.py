@@ -274,3 +274,29 @@ def test_values_of_the_largest_and_small_sizes(built, bits, rows, size):
     got = attend_and_check(case, 2, q=case.q(2, amp=0.3))
     assert (np64(got) > 0.85 * size).all()
     attend_and_check(case, 2, q=case.q(2, amp=0.3), window=500, sinks=3)
+
+
+@pytest.mark.parametrize("dtype,bits,scale", [("f16", 8, 300.0), ("f16", 4, 8000.0), ("bf16", 8, 2.0**121), ("bf16", 4, 2.0**125)])
+@pytest.mark.parametrize("d,gs", [(64, 32), (128, 128)])
+@pytest.mark.parametrize("rows", [1, 5, 150])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 2)])
+def test_hidden_values_past_the_type(built, dtype, bits, scale, d, gs, rows, window, sinks):
+    """Scales and biases that are finite but whose top codes pass the type's largest value (arrays that append did not
+    write): rows that see the position get infinities, the others never meet them, and the group's other values count."""
+    case = Case([rows + 260, rows + 40], [rows, rows], dtype=dtype, bits=bits, gs=gs, d=d, hk=1, page=16)
+    c = case.cache
+    tab = case.table.cpu()
+    top = 2**bits - 1
+    for b, L in enumerate(case.lens_l):
+        for i, j in enumerate(sorted({L - 1, L - 1 - rows // 2, L - rows - 52, L - rows - 10, 1, 3})):
+            at = (int(tab[b, j // 16]), 0, j % 16)
+            for t, x in ((c.v_scales, scale), (c.v_biases, -0.125 * scale)):
+                t[at][0] = x
+            codes = torch.randint(0, 2, (d,))  # small codes but for two, at other places for each position
+            codes[[3 * i, 3 * i + 1]] = top
+            words = K.pack(codes.numpy()[None], bits)[0].view(np.int32)
+            c.v[at] = torch.from_numpy(words.copy()).cuda()
+    hv = K.round_to(case.held("v"), dtype)
+    assert np.isinf(hv).any() and np.isfinite(np64(c.v_scales)).all()
+    # the finite values of those groups are as large as the type: their rounding is part of the tolerance
+    attend_and_check(case, 2, window=window, sinks=sinks, hk_v=(case.held("k"), hv))
