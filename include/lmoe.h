@@ -483,7 +483,8 @@ int lmoe_kv_read(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, void *k, 
 /* Attention of the rows over their sequences' cached positions (their own
  * included: append first).  q [n_rows, q_heads, head_dim] of dtype (strides as
  * above), q_heads a multiple of kv_heads (query head h reads key/value head
- * h / (q_heads / kv_heads)); out [n_rows, q_heads, head_dim] contiguous, must
+ * h / (q_heads / kv_heads)); out [n_rows, q_heads, head_dim] contiguous, of
+ * 2^38 bytes at most and 2^30 rows of a key/value head (LMOE_EUNSUPPORTED), must
  * not overlap q.  A row at position p sees position j of its sequence if 0 <=
  * j <= p and (window <= 0 or j > p - window or j < sinks):
  *   out = sum_j softmax_j(scale * q . k_j) v_j,

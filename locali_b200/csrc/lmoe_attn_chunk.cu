@@ -709,14 +709,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 uint8_t *to = whole ? reinterpret_cast<uint8_t *>(a.out + ((int64_t)ti.row0 * a.q_heads + ti.h * a.group) * D)
                                     : reinterpret_cast<uint8_t *>(part_ptr(a, gridDim.x, part_floats<kCkRows, D>(),
                                                                            blockIdx.x, b0 == 0 ? 1 : 0));
-                // the row's offset: 32 bytes at a time, so that it fits 32 bits
-                const uint32_t mine = whole ? (uint32_t)(((int64_t)tok * (a.q_heads - a.group) + row) * (D * 2 / 32))
-                                            : (uint32_t)((t * kCkSub + r) * (D * 4 / 32));
+                // the row's offset, 64 bytes at a time: it fits 32 bits for results of up to 2^38 bytes (kMaxOut)
+                const uint32_t mine = whole ? (uint32_t)(((int64_t)tok * (a.q_heads - a.group) + row) * (D * 2 / 64))
+                                            : (uint32_t)((t * kCkSub + r) * (D * 4 / 64));
                 uint8_t *dst[4];
                 const uint32_t ins = __ballot_sync(0xffffffffu, in);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    dst[x] = to + (int64_t)__shfl_sync(0xffffffffu, mine, 8 * x + (lane >> 2)) * 32 + (lane & 3) * 16;
+                    dst[x] = to + (int64_t)__shfl_sync(0xffffffffu, mine, 8 * x + (lane >> 2)) * 64 + (lane & 3) * 16;
                 const int cols = whole ? 32 : 16;  // columns of 64 bytes
 #pragma unroll 1
                 for (int c = 0; c < D; c += cols) {

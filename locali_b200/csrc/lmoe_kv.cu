@@ -544,6 +544,7 @@ int lmoe_paged_attention(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, i
     if (!strided_ok(q, q_token_stride, q_head_stride) || !out || !al16(out) || !al16(scratch)) return LMOE_EINVAL;
     // row numbers of the tiles (rows x heads of a group) are 32-bit
     if ((int64_t)a.r.n_rows * (q_heads / cache->kv_heads) > (1 << 30)) return LMOE_EUNSUPPORTED;
+    if ((int64_t)a.r.n_rows * q_heads * (cache->head_dim * 2) > kMaxOut) return LMOE_EUNSUPPORTED;
     const size_t need = lmoe_paged_attention_scratch(cache, rows, q_heads);
     if (scratch_bytes < need) return LMOE_EWORKSPACE;
     if (need && !scratch) return LMOE_EINVAL;

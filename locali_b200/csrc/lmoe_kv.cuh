@@ -72,6 +72,10 @@ struct KvRows {
     }
 };
 
+// Bytes of an attention result, at most (the chunk kernel counts them by 64 in
+// 32 bits): more than a B200 holds.
+constexpr int64_t kMaxOut = (int64_t)1 << 38;
+
 struct KvCopyArgs {
     KvView c;
     KvRows r;
