@@ -445,7 +445,8 @@ typedef struct lmoe_kv_cache {
  * p % page_size of page page_table[b * table_stride + p / page_size].  Rows
  * in front of row_start[0] and from row_start[n_seqs] on belong to no sequence
  * and are left alone.
- * All arrays are on the device and are read by the kernels only; entries of
+ * All arrays are on the device, are read by the kernels only and must not be
+ * written before the call's kernels have ended (stream order); entries of
  * page_table behind a sequence's last page, and (attention with a window)
  * those of pages that none of the sequence's rows sees a position of, are not
  * looked at and may hold anything.  A sequence's rows with a negative position

@@ -115,8 +115,10 @@ struct Cursor {
                 if (++t.rt * (long long)R >= (long long)t.n * a.group) {
                     t.rt = 0;
                     int b = t.b, nt;
-                    do nt = seq_rows<R>(a, ++b, t);
-                    while (nt == 0);
+                    do {
+                        if (++b >= a.r.n_seqs) return false;
+                        nt = seq_rows<R>(a, b, t);
+                    } while (nt == 0);
                 }
                 tile_range<R, KS>(a, t);
             }
@@ -147,7 +149,9 @@ __device__ __forceinline__ long long seq_units(const AttnArgs &a, int b) {
 // Finds the launch block's run; every thread of the block calls it (NTHR
 // threads, sm of NTHR / 32 + 4 long longs).  False: no work.  WARP: a warp for
 // each sequence (few sequences of many tiles), else a thread.  minu: units a
-// run has at least.
+// run has at least.  Lengths and row starts are read more than once and must
+// not change meanwhile; no search here or in Cursor::next rests its end on
+// that.
 template <int R, int KS, int X, int NTHR, bool WARP>
 __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long long *sm, Share &sh, Cursor<R, KS, X> &cur) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -165,6 +169,7 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long lon
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     if (lane == 0) sm[warp] = sum;
+    if (tid < 4) sm[NW + tid] = 0;
     __syncthreads();
     long long total = 0;
     for (int w = 0; w < NW; ++w) total += sm[w];
@@ -205,7 +210,7 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long lon
     const int nt = seq_rows<R>(a, (int)sm[NW], t);
     if (warp == 0) {
         long long off = s - sm[NW + 1];
-        for (int r0 = 0;; r0 += 32) {
+        for (int r0 = 0; r0 < nt; r0 += 32) {
             t.rt = r0 + lane;
             long long w = 0;
             if (t.rt < nt) {
@@ -233,7 +238,7 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int minu, long lon
     t.rt = (int)sm[NW + 2];
     tile_range<R, KS>(a, t);
     const long long off = sm[NW + 3];
-    t.h = (int)div_small(off, t.nblk + X);
+    t.h = min((int)div_small(off, t.nblk + X), a.c.kv_heads - 1);
     cur.at = s - (off - (long long)t.h * (t.nblk + X));
     cur.end = sh.begin(blockIdx.x + 1);
     cur.open(s);
