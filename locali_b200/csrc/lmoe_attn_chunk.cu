@@ -74,7 +74,8 @@ struct ChunkGeo {
     static constexpr bool LO = BITS != 16 && D == 64 && std::is_same<TA, __nv_bfloat16>::value;
     static constexpr int TILE = 128 * D * 2;  // an operand tile: 128 rows of D
     static constexpr int NG = BITS == 16 ? 1 : D / GS;
-    static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_L = 6 * TILE, OFF_X = (LO ? 8 : 6) * TILE;
+    static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_L = 6 * TILE,
+                         OFF_X = OFF_L + (LO ? 2 * TILE : 0);
     static constexpr int SCALES = BITS == 16 ? 0 : 8 * 32 * NG * (int)sizeof(uint2);  // scales and biases of the loader warps' rows
     static constexpr int OFF_STG = OFF_X + SCALES;                   // output staging of the softmax warps
     static constexpr int SMEM = 1024 + OFF_STG + 8 * kStgWarp;
@@ -384,48 +385,6 @@ __device__ __forceinline__ float row_try(uint32_t ts, float sc, float m, bool &a
             tmem_st32(ts + 32 * h, z);
         }
     }
-    float s0, s1;
-    unpack_f2(sum, s0, s1);
-    return s0 + s1;
-}
-
-// Terms exp2(S sc - mu) over S, as 16-bit pairs for the tensor core (32
-// columns of S become 16, behind the reads); returns their sum in fp32.
-template <typename TA, bool FULL, class F>
-__device__ __forceinline__ float row_terms(uint32_t ts, F &&mask, float sc, float mu) {
-    const uint64_t sc2 = pack_f2(sc, sc), mu2 = pack_f2(-mu, -mu);
-    uint64_t sum = 0;
-    auto take = [&](uint32_t (&v)[32], int c) {
-        const uint32_t mk = FULL ? 0u : mask(c);
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-            float p0, p1;
-            unpack_f2(fma_f2(pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, mu2), p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            if constexpr (!FULL) {
-                if (!(mk >> e & 1u)) p0 = 0.0f;
-                if (!(mk >> (e + 1) & 1u)) p1 = 0.0f;
-            }
-            sum = add_f2(sum, pack_f2(p0, p1));
-            pk[e / 2] = Act<TA>::pack2(p0, p1);
-        }
-        tmem_st16(ts + 16 * c, pk);
-    };
-    uint32_t v[32], y[32];
-    tmem_ld32(ts, v);
-    tmem_wait_ld32(v);
-    tmem_ld32(ts + 32, y);
-    tmem_wait_ld32(y);  // read before columns 16.. are written over
-    take(v, 0);
-    tmem_ld32(ts + 64, v);
-    take(y, 1);
-    tmem_wait_ld32(v);
-    tmem_ld32(ts + 96, y);
-    take(v, 2);
-    tmem_wait_ld32(y);
-    take(y, 3);
     float s0, s1;
     unpack_f2(sum, s0, s1);
     return s0 + s1;

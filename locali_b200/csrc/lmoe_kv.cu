@@ -438,15 +438,12 @@ int check_cache(const lmoe_kv_cache *c, KvView *v) {
         v->scale[1] = static_cast<uint16_t *>(c->v_scales);
         v->bias[0] = static_cast<uint16_t *>(c->k_biases);
         v->bias[1] = static_cast<uint16_t *>(c->v_biases);
-        v->groups = c->head_dim / c->group_size;
-        v->group_size = c->group_size;
     }
     v->n_pages = c->n_pages;
     v->page_size = c->page_size;
     while (((int64_t)1 << v->page_shift) < c->page_size) ++v->page_shift;
     v->page_mul = (((uint64_t)1 << (31 + v->page_shift)) + c->page_size - 1) / c->page_size;
     v->kv_heads = c->kv_heads;
-    v->row_bytes = c->head_dim * c->bits / 8;
     return LMOE_OK;
 }
 

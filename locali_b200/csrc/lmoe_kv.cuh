@@ -17,9 +17,6 @@ struct KvView {
     uint16_t *scale[2];  // nullptr when bits is 16
     uint16_t *bias[2];
     int32_t n_pages, page_size, kv_heads;
-    int32_t row_bytes;  // bytes of one head row: head_dim * bits / 8
-    int32_t groups;     // groups of one head row
-    int32_t group_size;
     uint64_t page_mul;  // ceil(2^(31 + page_shift) / page_size), 2^page_shift >= page_size
     int32_t page_shift;
     // p / page_size for 0 <= p < 2^31: the multiplier is off by less than
