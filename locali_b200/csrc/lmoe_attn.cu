@@ -59,9 +59,6 @@ struct RowsGeo {
     static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + kRowWarps * R * 8;
 };
 
-__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }

@@ -283,6 +283,10 @@ struct Term {
     static constexpr float kTop = kF16 ? 15.0f : -16.0f;
 };
 
+// 16 bytes into shared memory, `bytes` of them from src and zeros behind
+__device__ __forceinline__ void cp16z(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 // maximum that keeps a NaN
 __device__ __forceinline__ float max_nan(float x, float y) {
     float r;
@@ -300,11 +304,7 @@ template <typename TA>
 struct Pair;
 template <>
 struct Pair<__nv_bfloat16> {
-    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
-        uint32_t d;
-        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-        return d;
-    }
+    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) { return fma2<__nv_bfloat16>(a, b, c); }
     __device__ __forceinline__ static uint32_t mul(uint32_t a, uint32_t b) { return fma(a, b, 0x80008000u); }
     // 8-bit codes: the code's bits are a bf16 subnormal, c * 2^-133;
     // multiplied by 2^127 it is c * 2^-6 exactly, and the scale is taken times
@@ -325,11 +325,7 @@ struct Pair<__nv_bfloat16> {
 };
 template <>
 struct Pair<__half> {
-    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
-        uint32_t d;
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-        return d;
-    }
+    __device__ __forceinline__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) { return fma2<__half>(a, b, c); }
     template <int BITS>
     __device__ __forceinline__ static uint32_t scale(uint32_t s2) {
         return s2;

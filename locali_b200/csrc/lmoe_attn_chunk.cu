@@ -170,10 +170,6 @@ __device__ __forceinline__ uint32_t op_off(int r, int c) {
     return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ void cpa16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 template <typename TA>
 __device__ __forceinline__ bool nonfinite2(uint32_t x) {
     return nonfinite16<TA>(x) || nonfinite16<TA>(x >> 16);
@@ -202,25 +198,6 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w0, uint32_t w1, uint32_t s2,
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// packed fp32 pairs
-__device__ __forceinline__ uint64_t pack_f2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpack_f2(uint64_t v, float &x, float &y) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // 2^x of a pair on the FMA pipe, for x up to 120 or so: x = n + f with n the
 // nearest integer, 2^f by a polynomial on [-1/2, 1/2] (the minimax one of
 // degree 4 with value 1 at 0, relative error 2.9e-6 in fp32), n added to the
@@ -514,7 +491,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 const uint16_t *p = reinterpret_cast<const uint16_t *>(
                     __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), x));
                 const bool ok = ins >> x & 1u;
-                cpa16(qs + op_off(q4 * 32 + x, cc), ok ? p + cc * 8 : a.q, ok ? 16 : 0);
+                cp16z(qs + op_off(q4 * 32 + x, cc), ok ? p + cc * 8 : a.q, ok ? 16 : 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -869,12 +846,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                     const uint8_t *p0 = kv + lane_off + n.r0 * RB, *p1 = kv + lane_off + n.r1 * RB;
 #pragma unroll
                     for (int x = 0; x < IT; ++x)
-                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
+                        cp16z(dst + op_off(lw * 32 + x * RPI + rr, cc), (x * RPI < 16 ? p0 : p1) + (x * RPI % 16) * RB, 16);
                 } else {
 #pragma unroll 1
                     for (int x = 0; x < IT; ++x) {
                         const long long r = row_of(n, x * RPI + rr);
-                        cpa16(dst + op_off(lw * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv, r >= 0 ? 16 : 0);
+                        cp16z(dst + op_off(lw * 32 + x * RPI + rr, cc), r >= 0 ? kv + r * RB + cc * 16 : kv, r >= 0 ? 16 : 0);
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");

@@ -37,21 +37,6 @@ struct Fin<__half> {
     static constexpr uint16_t kNan = 0x7E00;
 };
 
-template <typename TA>
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c);
-template <>
-__device__ __forceinline__ uint32_t fma2<__nv_bfloat16>(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-template <>
-__device__ __forceinline__ uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
 // Scale and bias of a group from its extremes, as 16-bit values; false (both
 // NaN) where the group holds an infinity or a NaN.
 template <typename TA, int BITS>
@@ -107,25 +92,6 @@ __device__ __forceinline__ void group_extremes(const uint32_t (&w)[4], float &lo
     lo = -Act<TA>::to_f((uint16_t)(m >> 16));
 }
 
-__device__ __forceinline__ uint64_t f2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ void unf2(uint64_t v, float &x, float &y) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-
 // Codes clamp(rint((x - b) / s), 0, n) of 8 elements (x >= b), as if computed
 // exactly, in the low bytes of q.  (x - b) * (1 / s) in fp32 is within 7e-5
 // of the quotient up to 256, 5e-6 up to 16 (2^-24 of the difference, 2^-23 of the approximate
@@ -138,16 +104,16 @@ __device__ __forceinline__ void group_codes(const float (&x)[8], float b, float 
     constexpr float kSure = BITS == 8 ? 0.4999f : 0.49999f;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-    const uint64_t nb = f2(-b, -b), i2 = f2(inv, inv), mg = f2(kMagic, kMagic), um = f2(-kMagic, -kMagic);
-    const uint64_t neg = f2(-1.0f, -1.0f);
+    const uint64_t nb = pack_f2(-b, -b), i2 = pack_f2(inv, inv), mg = pack_f2(kMagic, kMagic), um = pack_f2(-kMagic, -kMagic);
+    const uint64_t neg = pack_f2(-1.0f, -1.0f);
     float off = 0.0f, t[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-        const uint64_t v = mul2(add2(f2(x[e], x[e + 1]), nb), i2);
-        const uint64_t r = add2(v, mg);
-        unf2(r, t[e], t[e + 1]);
+        const uint64_t v = mul_f2(add_f2(pack_f2(x[e], x[e + 1]), nb), i2);
+        const uint64_t r = add_f2(v, mg);
+        unpack_f2(r, t[e], t[e + 1]);
         float d0, d1;
-        unf2(add2(v, mul2(add2(r, um), neg)), d0, d1);
+        unpack_f2(add_f2(v, mul_f2(add_f2(r, um), neg)), d0, d1);
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d0)));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(d1)));
     }
