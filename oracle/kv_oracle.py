@@ -117,3 +117,33 @@ def tolerance(o, A, B, N, dtype: str, quantised: bool, keys: int):
     if dtype == "f16":
         t = t + N * 2.0**-25 + 2.0**-25
     return t + 1e-37
+
+
+def expected_error(q, k, v, see, scale, dtype: str, values: bool, keys: bool):
+    """(squared norm of the error that independent roundings leave, squared
+    norm of the result) over all rows.
+
+    A value x of mantissa m in [1, 2) is off by x times an error uniform in
+    +-u / m; with log m uniform the mean of 1 / m^2 is 3 / (8 ln 2), so the
+    error's deviation is g |x|, g = u sqrt(1 / (8 ln 2)) = 0.4247 u.  Rounded
+    are the result, the softmax terms, the values (``values``) and the keys
+    (``keys``: a score is then off by g scale sqrt(sum (q k)^2), and its term by
+    as much of itself).  What fp32 leaves is below a hundredth of that."""
+    g2 = HALF_STEP[dtype] ** 2 / (8 * np.log(2))
+    err = norm = 0.0
+    for r in range(q.shape[0]):
+        j = np.flatnonzero(see[r])
+        if j.size == 0:
+            continue
+        s = scale * (k[j] @ q[r])
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        o = p @ v[j]
+        p2 = p * p
+        e = (o * o).sum() + (1 + values) * (p2 @ (v[j] ** 2)).sum()
+        if keys:
+            off = scale**2 * ((k[j] * q[r]) ** 2).sum(1)
+            e += (p2 * off) @ ((v[j] - o) ** 2).sum(1)
+        err += g2 * e
+        norm += (o * o).sum()
+    return err, norm

@@ -300,3 +300,101 @@ def test_hidden_values_past_the_type(built, dtype, bits, scale, d, gs, rows, win
     assert np.isinf(hv).any() and np.isfinite(np64(c.v_scales)).all()
     # the finite values of those groups are as large as the type: their rounding is part of the tolerance
     attend_and_check(case, 2, window=window, sinks=sinks, hk_v=(case.held("k"), hv))
+
+
+# ------------------------------------------------------------------ how near to 64 bits
+def error_ratio(got, q, hk, hv, pos, scale, dtype, values, keys):
+    """Norm of got's error over the expected one's; got and q [rows, d], pos the rows' positions."""
+    see = K.visible(pos, len(hk), 0, 0)
+    err, _ = K.expected_error(q, hk, hv, see, scale, dtype, values, keys)
+    return ((got - K.attention(q, hk, hv, see, scale)[0]) ** 2).sum(), err
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits,gs,d", [(16, 32, 64), (16, 32, 128), (8, 32, 64), (8, 64, 64), (8, 32, 128), (8, 64, 128),
+                                       (8, 128, 128), (4, 32, 64), (4, 64, 64), (4, 32, 128), (4, 64, 128), (4, 128, 128)])
+@pytest.mark.parametrize("rows", [1, 7, 90])
+def test_error_is_that_of_the_roundings_alone(built, dtype, bits, gs, d, rows):
+    """Each path's error against 64 bits has the norm that the roundings it is to make leave, within a quarter: terms
+    and result, quantised values, and keys only in chunks, where bf16 heads of 64 bring a second tile with the rest.
+    The keys' channels have offsets, so that a rounded key, a tile that lacks or an offset taken off wrongly shows."""
+    heads = 2 if rows == 1 else 4
+    case = Case([rows + 400, rows + 211, rows + 30], [rows] * 3, dtype=dtype, bits=bits, gs=gs, d=d, hk=2, page=16)
+    c, cells = case.cache, case.n_pages * 16
+    g = torch.Generator("cuda").manual_seed(11)
+    ch = 12.0 * (torch.randint(0, 2, (2, d), generator=g, device="cuda") - 0.5)
+    k = (torch.randn(cells, 2, d, generator=g, device="cuda") * 0.5 + ch).to(T[dtype])
+    v = torch.randn(cells, 2, d, generator=g, device="cuda").to(T[dtype])
+    c.append(k, v, torch.arange(case.n_pages, **I32)[None], torch.tensor([cells], **I32), torch.tensor([0, cells], **I32))
+    q = case.q(heads)
+    got, qn = np64(c.attend(q, case.table, case.lens, case.start)), np64(q)
+    hk, hv = case.held("k"), case.held("v")
+    keys = bits < 16 and rows == 90 and not (dtype == "bf16" and d == 64)
+    total = expected = 0.0
+    for b, (L, n) in enumerate(zip(case.lens_l, case.rows_l)):
+        at = slice(case.start_l[b], case.start_l[b + 1])
+        for h in range(heads):
+            a, e = error_ratio(got[at, h], qn[at, h], case.seq(hk, b, h * 2 // heads), case.seq(hv, b, h * 2 // heads),
+                               np.arange(L - n, L), d**-0.5, dtype, bits < 16, keys)
+            total, expected = total + a, expected + e
+    ratio = np.sqrt(total / expected)
+    assert 0.6 < ratio < 1.25, ratio
+
+
+def test_chunk_terms_are_the_exponentials(built):
+    """One-hot values make a row's result its terms: every column of a block, terms over 17 powers of two and up to 2^7
+    above the first block's largest, on the exponential unit and the FMA pipe alike."""
+    L, rows, d = 128 * 5, 20, 64
+    case = Case([L], [rows], dtype="f16", bits=16, d=d, hk=1, page=16)
+    c = case.cache
+    for half in (0, 1):  # columns 0..63, then 64..127 of the second block
+        rng = np.random.default_rng(half)
+        a = np.full(L, -60.0)  # terms of exp(-60) and less
+        a[0] = 0.0
+        first = 128 + 64 * half
+        a[first:first + 64] = K.round_to(rng.uniform(-7.0, 4.8, 64), "f16")
+        k, v = torch.zeros(L, 1, d), torch.zeros(L, 1, d)
+        k[:, 0, 0] = torch.from_numpy(a)
+        v[first + torch.arange(64), 0, torch.arange(64)] = 1024.0
+        c.append(k.half().cuda(), v.half().cuda(), case.table, case.lens, torch.tensor([0, L], **I32))
+        amp = K.round_to(rng.uniform(0.5, 1.0, rows), "f16")
+        q = torch.zeros(rows, 1, d)
+        q[:, 0, 0] = torch.from_numpy(amp)
+        got = np64(c.attend(q.half().cuda(), case.table, case.lens, case.start, scale=1.0))[:, 0]
+        e = np.exp(amp[:, None] * a[None, first:first + 64])
+        want = 1024.0 * e / (1.0 + e.sum(1, keepdims=True))
+        # the term and the result rounded to f16 (the smallest result is 2^-14 and more), the exponential's own error
+        # under 2^-18, fp32 scores of up to 7: 2^-20
+        assert want.min() > 2.0**-14 and np.log2(e.max()) > 5
+        assert (np.abs(got / want - 1.0) <= 2.0**-11 * 2 + 2.0**-17).all(), np.abs(got / want - 1.0).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_prompt_chunks_and_tokens_each_near_64_bits(built, dtype, bits):
+    """A prompt in one chunk, in uneven chunks and token by token: each within a quarter of its roundings' error."""
+    n, hk, heads, d = 300, 2, 4, 64
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(n, hk, d, generator=g, device="cuda").to(T[dtype]) for _ in range(2))
+    q = torch.randn(n, heads, d, generator=g, device="cuda").to(T[dtype])
+    tab = torch.randperm(19, generator=g, device="cuda").to(torch.int32)[None]
+    for cuts in ([0, n], [0, 1, 20, 22, 150, n], list(range(n + 1))):
+        c = PagedKVCache(19, 16, hk, d, bits=bits, group_size=32, dtype=T[dtype])
+        parts = []
+        for a, b in zip(cuts, cuts[1:]):
+            lens, st = torch.tensor([b], **I32), torch.tensor([0, b - a], **I32)
+            c.append(k[a:b], v[a:b], tab, lens, st)
+            parts.append(c.attend(q[a:b], tab, lens, st))
+        c.check()
+        got, qn = np64(torch.cat(parts)), np64(q)
+        total = expected = 0.0
+        for h in range(heads):
+            held = []
+            for x in (k, v):
+                x = np64(x)[:, h // 2]
+                held.append(K.dequantise(*K.quantise(x, bits, 32, dtype), 32) if bits < 16 else x)
+            # f16 keys of chunks are rounded; by the unit scores here that is least for all of them
+            e = error_ratio(got[:, h], qn[:, h], *held, np.arange(n), d**-0.5, dtype, bits < 16,
+                            bits < 16 and dtype == "f16" and len(cuts) < n)
+            total, expected = total + e[0], expected + e[1]
+        assert 0.6 < np.sqrt(total / expected) < 1.25, (len(cuts), np.sqrt(total / expected))
