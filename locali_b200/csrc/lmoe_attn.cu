@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                 if constexpr (Q) {
                     for (int i2 = lane; i2 < KS * SW; i2 += 32) {
                         const uint32_t x = lds_u16(vu + G::CB + i2 * 2), y = lds_u16(vu + G::CB + G::SB + i2 * 2);
-                        odd |= group_nonfinite<TA, BITS>(x, y);
+                        odd |= group_past_type<TA, BITS>(x, y);
                     }
                 } else {
                     for (int i2 = lane; i2 < KS * W4; i2 += 32) {
@@ -498,11 +498,12 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                                     lds_words<1>(vu + unit_off<BITS, D, GS, 1>(k, byte & ~3), w);
                                     const uint32_t code = w[0] >> (dim * BITS % 32) & ((1u << BITS) - 1u);
                                     const uint32_t so = vu + G::CB + (k * SW + dim / GS) * 2;
-                                    v = Act<TA>::to_f((uint16_t)code_value<TA, BITS>(code, lds_u16(so), lds_u16(so + G::SB)));
+                                    v = code_value<TA, BITS>(code, lds_u16(so), lds_u16(so + G::SB));
                                 } else {
                                     v = Act<TA>::to_f((uint16_t)lds_u16(vu + unit_off<16, D, GS, 1>(k, dim * 2)));
                                 }
-                                if (!(fabsf(v) <= 3.402823466e38f)) {
+                                if (past_type<TA>(v)) {
+                                    v *= INFINITY;
 #pragma unroll
                                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -523,12 +524,12 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             const uint32_t wa = vu + unit_off<BITS, D, GS, 1>(k, byte);
                             const uint32_t so = vu + G::CB + (k * SW + byte * 8 / BITS / GS) * 2;
                             const uint32_t x = lds_u16(so), y = lds_u16(so + G::SB);
-                            if (!group_nonfinite<TA, BITS>(x, y)) continue;
+                            if (!group_past_type<TA, BITS>(x, y)) continue;
                             uint32_t w[1];
                             lds_words<1>(wa, w);
 #pragma unroll 1
                             for (int sh = 0; sh < 32; sh += BITS)
-                                if (nonfinite16<TA>(code_value<TA, BITS>(w[0] >> sh & ((1u << BITS) - 1u), x, y)))
+                                if (past_type<TA>(code_value<TA, BITS>(w[0] >> sh & ((1u << BITS) - 1u), x, y)))
                                     w[0] &= ~(((1u << BITS) - 1u) << sh);
                             sts_u16(wa, (uint16_t)w[0]);
                             sts_u16(wa + 2, (uint16_t)(w[0] >> 16));
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                         __syncwarp();
                         for (int i2 = lane; i2 < KS * SW; i2 += 32) {
                             const uint32_t sa = vu + G::CB + i2 * 2;
-                            if (nonfinite16<TA>(code_value<TA, BITS>(0u, lds_u16(sa), lds_u16(sa + G::SB)))) {
+                            if (past_type<TA>(code_value<TA, BITS>(0u, lds_u16(sa), lds_u16(sa + G::SB)))) {
                                 sts_u16(sa, 0);
                                 sts_u16(sa + G::SB, 0);
                             }

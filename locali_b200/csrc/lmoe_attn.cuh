@@ -21,7 +21,6 @@ struct Tile {
     int rows;           // rows of the tile, 1..R
     int minpos, maxpos; // positions of the tile's first and last row
     int hi;             // keys [0, hi) are looked at: those the table has room for
-    int low;            // no row sees keys in front of this, but for the first tokens that stay visible
     int nsink, lo;      // sink blocks, first block of the rest (held at the first one behind hi)
     int nblk;           // blocks; at least 1, so a tile that sees nothing is written
     __device__ __forceinline__ int block(int i) const { return i < nsink ? i : lo + i - nsink; }
@@ -39,7 +38,6 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
     // Held at the first block behind hi: the window of a length far past its
     // table may begin in the last block that 32 bits can count, whose end they
     // cannot.
-    t.low = low;
     t.lo = min(low / KS, (t.hi + KS - 1) / KS);
     t.nsink = t.lo > 0 ? min((min(a.sinks, t.hi) + KS - 1) / KS, t.lo) : 0;
     t.nblk = max(1, t.nsink + max(0, (t.hi + KS - 1) / KS - t.lo));
@@ -47,9 +45,10 @@ __device__ __forceinline__ void tile_range(const AttnArgs &a, Tile &t) {
 
 // Does a row of the tile see one of the 16 positions from p < hi?  Blocks
 // reach past the first tokens and the window's lower edge, and what lies
-// between those may have no page any more.
+// between those may have no page any more.  (In numbers the tile holds anyway:
+// one more cost registers and 3 % of the few-row kernel.)
 __device__ __forceinline__ bool run_seen(const AttnArgs &a, const Tile &t, int p) {
-    return p < a.sinks || p + 16 > t.low;
+    return a.window == 0 || t.minpos - p - 15 < a.window || p < a.sinks;
 }
 
 // Sequence b's rows into t; returns its tiles (of one head).
@@ -368,24 +367,27 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t u, int j, uint32_t s2, ui
     else return Pair<TA>::value8(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, s2, b2);
 }
 
-// The value of one code, as the pairs above give it, in 16 bits.
-template <typename TA, int BITS>
-__device__ __forceinline__ uint32_t code_value(uint32_t code, uint32_t s16, uint32_t b16) {
-    const uint32_t s2 = Pair<TA>::template scale<BITS>(s16 * 0x10001u), b2 = b16 * 0x10001u;
-    return (BITS == 4 ? Pair<TA>::value4(code, 0, s2, b2) : Pair<TA>::value8(code, s2, b2)) & 0xFFFFu;
-}
 template <typename TA>
 __device__ __forceinline__ bool nonfinite16(uint32_t x) {
     return (x & Pair<TA>::kExpMask) == Pair<TA>::kExpMask;
 }
-// Is a value of the group no number, or rounded past the type's largest?  The
-// values lie between the bias (code 0) and the last code's, and where the bias
-// is no number the last is none either.
+// The value of one code before its rounding; like the pairs above no number
+// for bf16 scales of 8-bit codes from 2^122 on.
 template <typename TA, int BITS>
-__device__ __forceinline__ bool group_nonfinite(uint32_t s16, uint32_t b16) {
-    // from here on values round past the largest
-    constexpr float lim = std::is_same<TA, __half>::value ? 65520.0f : 3.39617752923046e38f;
-    return !(fabsf(fmaf(Act<TA>::to_f((uint16_t)s16), (float)((1 << BITS) - 1), Act<TA>::to_f((uint16_t)b16))) < lim);
+__device__ __forceinline__ float code_value(uint32_t code, uint32_t s16, uint32_t b16) {
+    constexpr float up = RawCode<TA, BITS>::kScale;
+    return fmaf(Act<TA>::to_f((uint16_t)s16) * up, (float)code * (1.0f / up), Act<TA>::to_f((uint16_t)b16));
+}
+// no number, or rounded past the type's largest?
+template <typename TA>
+__device__ __forceinline__ bool past_type(float v) {
+    return !(fabsf(v) < (std::is_same<TA, __half>::value ? 65520.0f : 3.39617752923046e38f));
+}
+// Is a value of the group?  The values lie between the bias (code 0) and the
+// last code's, and where the bias is no number the last is none either.
+template <typename TA, int BITS>
+__device__ __forceinline__ bool group_past_type(uint32_t s16, uint32_t b16) {
+    return past_type<TA>(code_value<TA, BITS>((1u << BITS) - 1u, s16, b16));
 }
 
 int attn_num_sms();

@@ -628,12 +628,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                             if constexpr (Q) {
                                 const uint32_t by = a.c.kv[1][kr * RB + d * BITS / 8];
                                 const uint32_t code = BITS == 8 ? by : by >> (4 * (d & 1)) & 15u;
-                                y = Act<TA>::to_f((uint16_t)code_value<TA, BITS>(code, a.c.scale[1][kr * NG + d / GS],
-                                                                                 a.c.bias[1][kr * NG + d / GS]));
+                                y = code_value<TA, BITS>(code, a.c.scale[1][kr * NG + d / GS], a.c.bias[1][kr * NG + d / GS]);
                             } else {
                                 y = Act<TA>::to_f(reinterpret_cast<const uint16_t *>(a.c.kv[1])[kr * D + d]);
                             }
-                            if (fabsf(y) <= 3.402823466e38f) continue;  // the same for all lanes
+                            if (!past_type<TA>(y)) continue;  // the same for all lanes
+                            y *= INFINITY;
                             const float o = tmem_ld1(tm_o(t) + lanes + d);
                             tmem_st1(tm_o(t) + lanes + d, sees ? o + y : o);
                         }
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) attn_chunk_kernel(const AttnArg
                 for (int g = 0; g < NG; ++g) {
                     const uint32_t x = in_lane ? __byte_perm(sc[g / 2], bi[g / 2], g & 1 ? 0x7632 : 0x5410) : 0u;
                     // in a block that only some rows see, values that are no numbers are taken out
-                    if (which && n.part >= 0) no |= group_nonfinite<TA, BITS>(x & 0xFFFFu, x >> 16);
+                    if (which && n.part >= 0) no |= group_past_type<TA, BITS>(x & 0xFFFFu, x >> 16);
                     spair[lane * NG + g] = make_uint2(Pair<TA>::template scale<BITS>(__byte_perm(x, 0u, 0x1010)),
                                                       __byte_perm(x, 0u, 0x3232));
                 }
