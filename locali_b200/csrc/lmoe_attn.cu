@@ -363,8 +363,9 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             }
                             const uint32_t so = spart + (kt * 16 + 8 * h) * NG * 2 + gi * 2;
                             const float sv = Act<TA>::to_f((uint16_t)lds_u16(so)), bv = Act<TA>::to_f((uint16_t)lds_u16(so + G::SB));
-                            // a scale or bias that is no number (0 times it is none either) makes the key's score none
-                            bf[h] = fmaf(-RC::kOffset * RC::kDown, sv, bv * RC::kDown) + ((sv - sv) + (bv - bv));
+                            // a scale or bias that is no number makes the key's score none: 0 times it is none either
+                            bf[h] = fmaf(bv, RC::kDown, fmaf(bv, 0.0f, sv * 0.0f));
+                            if constexpr (RC::kOffset != 0.0f) bf[h] = fmaf(-RC::kOffset * RC::kDown, sv, bf[h]);
                             sf[h] = sv * (RC::kScale * RC::kDown);
                         }
 #pragma unroll
