@@ -469,8 +469,9 @@ typedef struct lmoe_kv_rows {
  * strides in elements between tokens and between heads, multiples of 8, data
  * 16-byte aligned) into their places, quantising them on the way.  Rows
  * without a place are not written.  No two rows of a call may share a place.
- * workspace: any lmoe workspace (its status word) or NULL; the same for the
- * two calls below. */
+ * workspace: any lmoe workspace (its status word) or NULL, in which case
+ * nothing tells of device errors (a page id out of range, a wait that gave up
+ * and left a result in part); the same for the two calls below. */
 int lmoe_kv_append(const lmoe_kv_cache *cache, const lmoe_kv_rows *rows, const void *k, int64_t k_token_stride,
                    int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
                    void *workspace, void *stream);

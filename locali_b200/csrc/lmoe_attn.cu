@@ -3,10 +3,12 @@
 //
 // out = sum_j softmax_j(scale q . k_j) v_j in one pass over the keys with the
 // running reference (the maximum, shifted: Term in lmoe_attn.cuh) and sum of
-// the softmax.  A tile's keys and values are read once.  On a B200 a 16-bit cache is bound by HBM (128 windowed sequences, 272
-// MB: 55 us, 4.9 of 6.5 TB/s); codes by the instructions that make numbers of
-// them (64 sequences of 4500 on average, 8 bits, 626 MB: 132 us, 4.7 TB/s, two
-// thirds of the issue slots busy; 4 bits, 482 MB: 137 us, 3.5 TB/s).
+// the softmax.  A tile's keys and values are read once.  On a B200 a 16-bit
+// cache is bound by HBM (128 windowed sequences, 272 MB: 54 us, 5.0 of 6.5
+// TB/s); codes by the instructions that make numbers of them (64 sequences of
+// 4500 on average, 8 bits, 626 MB: 134 us, 4.7 TB/s, 64 % of the issue slots
+// busy; 4 bits, 482 MB: 150 us, 3.2 TB/s).  Those are single launches; whole
+// calls back to back, the join among them, take 68, 156 and 145 us.
 //
 // Work.  Tiles are 8 or 16 rows (tokens x query heads of one key/value head);
 // the stream of their key blocks is cut evenly over the launch (Share in
@@ -14,8 +16,13 @@
 // own (KS positions, 4 KB of codes) and streams them through a private ring of
 // shared-memory units with 16-byte cp.async, so warps never wait for one
 // another inside a tile; their results meet once per tile.  Four launch blocks
-// an SM keep 16 warps with two units each in flight (128 KB), and one block's
-// hand-over from tile to tile overlaps the others' streams.
+// an SM keep 16 warps with two units each in flight (128 KB; three blocks where
+// a tile has 16 rows), and one block's hand-over from tile to tile overlaps the
+// others' streams.
+//
+// Registers are short: at heads of 128 the quantised instances spill, up to 114
+// bytes of stores with tiles of 8 rows and 436 with 16 (-Xptxas -v), of which
+// 0.1 % of the executed instructions are left (64 sequences, 8 bits).
 //
 // Arithmetic.  Both products are computed transposed, with the keys (values)
 // as the 16-row operand of mma.m16n8k16 and the tile's 8 rows as its 8
@@ -30,7 +37,8 @@
 // sum(q), so a key is never rounded (rounded to bf16 first, the keys were the
 // largest part of a result's error, 2.9e-3 of 3.9e-3) and a code costs two
 // instructions instead of four.  A constant added to the codes by the cheapest
-// way to make them numbers (128 or 1024) is taken off with the bias.  Values
+// way to make them numbers (128 or 1024) is taken off with the bias (RawCode
+// in lmoe_attn.cuh).  Values
 // are dequantised to the 16-bit type: there a scale belongs to a position of
 // the contraction.
 #include "lmoe_attn.cuh"

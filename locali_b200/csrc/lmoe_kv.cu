@@ -5,9 +5,12 @@
 // thread owns 8 consecutive elements, head_dim / 8 threads a head row, so a
 // group of 32, 64 or 128 elements is 4, 8 or 16 neighbouring lanes and its
 // minimum and maximum are a few shuffles.  Every byte moves once; at 31 k rows
-// of 8 heads of 128, 8-bit groups of 64 (B200): read 47 us, 4.2 TB/s of the
-// 6.5 a copy reaches, append 90 us, 2.2 TB/s and bound by issue (about 200
-// instructions for 8 elements: extremes, the scale's division, exact codes).
+// of 8 heads of 128 (B200, launches timed alone): 16 bits, append and read 49
+// us each, 5.2 TB/s of the 6.5 a copy reaches; 8-bit groups of 64, read 47 us,
+// 4.2 TB/s (a thread's loads are 8 bytes, two in flight), append 90 us, 2.2
+// TB/s and bound by issue (about 200 instructions for 8 elements: extremes, the
+// scale's division, exact codes; 40 to 60 bytes of spills at five blocks an
+// SM); 4 bits, read 49 us, append 95.
 #include "../../include/lmoe.h"
 
 #include <cmath>

@@ -145,7 +145,8 @@ class PagedKVCache:
         self._scratch_bytes: dict[tuple, int] = {}
 
     def check(self) -> None:
-        """Synchronise and raise if a kernel met a page id, length or row start out of range."""
+        """Wait for the current stream and raise if a kernel met a page id, length or row start out of range, or gave up
+        a wait.  Calls on other streams are covered once that stream waits for them."""
         with _on(self.device):
             self.ws.check()
 
@@ -254,7 +255,8 @@ class PagedKVCache:
         ``window`` > 0 a row sees its own and the ``window - 1`` positions
         before it, and the sequence's first ``sinks`` positions; table entries
         of pages that no row sees a position of may hold anything.  A row that
-        sees nothing is zero.  ``out`` must not share memory with q."""
+        sees nothing is zero.  ``out`` must not share memory with q; rows of
+        no sequence are left as ``out`` has them (undefined without it)."""
         _need_cuda(q)
         q = self._heads(q, "q", None)
         n, heads = int(q.shape[0]), int(q.shape[1])
