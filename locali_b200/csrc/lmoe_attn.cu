@@ -38,9 +38,8 @@
 // largest part of a result's error, 2.9e-3 of 3.9e-3) and a code costs two
 // instructions instead of four.  A constant added to the codes by the cheapest
 // way to make them numbers (128 or 1024) is taken off with the bias (RawCode
-// in lmoe_attn.cuh).  Values
-// are dequantised to the 16-bit type: there a scale belongs to a position of
-// the contraction.
+// in lmoe_attn.cuh).  Values are dequantised to the 16-bit type: there a scale
+// belongs to a position of the contraction.
 #include "lmoe_attn.cuh"
 
 namespace lmoe {

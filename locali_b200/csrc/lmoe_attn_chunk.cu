@@ -25,8 +25,7 @@
 // which keeps them half a block apart: one's softmax overlaps the other's
 // MMAs.  Issued as they came, the MMAs of both interleaved and ended together,
 // and the two softmaxes then shared the exponential unit while the tensor pipe
-// waited.  The
-// reference of a row (Term in lmoe_attn.cuh) moves only when a score passes it
+// waited.  The reference of a row (Term in lmoe_attn.cuh) moves only when a score passes it
 // by some powers of two: until then terms grow, which costs nothing in fp32
 // and leaves the sums in tensor memory untouched.
 //
@@ -38,10 +37,11 @@
 // at a head of 128) and beside it the exponentials (one per row and key, 16 a
 // cycle: 2048 cycles too).  Measured on a B200: 2048 new tokens over 32 k
 // cached, 32 query heads on 8, 8-bit codes: 1.15 ms a call behind an idle GPU
-// (905 TFLOP/s, about 4400 cycles a block), 1.26 ms back to back.  What bounds it is the chain of one sub-tile: its softmax
-// (about 2000 cycles, one thread a row), then P V and the next S (1100), then
-// the hand-overs; without the softmax the same launch takes 0.72 ms, without
-// dequantisation or its stores no less than with them.
+// (905 TFLOP/s, about 4400 cycles a block), 1.26 ms back to back.  What bounds
+// it is the chain of one sub-tile: its softmax (about 2000 cycles, one thread a
+// row), then P V and the next S (1100), then the hand-overs; without the
+// softmax the same launch takes 0.72 ms, without dequantisation or its stores
+// no less than with them.
 #include "lmoe_attn.cuh"
 #include "lmoe_tc.cuh"
 
