@@ -8,7 +8,7 @@
 // TB/s); codes by the instructions that make numbers of them (64 sequences of
 // 4500 on average, 8 bits, 626 MB: 134 us, 4.7 TB/s, 64 % of the issue slots
 // busy; 4 bits, 482 MB: 150 us, 3.2 TB/s).  Those are single launches; whole
-// calls back to back, the join among them, take 68, 156 and 145 us.
+// calls back to back, the join among them, take 68, 156 and 143 us.
 //
 // Work.  Tiles are 8 or 16 rows (tokens x query heads of one key/value head);
 // the stream of their key blocks is cut evenly over the launch (Share in
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kRowThreads, NT == 1 ? 4 : 3) attn_rows_kernel
                             // a scale or bias that is no number makes the key's score none: 0 times it is none either
                             bf[h] = fmaf(bv, RC::kDown, fmaf(bv, 0.0f, sv * 0.0f));
                             if constexpr (RC::kOffset != 0.0f) bf[h] = fmaf(-RC::kOffset * RC::kDown, sv, bf[h]);
-                            sf[h] = sv * (RC::kScale * RC::kDown);
+                            sf[h] = sv * (RC::kDown / RC::kUnit);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n)

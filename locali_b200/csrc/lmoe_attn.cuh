@@ -342,19 +342,20 @@ struct Pair<__half> {
     static constexpr uint32_t kExpMask = 0x7C00u;
 };
 
-// Pair j of a word's two halves as an operand without scale and bias: 4-bit
-// codes j = 0..3 and f16 8-bit codes carry kOffset, bf16 8-bit codes are
-// multiplied by 1 / kScale.  Scores are summed times kDown: a bf16 scale of
+// Pair j of a word's two halves as an operand without scale and bias, (code +
+// kOffset) kUnit: what the cheapest way to a number gives (j = 0..3 for 4-bit
+// codes, 0..1 for 8-bit ones).  Scores are summed times kDown: a bf16 scale of
 // 4-bit codes may be 2^125, and 128 of those are no fp32 (8 bits down they
-// are, and the smallest scale and bias stay exact).
+// are, and the smallest scale and bias stay exact; the codes are put there by
+// their exponent, so the scale needs no multiplication).
 template <typename TA, int BITS>
 struct RawCode {
     static constexpr bool kBf = std::is_same<TA, __nv_bfloat16>::value;
     static constexpr float kOffset = kBf ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f;
-    static constexpr float kScale = kBf && BITS == 8 ? 64.0f : 1.0f;
+    static constexpr float kUnit = kBf ? (BITS == 8 ? 1.0f / 64.0f : 1.0f / 256.0f) : 1.0f;
     static constexpr float kDown = kBf && BITS == 4 ? 1.0f / 256.0f : 1.0f;
     __device__ __forceinline__ static uint32_t pair(uint32_t u, int j) {
-        if constexpr (BITS == 4) return and_or(u >> (4 * j), 0x000F000Fu, Act<TA>::kMagic);
+        if constexpr (BITS == 4) return and_or(u >> (4 * j), 0x000F000Fu, kBf ? 0x3F003F00u : 0x64006400u);
         else if constexpr (kBf) return Pair<TA>::mul(j ? __byte_perm(u, 0u, 0x4341) : u & 0x00FF00FFu, 0x7F007F00u);
         else return j ? __byte_perm(u, 0x64646464u, 0x4341) : and_or(u, 0x00FF00FFu, 0x64006400u);
     }
@@ -375,7 +376,7 @@ __device__ __forceinline__ bool nonfinite16(uint32_t x) {
 // for bf16 scales of 8-bit codes from 2^122 on.
 template <typename TA, int BITS>
 __device__ __forceinline__ float code_value(uint32_t code, uint32_t s16, uint32_t b16) {
-    constexpr float up = RawCode<TA, BITS>::kScale;
+    constexpr float up = std::is_same<TA, __nv_bfloat16>::value && BITS == 8 ? 64.0f : 1.0f;
     return fmaf(Act<TA>::to_f((uint16_t)s16) * up, (float)code * (1.0f / up), Act<TA>::to_f((uint16_t)b16));
 }
 // no number, or rounded past the type's largest?
